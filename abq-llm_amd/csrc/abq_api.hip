@@ -127,7 +127,7 @@ static const KernelTable *find_table(const KernelTable *tables, int x_bits, int 
 
 static thread_local int g_last_hip_error = 0;
 
-static abq_status hip_status(hipError_t e)
+abq_status hip_status(hipError_t e)
 {
     if (e == hipSuccess)
         return ABQ_OK;

@@ -1,0 +1,314 @@
+// Causal attention of packed prompts with grouped heads.
+//
+// A workgroup takes a block of one sequence's queries and one head, its four waves 32 (or 64) queries each, and goes over the
+// keys in tiles of 64 tokens with the running maximum and sum of the softmax.  Both products are taken transposed,
+// S^T = K q^T and out^T = V^T P^T (32 x 32 x 16 MFMA): lane (i, h) of the first result holds the scores of query i for tokens
+// 8 j + 4 h .. + 3, which are, eight at a time, an operand of the second product as they are, if the values' tokens
+// come in the same order; so P never leaves its registers, and a query's statistics are two lanes'.  The values are
+// transposed on the way out of LDS (ds_read_b64_tr_b16: four tokens of one element per lane).
+//
+// Tiles of keys and values are loaded straight into LDS, one tile ahead.  A load places a wave's 64 pieces of 16 bytes one
+// behind the other, so the pieces of a row change places by the choice of what each lane loads: keys by the row's number
+// (32 rows of one column of pieces lie in different banks), values by the row modulo 4 (so do four rows of four pieces).
+//
+// P is rounded to the type of the inputs for the second product; its sum is taken in fp32 before that.
+#include "abq_attn.h"
+#include "abq_lds_dma.h"
+
+namespace abq {
+
+namespace {
+
+struct PromptArgs {
+    abq_rows q, k, v, out;
+    const int32_t *q_starts, *k_starts;
+    int heads, kv_heads, seqs, blocks; // blocks: of queries in the longest sequence
+    float scale_log2;
+};
+
+constexpr int kTokens = 64; // of a tile
+
+typedef __attribute__((ext_vector_type(4))) short short4v;
+
+template <int DTYPE> __device__ __forceinline__ float16v mfma_32x32x16(uint4 a, uint4 b, float16v c)
+{
+    if constexpr (DTYPE == ABQ_BF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8v, a), __builtin_bit_cast(bf16x8v, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8v, a), __builtin_bit_cast(half8v, b), c, 0, 0, 0);
+}
+
+// Where piece c of row r of a tile stands in LDS (in pieces of 16 bytes from the row's start)
+template <int D> __device__ __forceinline__ int key_piece(int r, int c) { return c ^ (D == 128 ? r & 15 : r >> 1 & 7); }
+template <int D> __device__ __forceinline__ int value_piece(int r, int c) { return c ^ (D == 128 ? 4 * (r & 3) : 4 * (r >> 1 & 1)); }
+
+template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256) void attn_prompt_kernel(PromptArgs a)
+{
+    constexpr int kBlock = 128 * QT;            // queries of the workgroup
+    constexpr int kPieces = D / 8;              // of a row
+    constexpr int kTile = kTokens * D * 2;      // bytes
+    constexpr int kLoads = kTile / 1024 / 4;    // of a wave per tile
+    __shared__ __align__(1024) uint8_t lds[2][2][kTile];
+    __shared__ int odd_values[4];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ql = lane & 31, half = lane >> 5;
+    // Blocks with the most keys first.  Heads that share keys are kv_heads apart, so with 8 key heads (or a multiple) each
+    // stays with one XCD's L2.
+    const uint32_t per_block = a.heads * a.seqs;
+    const int block = a.blocks - 1 - (int)(blockIdx.x / per_block);
+    const int seq = blockIdx.x % per_block / a.heads, order = blockIdx.x % a.heads;
+    const int kv_head = order % a.kv_heads, head = kv_head * (a.heads / a.kv_heads) + order / a.kv_heads;
+
+    const SeqRows qs = seq_rows(a.q_starts, seq, a.q.rows), ks = seq_rows(a.k_starts, seq, a.k.rows);
+    if (block * kBlock >= qs.count)
+        return;
+    const int ahead = ks.count - qs.count; // query i sees keys up to ahead + i
+    const int first = block * kBlock + wave * 32 * QT; // the wave's first query
+    const int last_key = ahead + min(block * kBlock + kBlock, qs.count) - 1; // seen by the block
+    const int wave_last = ahead + min(first + 32 * QT, qs.count) - 1;        // seen by the wave
+    const int tiles = last_key < 0 ? 0 : last_key / kTokens + 1;
+
+    uint4 q[QT][D / 16];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+        const int64_t row = qs.first + min(first + 32 * qt + ql, qs.count - 1);
+        const uint16_t *src = (const uint16_t *)a.q.data + row * a.q.row_stride + (int64_t)head * a.q.head_stride + 8 * half;
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s)
+            q[qt][s] = *(const uint4 *)(src + 16 * s);
+    }
+    float16v out[QT][D / 32];
+    float m[QT], l[QT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+        m[qt] = -INFINITY;
+        l[qt] = 0;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                out[qt][d][i] = 0;
+    }
+
+    const uint16_t *k_src = (const uint16_t *)a.k.data + (int64_t)kv_head * a.k.head_stride;
+    const uint16_t *v_src = (const uint16_t *)a.v.data + (int64_t)kv_head * a.v.head_stride;
+    const unsigned lds_at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)&lds[0][0][0];
+    auto load_tile = [&](int tile, int buffer) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int piece = (wave * kLoads + i) * 64 + lane, r = piece / kPieces, c = piece % kPieces;
+            const int64_t row = ks.first + min(tile * kTokens + r, ks.count - 1); // (rows behind the last: never seen)
+            lds_dma16(k_src + row * a.k.row_stride + 8 * key_piece<D>(r, c), lds_at + buffer * 2 * kTile + (wave * kLoads + i) * 1024);
+            lds_dma16(v_src + row * a.v.row_stride + 8 * value_piece<D>(r, c), lds_at + (buffer * 2 + 1) * kTile + (wave * kLoads + i) * 1024);
+        }
+    };
+
+    if (tiles > 0)
+        load_tile(0, 0);
+    for (int tile = 0; tile < tiles; ++tile) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (tile + 1 < tiles)
+            load_tile(tile + 1, tile + 1 & 1);
+        const uint8_t *kt = lds[tile & 1][0], *vt = lds[tile & 1][1];
+        const int at = tile * kTokens;
+        const bool masked = at + kTokens - 1 > ahead + block * kBlock;
+        // A weight of 0 does not keep an infinite value out of a product, so tiles that some query sees a part of are
+        // looked through for values that are not finite.
+        bool odd = false;
+        if (masked) {
+            uint32_t found = 0;
+#pragma unroll
+            for (int i = 0; i < kTile / 4096; ++i) {
+                const uint4 w = *(const uint4 *)(vt + (i * 256 + threadIdx.x) * 16);
+                const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) // all ones in the exponent: adding one to it carries
+                    found |= DTYPE == ABQ_BF16 ? (x[j] & 0x7f807f80u) + 0x00800080u : (x[j] & 0x7c007c00u) + 0x04000400u;
+            }
+            if (lane == 0)
+                odd_values[wave] = 0;
+            if (__any((found & 0x80008000u) != 0) && lane == 0)
+                odd_values[wave] = 1;
+            __syncthreads();
+            odd = odd_values[0] | odd_values[1] | odd_values[2] | odd_values[3];
+        }
+        if (at > wave_last)
+            continue;
+
+        // S^T: scores of 2 x 32 tokens
+        float16v score[QT][2];
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    score[qt][tt][i] = 0;
+#pragma unroll
+            for (int s = 0; s < D / 16; ++s) {
+                const int r = 32 * tt + ql;
+                const uint4 k = *(const uint4 *)(kt + r * D * 2 + key_piece<D>(r, 2 * s + half) * 16);
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt)
+                    score[qt][tt] = mfma_32x32x16<DTYPE>(k, q[qt][s], score[qt][tt]);
+            }
+        }
+        uint32_t p[QT][2][8];
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) {
+            const int sees = ahead + first + 32 * qt + ql - at - 4 * half; // tokens up to this one, less what the lane stands for
+            if (masked)
+#pragma unroll
+                for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        score[qt][tt][i] = 32 * tt + 8 * (i / 4) + i % 4 <= sees ? score[qt][tt][i] : -INFINITY;
+            float most = -INFINITY;
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    most = fmaxf(most, score[qt][tt][i]);
+            most = fmaxf(max_across_halves(most), m[qt]);
+            const float base = most == -INFINITY ? 0.f : most * a.scale_log2;
+            if (__any(most > m[qt])) {
+                const float down = __builtin_amdgcn_exp2f(m[qt] * a.scale_log2 - base);
+                l[qt] *= down;
+#pragma unroll
+                for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        out[qt][d][i] *= down;
+            }
+            m[qt] = most;
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    score[qt][tt][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[qt][tt][i], a.scale_log2, -base));
+                    l[qt] += score[qt][tt][i];
+                }
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    p[qt][tt][i] = pack16<DTYPE>(score[qt][tt][2 * i], score[qt][tt][2 * i + 1]);
+        }
+        if (odd) {
+            // token by token, adding only what is seen
+#pragma unroll 1
+            for (int tok = 0; tok < kTokens; ++tok) {
+                const int i = tok % 32 / 8 * 4 + tok % 4;
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt) {
+                    float w = 0;
+#pragma unroll
+                    for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            w = tok / 32 == tt && i == j ? score[qt][tt][j] : w;
+                    w = __shfl(w, ql + 32 * (tok / 4 % 2));
+                    if (at + tok > ahead + first + 32 * qt + ql)
+                        continue;
+#pragma unroll
+                    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const int e = 32 * d + 8 * (j / 4) + 4 * half + j % 4;
+                            const uint16_t x = *(const uint16_t *)(vt + tok * D * 2 + value_piece<D>(tok, e / 8) * 16 + e % 8 * 2);
+                            out[qt][d][j] += w * value16<DTYPE>(x);
+                        }
+                }
+            }
+            continue;
+        }
+        // out^T += V^T P^T, 16 tokens at a time
+        const int tr = (lane & 15) / 4 + 4 * half, tc = 16 * (lane >> 4 & 1) + 4 * (lane & 3); // the lane's row and element
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int d = 0; d < D / 32; ++d) {
+                    uint2 v[2];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const int r = 32 * tt + 16 * s + 8 * x + tr, e = 32 * d + tc;
+                        v[x] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (__attribute__((address_space(3))) short4v *)(vt + r * D * 2 + value_piece<D>(r, e / 8) * 16 + e % 8 * 2)));
+                    }
+#pragma unroll
+                    for (int qt = 0; qt < QT; ++qt)
+                        out[qt][d] = mfma_32x32x16<DTYPE>(uint4{v[0].x, v[0].y, v[1].x, v[1].y},
+                                                          uint4{p[qt][tt][4 * s], p[qt][tt][4 * s + 1], p[qt][tt][4 * s + 2], p[qt][tt][4 * s + 3]}, out[qt][d]);
+                }
+    }
+
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+        const float total = sum_across_halves(l[qt]);
+        const float f = total > 0 ? 1.f / total : total; // (a sum that is not a number stays one)
+        const int i = first + 32 * qt + ql;
+        uint16_t *to = (uint16_t *)a.out.data + (int64_t)(qs.first + i) * a.out.row_stride + (int64_t)head * a.out.head_stride;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                // elements 8 x + 4 h .. + 3 of the lanes h = 0, 1: eight neighbours per lane after an exchange
+                uint32_t x[2][2];
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        x[y][e] = pack16<DTYPE>(out[qt][d][8 * j + 4 * y + 2 * e] * f, out[qt][d][8 * j + 4 * y + 2 * e + 1] * f);
+                const auto r0 = __builtin_amdgcn_permlane32_swap(x[0][0], x[1][0], false, false);
+                const auto r1 = __builtin_amdgcn_permlane32_swap(x[0][1], x[1][1], false, false);
+                if (i < qs.count)
+                    *(uint4 *)(to + 32 * d + 16 * j + 8 * half) = uint4{r0[0], r1[0], r0[1], r1[1]};
+            }
+    }
+}
+
+} // namespace
+
+void plan_attn_prompt(abq_attn_state *st, int most_parts)
+{
+    (void)most_parts;
+    st->block_rows = 128;
+    st->parts = 1;
+}
+
+#define ABQ_PROMPT(T, D_, QT) hipLaunchKernelGGL((attn_prompt_kernel<T, D_, QT>), grid, dim3(256), 0, stream, a)
+#define ABQ_PROMPT_DIM(T)                    \
+    do {                                     \
+        if (st.head_dim == 64)               \
+            ABQ_PROMPT(T, 64, 1);            \
+        else                                 \
+            ABQ_PROMPT(T, 128, 1);           \
+    } while (0)
+
+hipError_t launch_attn_prompt(const abq_attn_state &st, hipStream_t stream)
+{
+    PromptArgs a;
+    a.q = st.q;
+    a.k = st.k;
+    a.v = st.v;
+    a.out = st.out;
+    a.q_starts = st.q_starts;
+    a.k_starts = st.k_starts;
+    a.heads = st.heads;
+    a.kv_heads = st.kv_heads;
+    a.seqs = st.seqs;
+    a.blocks = (st.max_q + st.block_rows - 1) / st.block_rows;
+    a.scale_log2 = st.scale * kLog2e;
+    const dim3 grid((unsigned)((int64_t)a.blocks * st.heads * st.seqs));
+    if (st.dtype == ABQ_BF16)
+        ABQ_PROMPT_DIM(ABQ_BF16);
+    else
+        ABQ_PROMPT_DIM(ABQ_F16);
+    return hipGetLastError();
+}
+
+} // namespace abq

@@ -1,0 +1,546 @@
+// Attention of drafted tokens (ordinary decoding: one) over the quantised, paged cache.
+//
+// The query heads that share a key head and the drafts of a sequence are the rows of one product: row r is draft r / group,
+// head r % group.  With u the stored codes, s and z a token's scale and zero point, and everything in powers of two,
+//     score[t][r] = s_k[t] (u_k[t] . q[r] - z_k[t] sum(q[r])) scale log2(e)
+//     w[t][r]     = 2^(score[t][r] + log2(s_v[t]) - max_t(same))
+//     out[r]      = (sum_t w[t][r] u_v[t] - sum_t w[t][r] z_v[t]) / sum_t (w[t][r] / s_v[t])
+// so codes enter the matrix cores as the whole numbers they are, exact in fp16, and are never scaled one by one: a code costs
+// one half of a byte permute (or mask) and one half of a packed add.  Folding s_v into the exponent keeps the largest weight at
+// 1 whatever the scales are, so that weights rounded to fp16 (11 bits; the one rounding of the sum, as large as that of the
+// result) do not run into its subnormals.  Queries in bf16 become fp16 after a division of each row by a power of two, which
+// loses nothing that a 32-bit sum would keep.
+//
+// Both products are taken transposed, scores^T = K q^T and out^T = V^T w^T (16 x 16 x 32 MFMA), because the result of the
+// first then lies in the registers as the second wants it: lane (r, g) gets the scores of row r for tokens 4 g .. 4 g + 3, and
+// gives the weights of the tokens 4 g .. 4 g + 3 of both halves of a 32-token step as its eight.  The cache keeps four tokens'
+// values beside each other for the same reason.  A wave goes from global memory to registers in 16-byte loads and needs no
+// LDS until its tokens are done.
+//
+// Bound by the cache's bytes.  A sequence's tokens are split over workgroups (parts) until the chip is covered, and inside
+// one over its four waves, step by step; the waves' results are joined in LDS, the parts' by a second launch.
+#include "abq_attn.h"
+
+namespace abq {
+
+namespace {
+
+struct TreeArgs {
+    abq_kv_cache c;
+    abq_rows q, out;
+    const int32_t *page_table, *context, *q_starts;
+    const uint64_t *mask;
+    int heads, group, seqs, max_pages, row_blocks, dtype;
+    int page_shift;
+    float scale_log2;
+    AttnParts parts;
+};
+
+constexpr int kStep = 32;  // tokens of a wave's step
+constexpr int kWaves = 4;
+
+__device__ __forceinline__ half2v half2_bits(uint32_t w) { return __builtin_bit_cast(half2v, w); }
+__device__ __forceinline__ uint32_t bits(half2v h) { return __builtin_bit_cast(uint32_t, h); }
+
+// What a wave reads for one step.  K: per 16 tokens, the lane's bytes of its token's row.  V: per half, four tokens' words.
+template <int BITS, bool ASYM, int D> struct Step {
+    // words of a lane per 16 tokens, of keys and of values
+    static constexpr int kWords = D * BITS / 128;
+    static constexpr int kLoad = kWords < 4 ? kWords : 4; // words per load
+    uint32_t k[2][kWords], v[2][kWords];
+    float ks[2][4], vs[2][4];
+    float kz[ASYM ? 2 : 1][4], vz[ASYM ? 2 : 1][4];
+};
+
+template <int N> __device__ __forceinline__ void load_words(uint32_t *to, const void *from)
+{
+    if constexpr (N == 4) {
+        const uint4 w = *(const uint4 *)from;
+        to[0] = w.x, to[1] = w.y, to[2] = w.z, to[3] = w.w;
+    } else {
+        const uint2 w = *(const uint2 *)from;
+        to[0] = w.x, to[1] = w.y;
+    }
+}
+__device__ __forceinline__ void load_floats(float *to, const float *from)
+{
+    const float4 w = *(const float4 *)from;
+    to[0] = w.x, to[1] = w.y, to[2] = w.z, to[3] = w.w;
+}
+
+// `seen`: bit h is cleared if half h lies on a page outside the cache
+template <int BITS, bool ASYM, int D>
+__device__ __forceinline__ void load_step(Step<BITS, ASYM, D> &s, const TreeArgs &a, const int32_t *pages, int last_page, int head, int at, int lane,
+                                          uint32_t *seen)
+{
+    using S = Step<BITS, ASYM, D>;
+    constexpr int R = D * BITS / 8;
+    const int t = lane & 15, g = lane >> 4;
+    *seen = 3;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int pos = at + 16 * h;
+        int page = pages[min(pos >> a.page_shift, last_page)];
+        if ((uint32_t)page >= (uint32_t)a.c.num_pages) {
+            page = 0;
+            *seen &= ~(1u << h);
+        }
+        const int in_page = pos & (a.c.page_size - 1);
+        const int64_t row = ((int64_t)page * a.c.kv_heads + head) * a.c.page_size;
+        const uint8_t *k = (const uint8_t *)a.c.k_codes + (row + in_page + t) * R;
+        const uint8_t *v = (const uint8_t *)a.c.v_codes + (row + in_page + 4 * g) * R;
+#pragma unroll
+        for (int l = 0; l < S::kWords / S::kLoad; ++l) {
+            load_words<S::kLoad>(&s.k[h][l * S::kLoad], k + l * 64 + g * 4 * S::kLoad);
+            load_words<S::kLoad>(&s.v[h][l * S::kLoad], v + l * 256 + t * 4 * S::kLoad);
+        }
+        const int64_t at_scale = (ASYM ? 2 * row : row) + in_page + 4 * g;
+        load_floats(s.ks[h], a.c.k_scales + at_scale);
+        load_floats(s.vs[h], a.c.v_scales + at_scale);
+        if (ASYM) {
+            load_floats(s.kz[h], a.c.k_scales + at_scale + a.c.page_size);
+            load_floats(s.vz[h], a.c.v_scales + at_scale + a.c.page_size);
+        }
+    }
+}
+
+// Four codes of a word as whole numbers less half the range, in two pairs: 1024 + u is the fp16 number 0x6400 | u.
+__device__ __forceinline__ void four_codes(uint32_t w, uint32_t *lo, uint32_t *hi)
+{
+    const half2v off = {(_Float16)1152, (_Float16)1152};
+    *lo = bits(half2_bits(__builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) - off);
+    *hi = bits(half2_bits(__builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) - off);
+}
+// Eight 4-bit codes of a word: nibbles (0, 4), (1, 5), (2, 6), (3, 7).  A nibble in bits 4 - 7 stands for 16 times its value.
+__device__ __forceinline__ void eight_codes(uint32_t w, uint32_t *out)
+{
+    const half2v off = {(_Float16)1032, (_Float16)1032}, part = {(_Float16)0.0625f, (_Float16)0.0625f}, off16 = {(_Float16)72, (_Float16)72};
+    const uint32_t w8 = w >> 8;
+    out[0] = bits(half2_bits((w & 0x000f000fu) | 0x64006400u) - off);
+    out[1] = bits(half2_bits((w & 0x00f000f0u) | 0x64006400u) * part - off16);
+    out[2] = bits(half2_bits((w8 & 0x000f000fu) | 0x64006400u) - off);
+    out[3] = bits(half2_bits((w8 & 0x00f000f0u) | 0x64006400u) * part - off16);
+}
+
+__device__ __forceinline__ half8v half8_bits(const uint32_t *w)
+{
+    const uint4 x = {w[0], w[1], w[2], w[3]};
+    return __builtin_bit_cast(half8v, x);
+}
+
+// A lane's 8-element pieces of the queries: piece ks of D / 32, in the order of the keys' bytes
+template <int BITS, int D> __device__ __forceinline__ int query_offset(int ks, int g)
+{
+    constexpr int kPieces = BITS == 8 ? 2 : (D == 128 ? 4 : 2); // pieces per load of a lane
+    return (ks / kPieces) * (32 * kPieces) + g * 8 * kPieces + (ks % kPieces) * 8;
+}
+
+template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(256) void attn_tree_kernel(TreeArgs a)
+{
+    using S = Step<BITS, ASYM, D>;
+    constexpr int kTiles = D / 16; // 16 x 16 tiles of out^T
+    constexpr int kPad = D + 4;
+    __shared__ __align__(16) float sums[kWaves][16][kPad];
+    __shared__ float stat_m[kWaves][16 * RT], stat_l[kWaves][16 * RT], stat_z[kWaves][16 * RT];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int t = lane & 15, g = lane >> 4;
+    // Workgroups go round the eight XCDs: those that read the same tokens (other rows of them) are eight apart, on one L2.
+    const uint32_t round = 8 * a.row_blocks, in_round = blockIdx.x % round;
+    const uint32_t unit = blockIdx.x / round * 8 + in_round % 8;
+    const int row_block = in_round / 8;
+    if (unit >= (uint32_t)a.seqs * a.c.kv_heads * a.parts.parts)
+        return;
+    const int part = unit % a.parts.parts, head = unit / a.parts.parts % a.c.kv_heads, seq = unit / a.parts.parts / a.c.kv_heads;
+
+    const SeqRows own = seq_rows(a.q_starts, seq, a.q.rows);
+    const int n = min(own.count, 64);
+    const int rows = n * a.group, row0 = row_block * 16 * RT;
+    if (row0 >= rows)
+        return;
+    const int64_t places = (int64_t)a.max_pages << a.page_shift;
+    const int context = (int)min((int64_t)max(a.context[seq], 0), places);
+    const int len = (int)min((int64_t)context + n, places);
+    const int32_t *pages = a.page_table + (int64_t)seq * a.max_pages;
+    const int last_page = (len - 1) >> a.page_shift; // (len is 0 only without steps)
+
+    // the queries, and what turns their products into exponents of 2
+    half8v q[RT][D / 32];
+    float factor[RT], qsum[RT];
+    uint64_t sees[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int row = min(row0 + 16 * rt + t, rows - 1), draft = row / a.group;
+        const uint16_t *src = (const uint16_t *)a.q.data + (int64_t)(own.first + draft) * a.q.row_stride + (int64_t)(head * a.group + row % a.group) * a.q.head_stride;
+        sees[rt] = a.mask ? a.mask[own.first + draft] : ~0ull >> (63 - draft);
+        factor[rt] = a.scale_log2;
+        float sum = 0;
+        uint4 w[D / 32];
+#pragma unroll
+        for (int ks = 0; ks < D / 32; ++ks)
+            w[ks] = *(const uint4 *)(src + query_offset<BITS, D>(ks, g));
+        if (a.dtype == ABQ_BF16) {
+            float most = 0;
+#pragma unroll
+            for (int ks = 0; ks < D / 32; ++ks) {
+                const uint32_t x[4] = {w[ks].x, w[ks].y, w[ks].z, w[ks].w};
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    most = fmaxf(most, fabsf(bf16_value(x[i / 2] >> (16 * (i & 1)) & 0xffff)));
+            }
+            most = max_across_quarters(most);
+            const int e = most > 0 && most < INFINITY ? 14 - (int)(__builtin_bit_cast(uint32_t, most) >> 23) + 127 : 0; // the largest becomes [2^14, 2^15)
+            factor[rt] = ldexpf(factor[rt], -e);
+#pragma unroll
+            for (int ks = 0; ks < D / 32; ++ks) {
+                const uint32_t x[4] = {w[ks].x, w[ks].y, w[ks].z, w[ks].w};
+                uint32_t y[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    y[i] = pack16<ABQ_F16>(ldexpf(bf16_value(x[i] & 0xffff), e), ldexpf(bf16_value(x[i] >> 16), e));
+                q[rt][ks] = half8_bits(y);
+            }
+        } else
+#pragma unroll
+            for (int ks = 0; ks < D / 32; ++ks)
+                q[rt][ks] = __builtin_bit_cast(half8v, w[ks]);
+#pragma unroll
+        for (int ks = 0; ks < D / 32; ++ks)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                sum += (float)q[rt][ks][i];
+        qsum[rt] = ASYM ? sum_across_quarters(sum) : 0;
+    }
+
+    float4v out[RT][kTiles];
+    float m[RT], l[RT], z[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        m[rt] = -INFINITY;
+        l[rt] = z[rt] = 0;
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i)
+            out[rt][i] = float4v{0, 0, 0, 0};
+    }
+
+    const int steps = (len + kStep - 1) / kStep;
+    const int step0 = (int)((int64_t)steps * part / a.parts.parts) + wave, step1 = (int)((int64_t)steps * (part + 1) / a.parts.parts);
+    S next;
+    uint32_t next_seen = 0;
+    if (step0 < step1)
+        load_step<BITS, ASYM, D>(next, a, pages, last_page, head, step0 * kStep, lane, &next_seen);
+    for (int step = step0; step < step1; step += kWaves) {
+        S s = next;
+        const uint32_t seen = next_seen;
+        if (step + kWaves < step1)
+            load_step<BITS, ASYM, D>(next, a, pages, last_page, head, (step + kWaves) * kStep, lane, &next_seen);
+
+        // scores
+        float score[RT][2][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float4v acc[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+                acc[rt] = float4v{0, 0, 0, 0};
+#pragma unroll
+            for (int ks = 0; ks < D / 32; ++ks) {
+                uint32_t w[4];
+                if (BITS == 8) {
+                    four_codes(s.k[h][2 * ks], &w[0], &w[1]);
+                    four_codes(s.k[h][2 * ks + 1], &w[2], &w[3]);
+                } else
+                    eight_codes(s.k[h][ks], w);
+                const half8v k = half8_bits(w);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+                    acc[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[rt][ks], acc[rt], 0, 0, 0);
+            }
+            // (codes are less half their range here, and so is the zero point)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    score[rt][h][i] = (ASYM ? acc[rt][i] - (s.kz[ASYM ? h : 0][i] - (float)(1 << (BITS - 1))) * qsum[rt] : acc[rt][i]) * (s.ks[h][i] * factor[rt]);
+        }
+        // what no row sees holds anything: its scales are replaced
+        const int at = step * kStep;
+        if (at + kStep > context || seen != 3) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int pos = at + 16 * h + 4 * g + i;
+                    const bool there = pos < len && (seen >> h & 1);
+                    s.vs[h][i] = there ? s.vs[h][i] : 1.f;
+                    if (ASYM)
+                        s.vz[ASYM ? h : 0][i] = there ? s.vz[ASYM ? h : 0][i] : 0.f;
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt)
+                        score[rt][h][i] = there && (pos < context || (sees[rt] >> ((pos - context) & 63) & 1)) ? score[rt][h][i] : -INFINITY;
+                }
+        }
+        float v_log[2][4], v_recip[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v_log[h][i] = __builtin_amdgcn_logf(s.vs[h][i]);
+                v_recip[h][i] = __builtin_amdgcn_rcpf(s.vs[h][i]);
+            }
+        // weights
+        half8v w[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            float most = -INFINITY;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    score[rt][h][i] += v_log[h][i];
+                    most = fmaxf(most, score[rt][h][i]);
+                }
+            most = fmaxf(max_across_quarters(most), m[rt]);
+            const float base = most == -INFINITY ? 0.f : most;
+            if (__any(most > m[rt])) {
+                const float down = __builtin_amdgcn_exp2f(m[rt] - base);
+                l[rt] *= down;
+                z[rt] *= down;
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i)
+                    out[rt][i] *= down;
+            }
+            m[rt] = most;
+            uint32_t pair[4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float x[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[i] = __builtin_amdgcn_exp2f(score[rt][h][i] - base);
+                    l[rt] += x[i] * v_recip[h][i];
+                }
+                pair[2 * h] = pack16<ABQ_F16>(x[0], x[1]);
+                pair[2 * h + 1] = pack16<ABQ_F16>(x[2], x[3]);
+                if (ASYM) // with the weights as they are multiplied, so that the two sums' difference has no error of its own
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        z[rt] += f16_value(pair[2 * h + i / 2] >> (16 * (i & 1)) & 0xffff) * (s.vz[ASYM ? h : 0][i] - (float)(1 << (BITS - 1)));
+            }
+            w[rt] = half8_bits(pair);
+        }
+        // out^T += V^T w^T.  8 bits: word j of load i is element 64 i + 4 t + j; 4 bits: two elements, D / 2 apart
+#pragma unroll
+        for (int j = 0; j < S::kWords; ++j) {
+            if (BITS == 8) {
+                uint32_t x[4];
+                four_codes(s.v[0][j], &x[0], &x[1]);
+                four_codes(s.v[1][j], &x[2], &x[3]);
+                const half8v v = half8_bits(x);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+                    out[rt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[rt], out[rt][j], 0, 0, 0);
+            } else {
+                uint32_t x[4], y[4];
+                eight_codes(s.v[0][j], x);
+                eight_codes(s.v[1][j], y);
+                const uint32_t low[4] = {x[0], x[2], y[0], y[2]}, high[4] = {x[1], x[3], y[1], y[3]};
+                const half8v v0 = half8_bits(low), v1 = half8_bits(high);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    out[rt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, w[rt], out[rt][j], 0, 0, 0);
+                    out[rt][j + S::kWords] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, w[rt], out[rt][j + S::kWords], 0, 0, 0);
+                }
+            }
+        }
+    }
+
+    // the waves' results joined
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const float total = sum_across_quarters(l[rt]), zeros = ASYM ? sum_across_quarters(z[rt]) : 0;
+        if (g == 0) {
+            stat_m[wave][16 * rt + t] = m[rt];
+            stat_l[wave][16 * rt + t] = total;
+            stat_z[wave][16 * rt + t] = zeros;
+        }
+    }
+    constexpr int kSpan = BITS == 8 ? 4 : S::kWords; // neighbouring elements that tiles j, j + 1 .. hold
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kTiles; j += kSpan)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < kSpan; ++e)
+                    sums[wave][t][j * 16 + (4 * g + i) * kSpan + e] = out[rt][j + e][i];
+        __syncthreads();
+        constexpr int kEach = D / 16;
+        const int r = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * kEach, row = row0 + 16 * rt + r;
+        float most = -INFINITY, total = 0, acc[kEach];
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w)
+            most = fmaxf(most, stat_m[w][16 * rt + r]);
+        const float base = most == -INFINITY ? 0.f : most;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e)
+            acc[e] = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float f = __builtin_amdgcn_exp2f(stat_m[w][16 * rt + r] - base);
+            total += f * stat_l[w][16 * rt + r];
+#pragma unroll
+            for (int e = 0; e < kEach; ++e)
+                acc[e] += f * (sums[w][r][d0 + e] - (ASYM ? stat_z[w][16 * rt + r] : 0.f));
+        }
+        if (row < rows) {
+            const int64_t q_row = own.first + row / a.group;
+            const int q_head = head * a.group + row % a.group;
+            if (a.parts.parts > 1) {
+                const int64_t at = (q_row * a.heads + q_head) * a.parts.parts + part;
+                float *to = a.parts.sums + at * D + d0;
+#pragma unroll
+                for (int e = 0; e < kEach; e += 4)
+                    *(float4 *)(to + e) = float4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
+                if ((threadIdx.x & 15) == 0)
+                    a.parts.stats[at] = float2{most, total};
+            } else {
+                const float f = total > 0 ? 1.f / total : total; // (a sum that is not a number stays one)
+                uint16_t *to = (uint16_t *)a.out.data + q_row * a.out.row_stride + (int64_t)q_head * a.out.head_stride + d0;
+                uint32_t x[kEach / 2];
+#pragma unroll
+                for (int e = 0; e < kEach / 2; ++e)
+                    x[e] = a.dtype == ABQ_BF16 ? pack16<ABQ_BF16>(acc[2 * e] * f, acc[2 * e + 1] * f) : pack16<ABQ_F16>(acc[2 * e] * f, acc[2 * e + 1] * f);
+                if constexpr (kEach == 8)
+                    *(uint4 *)to = uint4{x[0], x[1], x[2], x[3]};
+                else
+                    *(uint2 *)to = uint2{x[0], x[1]};
+            }
+        }
+    }
+}
+
+// The parts of one query row and head per wave: D / 64 elements a lane
+struct JoinArgs {
+    abq_rows out;
+    AttnParts parts;
+    const int32_t *q_starts;
+    int seqs, max_q, heads, dtype;
+};
+
+template <int D> __global__ __launch_bounds__(256) void attn_join_kernel(JoinArgs a)
+{
+    const int lane = threadIdx.x & 63;
+    const uint32_t unit = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int head = unit % a.heads, draft = unit / a.heads % a.max_q, seq = unit / a.heads / a.max_q;
+    if (seq >= a.seqs)
+        return;
+    const SeqRows own = seq_rows(a.q_starts, seq, a.out.rows);
+    if (draft >= own.count)
+        return;
+    const int64_t row = own.first + draft, at = (row * a.heads + head) * a.parts.parts;
+    float most = -INFINITY;
+    for (int p = lane; p < a.parts.parts; p += 64)
+        most = fmaxf(most, a.parts.stats[at + p].x);
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2)
+        most = fmaxf(most, __shfl_xor(most, o));
+    const float base = most == -INFINITY ? 0.f : most;
+    constexpr int kEach = D / 64;
+    float total = 0, acc[kEach] = {};
+    for (int p = 0; p < a.parts.parts; ++p) {
+        const float2 st = a.parts.stats[at + p];
+        const float f = __builtin_amdgcn_exp2f(st.x - base);
+        total += f * st.y;
+        const float *from = a.parts.sums + (at + p) * D + lane * kEach;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e)
+            acc[e] += f * from[e];
+    }
+    const float f = total > 0 ? 1.f / total : total;
+    uint16_t *to = (uint16_t *)a.out.data + row * a.out.row_stride + (int64_t)head * a.out.head_stride + lane * kEach;
+    const uint32_t x = a.dtype == ABQ_BF16 ? pack16<ABQ_BF16>(acc[0] * f, acc[kEach - 1] * f) : pack16<ABQ_F16>(acc[0] * f, acc[kEach - 1] * f);
+    if (kEach == 2)
+        *(uint32_t *)to = x;
+    else
+        *to = (uint16_t)x;
+}
+
+} // namespace
+
+hipError_t launch_attn_join(const abq_attn_state &st, hipStream_t stream)
+{
+    const JoinArgs a = {st.out, attn_parts(st), st.q_starts, st.seqs, st.max_q, st.heads, st.dtype};
+    const dim3 grid((unsigned)(((int64_t)st.seqs * st.max_q * st.heads + 3) / 4));
+    if (st.head_dim == 64)
+        hipLaunchKernelGGL(attn_join_kernel<64>, grid, dim3(256), 0, stream, a);
+    else
+        hipLaunchKernelGGL(attn_join_kernel<128>, grid, dim3(256), 0, stream, a);
+    return hipGetLastError();
+}
+
+void plan_attn_tree(abq_attn_state *st, int most_parts)
+{
+    const int rows = st->max_q * (st->heads / st->kv_heads);
+    st->block_rows = rows <= 16 ? 16 : 32;
+    const int64_t units = (int64_t)st->seqs * st->kv_heads * ((rows + st->block_rows - 1) / st->block_rows);
+    const int64_t steps = ((int64_t)st->max_k + kStep - 1) / kStep;
+    int64_t parts = units > 0 ? (1024 + units - 1) / units : 1;
+    parts = parts < steps / kWaves ? parts : steps / kWaves;
+    parts = parts < most_parts ? parts : most_parts;
+    st->parts = parts < 1 ? 1 : (int)parts;
+}
+
+#define ABQ_TREE(B, A, D_, RT_) hipLaunchKernelGGL((attn_tree_kernel<B, A, D_, RT_>), grid, dim3(256), 0, stream, a)
+#define ABQ_TREE_ROWS(B, A, D_)           \
+    do {                                  \
+        if (st.block_rows == 16)          \
+            ABQ_TREE(B, A, D_, 1);        \
+        else                              \
+            ABQ_TREE(B, A, D_, 2);        \
+    } while (0)
+#define ABQ_TREE_DIM(B, A)                \
+    do {                                  \
+        if (st.head_dim == 64)            \
+            ABQ_TREE_ROWS(B, A, 64);      \
+        else                              \
+            ABQ_TREE_ROWS(B, A, 128);     \
+    } while (0)
+
+hipError_t launch_attn_tree(const abq_attn_state &st, hipStream_t stream)
+{
+    TreeArgs a;
+    a.c = st.cache;
+    a.q = st.q;
+    a.out = st.out;
+    a.page_table = st.page_table;
+    a.context = st.context;
+    a.q_starts = st.q_starts;
+    a.mask = st.mask;
+    a.heads = st.heads;
+    a.group = st.heads / st.kv_heads;
+    a.seqs = st.seqs;
+    a.max_pages = st.max_pages;
+    a.row_blocks = (st.max_q * a.group + st.block_rows - 1) / st.block_rows;
+    a.dtype = st.dtype;
+    a.page_shift = __builtin_ctz((unsigned)st.cache.page_size);
+    a.scale_log2 = st.scale * kLog2e;
+    a.parts = attn_parts(st);
+    const int64_t units = (int64_t)st.seqs * st.kv_heads * st.parts;
+    const dim3 grid((unsigned)((units + 7) / 8 * 8 * a.row_blocks));
+    if (st.cache.bits == 8) {
+        if (st.cache.symmetric)
+            ABQ_TREE_DIM(8, false);
+        else
+            ABQ_TREE_DIM(8, true);
+    } else if (st.cache.symmetric)
+        ABQ_TREE_DIM(4, false);
+    else
+        ABQ_TREE_DIM(4, true);
+    const hipError_t e = hipGetLastError();
+    return e != hipSuccess || st.parts < 2 ? e : launch_attn_join(st, stream);
+}
+
+} // namespace abq

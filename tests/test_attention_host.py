@@ -1,0 +1,138 @@
+"""Host side of attention on the quantised cache: symbols, structures, refusals, and how work is laid out.  No GPU."""
+import ctypes
+import os
+import re
+import subprocess
+
+import pytest
+
+pytest.importorskip("torch")
+
+from attention_reference import load_abq_attention  # noqa: E402
+from conftest import ROOT  # noqa: E402
+
+
+@pytest.fixture(scope="module")
+def attn():
+    return load_abq_attention()
+
+
+def test_library_exports_every_declared_symbol(attn):
+    header = open(os.path.join(ROOT, "include", "abq_attention.h")).read()
+    declared = set(re.findall(r"^(?:abq_status|size_t)\s+(abq_\w+)\(", header, re.M))
+    assert declared == set(attn.EXPORTED)
+    for name in attn.EXPORTED:
+        getattr(attn.lib(), name)
+
+
+def test_structures_match_the_header(attn, tmp_path):
+    src = '#include "abq_attention.h"\n#include <stdio.h>\n#include <stddef.h>\nint main(){printf("%zu %zu %zu %zu %zu %zu", sizeof(abq_rows), ' \
+          'sizeof(abq_kv_cache), sizeof(abq_attn_state), offsetof(abq_attn_state, q), offsetof(abq_attn_state, mask), ' \
+          'offsetof(abq_attn_state, workspace));return 0;}'
+    exe = str(tmp_path / "sizes")
+    subprocess.run(["gcc", "-x", "c", "-I" + os.path.join(ROOT, "include"), "-o", exe, "-"], input=src.encode(), check=True)
+    want = [int(x) for x in subprocess.check_output([exe]).split()]
+    assert want == [ctypes.sizeof(attn.Rows), ctypes.sizeof(attn.KvCacheDesc), ctypes.sizeof(attn.AttnState), attn.AttnState.q.offset,
+                    attn.AttnState.mask.offset, attn.AttnState.workspace.offset]
+
+
+A = 0x10000  # an address no call may reach: every check comes before
+
+
+def cache_desc(attn, **kw):
+    d = dict(bits=8, symmetric=1, kv_heads=2, head_dim=128, page_size=64, num_pages=10, k_codes=A, v_codes=2 * A, k_scales=3 * A, v_scales=4 * A)
+    d.update(kw)
+    return attn.KvCacheDesc(*d.values())
+
+
+def test_cache_sizes(attn):
+    L = attn.lib()
+    for kw, codes, scales in [({}, 10 * 64 * 2 * 128, 10 * 64 * 2 * 4), ({"bits": 4, "symmetric": 0}, 10 * 64 * 2 * 64, 10 * 64 * 2 * 8),
+                              ({"head_dim": 64, "page_size": 16, "kv_heads": 7}, 10 * 16 * 7 * 64, 10 * 16 * 7 * 4),
+                              ({"num_pages": 1 << 24, "kv_heads": 40}, (1 << 30) * 40 * 128, (1 << 30) * 40 * 4),
+                              ({"bits": 5}, 0, 0), ({"head_dim": 96}, 0, 0), ({"page_size": 8}, 0, 0), ({"page_size": 48}, 0, 0), ({"page_size": 8192}, 0, 0),
+                              ({"num_pages": 0}, 0, 0), ({"kv_heads": -1}, 0, 0), ({"num_pages": 1 << 25}, 0, 0)]:
+        d = cache_desc(attn, **kw)
+        assert (L.abq_kv_codes_bytes(ctypes.byref(d)), L.abq_kv_scales_bytes(ctypes.byref(d))) == (codes, scales), kw
+    assert L.abq_kv_codes_bytes(None) == 0
+    with pytest.raises(ValueError):
+        attn.KvCache(3, 20, 2, 128, device="cpu")
+
+
+def rows(attn, **kw):
+    d = dict(data=8 * A, rows=12, row_stride=256, head_stride=128)
+    d.update(kw)
+    return attn.Rows(*d.values())
+
+
+BAD_ROWS = [{"data": None}, {"data": 8 * A + 8}, {"rows": -1}, {"rows": 11}, {"row_stride": 255}, {"head_stride": 130}, {"head_stride": 64}, {"row_stride": -256}]
+
+
+def test_cache_calls_are_refused(attn):
+    L, ok = attn.lib(), attn.abq_gemm
+    for fn in (L.abq_kv_append, L.abq_kv_read):
+        def call(c={}, k={}, v={}, dtype=0, slots=5 * A):
+            return fn(ctypes.byref(cache_desc(attn, **c)), ctypes.byref(rows(attn, **k)), ctypes.byref(rows(attn, **v)), dtype, slots, None)
+        for c in ({"bits": 3}, {"bits": 16}, {"head_dim": 80}):
+            assert call(c=c) == ok.ABQ_ERR_UNSUPPORTED, c
+        for c in ({"page_size": 20}, {"num_pages": 0}, {"kv_heads": 0}, {"k_codes": None}, {"v_codes": A + 4}, {"k_scales": None}, {"v_scales": A + 8}):
+            assert call(c=c) == ok.ABQ_ERR_INVALID_ARG, c
+        for bad in BAD_ROWS:
+            assert call(v=bad) == ok.ABQ_ERR_INVALID_ARG, bad
+            if "rows" not in bad:
+                assert call(k=bad) == ok.ABQ_ERR_INVALID_ARG, bad
+        assert call(dtype=2) == ok.ABQ_ERR_INVALID_ARG and call(slots=None) == ok.ABQ_ERR_INVALID_ARG
+        assert call(k={"rows": 1 << 31}, v={"rows": 1 << 31}) == ok.ABQ_ERR_TOO_LARGE
+        assert call(k={"rows": 0}, v={"rows": 0}, slots=None) == ok.ABQ_OK  # nothing to do: no launch
+        assert fn(None, ctypes.byref(rows(attn)), ctypes.byref(rows(attn)), 0, A, None) == ok.ABQ_ERR_INVALID_ARG
+        assert fn(ctypes.byref(cache_desc(attn)), None, ctypes.byref(rows(attn)), 0, A, None) == ok.ABQ_ERR_INVALID_ARG
+
+
+def prompt(attn, q={}, k={}, v={}, out={}, dtype=0, heads=2, kv_heads=2, head_dim=128, q_starts=A, k_starts=A, seqs=2, max_q=10, max_k=10, scale=0.1):
+    st = attn.AttnState()
+    return attn.lib().abq_attn_prompt_init(*[ctypes.byref(rows(attn, **r)) for r in (q, k, v, out)], dtype, heads, kv_heads, head_dim, q_starts, k_starts,
+                                           seqs, max_q, max_k, scale, ctypes.byref(st)), st
+
+
+def tree(attn, cache={}, q={}, out={}, dtype=0, heads=2, page_table=A, max_pages=4, context=A, q_starts=A, mask=A, seqs=2, max_q=10, max_context=100, scale=0.1):
+    st = attn.AttnState()
+    return attn.lib().abq_attn_tree_init(ctypes.byref(cache_desc(attn, **cache)), ctypes.byref(rows(attn, **q)), ctypes.byref(rows(attn, **out)), dtype, heads,
+                                         page_table, max_pages, context, q_starts, mask, seqs, max_q, max_context, scale, ctypes.byref(st)), st
+
+
+def test_attention_calls_are_refused(attn):
+    ok = attn.abq_gemm
+    common = [{"dtype": 2}, {"dtype": -1}, {"heads": 0}, {"heads": 3}, {"q_starts": None}, {"seqs": 0}, {"max_q": 0}, {"scale": 0.0}, {"scale": -1.0},
+              {"scale": float("nan")}, {"scale": float("inf")}] + [{"out": b} for b in BAD_ROWS] + [{"q": b} for b in BAD_ROWS]
+    for kw in common + [{"kv_heads": 0}, {"max_k": 0}, {"k_starts": None, "k": {"rows": 13}, "v": {"rows": 13}}] + [{"v": b} for b in BAD_ROWS]:
+        assert prompt(attn, **kw)[0] == ok.ABQ_ERR_INVALID_ARG and not prompt(attn, **kw)[1].init_success, kw
+    for kw in common + [{"page_table": None}, {"context": None}, {"max_pages": 0}, {"max_context": -1}, {"cache": {"k_codes": None}}]:
+        assert tree(attn, **kw)[0] == ok.ABQ_ERR_INVALID_ARG and not tree(attn, **kw)[1].init_success, kw
+    assert prompt(attn, head_dim=96)[0] == ok.ABQ_ERR_UNSUPPORTED and tree(attn, cache={"bits": 2})[0] == ok.ABQ_ERR_UNSUPPORTED
+    assert tree(attn, max_q=65)[0] == ok.ABQ_ERR_TOO_LARGE and tree(attn, max_pages=1 << 26)[0] == ok.ABQ_ERR_TOO_LARGE
+    assert prompt(attn, max_q=2 ** 31 - 1, seqs=100000)[0] == ok.ABQ_ERR_TOO_LARGE
+    assert tree(attn, max_q=64, seqs=2 ** 31 - 1)[0] == ok.ABQ_ERR_TOO_LARGE
+    L, st = attn.lib(), attn.AttnState()
+    assert L.abq_attn_exec(ctypes.byref(st), None) == ok.ABQ_ERR_NOT_INITIALIZED and L.abq_attn_exec(None, None) == ok.ABQ_ERR_INVALID_ARG
+    assert L.abq_attn_set_workspace(ctypes.byref(st), A, 100) == ok.ABQ_ERR_NOT_INITIALIZED and L.abq_attn_workspace_bytes(ctypes.byref(st)) == 0
+    assert L.abq_attn_prompt_init(None, None, None, None, 0, 1, 1, 64, None, None, 1, 1, 1, 1.0, None) == ok.ABQ_ERR_INVALID_ARG
+    s, st = tree(attn)
+    assert s == ok.ABQ_OK and st.init_success
+    assert L.abq_attn_set_workspace(ctypes.byref(st), A + 8, 100) == ok.ABQ_ERR_INVALID_ARG
+    assert L.abq_attn_set_workspace(ctypes.byref(st), None, 100) == ok.ABQ_ERR_INVALID_ARG
+    s, st = tree(attn, q={"rows": 0}, out={"rows": 0})
+    assert s == ok.ABQ_OK and L.abq_attn_exec(ctypes.byref(st), None) == ok.ABQ_OK  # no rows: no launch
+
+
+def test_parts_follow_the_workspace(attn):
+    L = attn.lib()
+    s, st = tree(attn, max_q=1, max_context=30000, max_pages=600)
+    need = L.abq_attn_workspace_bytes(ctypes.byref(st))
+    assert st.parts == 1 and need > 0
+    assert L.abq_attn_set_workspace(ctypes.byref(st), A, need) == 0 and st.parts > 1
+    per_part = 12 * 2 * (128 + 2) * 4
+    assert need == st.parts * per_part
+    for parts in (1, 2, 3):
+        assert L.abq_attn_set_workspace(ctypes.byref(st), A, parts * per_part + 5) == 0 and st.parts == parts
+    assert L.abq_attn_set_workspace(ctypes.byref(st), None, 0) == 0 and st.parts == 1
+    assert L.abq_attn_workspace_bytes(ctypes.byref(st)) == need  # what it would take is not what it has
