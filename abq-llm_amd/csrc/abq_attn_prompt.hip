@@ -42,13 +42,13 @@ template <int DTYPE> __device__ __forceinline__ float16v mfma_32x32x16(uint4 a, 
 template <int D> __device__ __forceinline__ int key_piece(int r, int c) { return c ^ (D == 128 ? r & 15 : r >> 1 & 7); }
 template <int D> __device__ __forceinline__ int value_piece(int r, int c) { return c ^ (D == 128 ? 4 * (r & 3) : 4 * (r >> 1 & 1)); }
 
-template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256) void attn_prompt_kernel(PromptArgs a)
+template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256, 3 - QT) void attn_prompt_kernel(PromptArgs a)
 {
     constexpr int kBlock = 128 * QT;            // queries of the workgroup
     constexpr int kPieces = D / 8;              // of a row
     constexpr int kTile = kTokens * D * 2;      // bytes
     constexpr int kLoads = kTile / 1024 / 4;    // of a wave per tile
-    __shared__ __align__(1024) uint8_t lds[2][2][kTile];
+    __shared__ __align__(1024) uint8_t lds[4][kTile]; // keys of even and odd tiles, values of even and odd tiles
     __shared__ int odd_values[4];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -66,8 +66,10 @@ template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256) void attn_
     const int ahead = ks.count - qs.count; // query i sees keys up to ahead + i
     const int first = block * kBlock + wave * 32 * QT; // the wave's first query
     const int last_key = ahead + min(block * kBlock + kBlock, qs.count) - 1; // seen by the block
-    const int wave_last = ahead + min(first + 32 * QT, qs.count) - 1;        // seen by the wave
+    const int wave_last = ahead + min(first + 32 * QT, qs.count) - 1;        // seen by the wave (nothing if it has no queries)
     const int tiles = last_key < 0 ? 0 : last_key / kTokens + 1;
+    const int wave_tiles = first >= qs.count || wave_last < 0 ? 0 : wave_last / kTokens + 1;
+    const int whole = min(max(ahead + block * kBlock + 1, 0) / kTokens, tiles); // tiles that every query sees in full
 
     uint4 q[QT][D / 16];
 #pragma unroll
@@ -78,11 +80,16 @@ template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256) void attn_
         for (int s = 0; s < D / 16; ++s)
             q[qt][s] = *(const uint4 *)(src + 16 * s);
     }
+    // Weights are 2^(score - base + kLift): base follows the running maximum only when that has left it 2^kSlack behind, which
+    // spares nearly every rescaling, and the lift leaves fp16 its normal range down to 2^-20 of the largest weight.
+    constexpr float kSlack = 8, kLift = 6;
+    const float slack = kSlack / a.scale_log2;
     float16v out[QT][D / 32];
-    float m[QT], l[QT];
+    float base[QT], shift[QT], l[QT], most[QT]; // base: in scores; shift: what is added to scores in powers of two
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
-        m[qt] = -INFINITY;
+        base[qt] = -INFINITY;
+        shift[qt] = 0;
         l[qt] = 0;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
@@ -91,90 +98,83 @@ template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256) void attn_
                 out[qt][d][i] = 0;
     }
 
-    const uint16_t *k_src = (const uint16_t *)a.k.data + (int64_t)kv_head * a.k.head_stride;
-    const uint16_t *v_src = (const uint16_t *)a.v.data + (int64_t)kv_head * a.v.head_stride;
-    const unsigned lds_at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)&lds[0][0][0];
-    auto load_tile = [&](int tile, int buffer) {
+    // loads of a tile: the lane's place in it, in bytes
+    const uint16_t *k_src = (const uint16_t *)a.k.data + (int64_t)ks.first * a.k.row_stride + (int64_t)kv_head * a.k.head_stride;
+    const uint16_t *v_src = (const uint16_t *)a.v.data + (int64_t)ks.first * a.v.row_stride + (int64_t)kv_head * a.v.head_stride;
+    const unsigned lds_at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)&lds[0][0] + wave * kLoads * 1024;
+    const int load_row = (wave * kLoads * 64 + lane) / kPieces, load_piece = lane % kPieces;
+    constexpr int kRowStep = 64 / kPieces; // rows between a wave's loads
+    auto load_keys = [&](int tile) {
+        const int rows = ks.count - tile * kTokens - 1; // (rows behind the last one are copies of it, and never seen)
+        const uint16_t *src = k_src + (int64_t)tile * kTokens * a.k.row_stride;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int piece = (wave * kLoads + i) * 64 + lane, r = piece / kPieces, c = piece % kPieces;
-            const int64_t row = ks.first + min(tile * kTokens + r, ks.count - 1); // (rows behind the last: never seen)
-            lds_dma16(k_src + row * a.k.row_stride + 8 * key_piece<D>(r, c), lds_at + buffer * 2 * kTile + (wave * kLoads + i) * 1024);
-            lds_dma16(v_src + row * a.v.row_stride + 8 * value_piece<D>(r, c), lds_at + (buffer * 2 + 1) * kTile + (wave * kLoads + i) * 1024);
+            const int r = load_row + i * kRowStep;
+            lds_dma16(src, (uint32_t)(min(r, rows) * (int)a.k.row_stride + 8 * key_piece<D>(r, load_piece)) * 2, lds_at + (tile & 1) * kTile + i * 1024);
+        }
+    };
+    auto load_values = [&](int tile) {
+        const int rows = ks.count - tile * kTokens - 1;
+        const uint16_t *src = v_src + (int64_t)tile * kTokens * a.v.row_stride;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int r = load_row + i * kRowStep;
+            lds_dma16(src, (uint32_t)(min(r, rows) * (int)a.v.row_stride + 8 * value_piece<D>(r, load_piece)) * 2, lds_at + (2 + (tile & 1)) * kTile + i * 1024);
         }
     };
 
-    if (tiles > 0)
-        load_tile(0, 0);
-    for (int tile = 0; tile < tiles; ++tile) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (tile + 1 < tiles)
-            load_tile(tile + 1, tile + 1 & 1);
-        const uint8_t *kt = lds[tile & 1][0], *vt = lds[tile & 1][1];
-        const int at = tile * kTokens;
-        const bool masked = at + kTokens - 1 > ahead + block * kBlock;
-        // A weight of 0 does not keep an infinite value out of a product, so tiles that some query sees a part of are
-        // looked through for values that are not finite.
-        bool odd = false;
-        if (masked) {
-            uint32_t found = 0;
-#pragma unroll
-            for (int i = 0; i < kTile / 4096; ++i) {
-                const uint4 w = *(const uint4 *)(vt + (i * 256 + threadIdx.x) * 16);
-                const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) // all ones in the exponent: adding one to it carries
-                    found |= DTYPE == ABQ_BF16 ? (x[j] & 0x7f807f80u) + 0x00800080u : (x[j] & 0x7c007c00u) + 0x04000400u;
-            }
-            if (lane == 0)
-                odd_values[wave] = 0;
-            if (__any((found & 0x80008000u) != 0) && lane == 0)
-                odd_values[wave] = 1;
-            __syncthreads();
-            odd = odd_values[0] | odd_values[1] | odd_values[2] | odd_values[3];
-        }
-        if (at > wave_last)
-            continue;
-
-        // S^T: scores of 2 x 32 tokens
-        float16v score[QT][2];
+    // S^T of a tile
+    float16v score[QT][2];
+    auto scores = [&](int tile, float16v (&sc)[QT][2]) {
+        const uint8_t *kt = lds[tile & 1];
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) {
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    score[qt][tt][i] = 0;
+                    sc[qt][tt][i] = 0;
 #pragma unroll
             for (int s = 0; s < D / 16; ++s) {
                 const int r = 32 * tt + ql;
                 const uint4 k = *(const uint4 *)(kt + r * D * 2 + key_piece<D>(r, 2 * s + half) * 16);
 #pragma unroll
                 for (int qt = 0; qt < QT; ++qt)
-                    score[qt][tt] = mfma_32x32x16<DTYPE>(k, q[qt][s], score[qt][tt]);
+                    sc[qt][tt] = mfma_32x32x16<DTYPE>(k, q[qt][s], sc[qt][tt]);
             }
         }
-        uint32_t p[QT][2][8];
+    };
+    auto hide = [&](int tile) { // what a query does not see
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
-            const int sees = ahead + first + 32 * qt + ql - at - 4 * half; // tokens up to this one, less what the lane stands for
-            if (masked)
-#pragma unroll
-                for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        score[qt][tt][i] = 32 * tt + 8 * (i / 4) + i % 4 <= sees ? score[qt][tt][i] : -INFINITY;
-            float most = -INFINITY;
+            const int sees = ahead + first + 32 * qt + ql - tile * kTokens - 4 * half;
 #pragma unroll
             for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    most = fmaxf(most, score[qt][tt][i]);
-            most = fmaxf(max_across_halves(most), m[qt]);
-            const float base = most == -INFINITY ? 0.f : most * a.scale_log2;
-            if (__any(most > m[qt])) {
-                const float down = __builtin_amdgcn_exp2f(m[qt] * a.scale_log2 - base);
+                    score[qt][tt][i] = 32 * tt + 8 * (i / 4) + i % 4 <= sees ? score[qt][tt][i] : -INFINITY;
+        }
+    };
+    auto find_most = [&]() {
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) {
+            float x = -INFINITY;
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    x = fmaxf(x, score[qt][tt][i]);
+            most[qt] = max_across_halves(x);
+        }
+    };
+    auto follow = [&]() {
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt)
+            if (__any(most[qt] > base[qt] + slack)) {
+                const float to = fmaxf(most[qt], base[qt]);
+                const float down = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((base[qt] - to) * a.scale_log2);
+                base[qt] = to;
+                shift[qt] = to == -INFINITY ? 0.f : kLift - to * a.scale_log2;
                 l[qt] *= down;
 #pragma unroll
                 for (int d = 0; d < D / 32; ++d)
@@ -182,50 +182,26 @@ template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256) void attn_
                     for (int i = 0; i < 16; ++i)
                         out[qt][d][i] *= down;
             }
-            m[qt] = most;
+    };
+    uint32_t p[QT][2][8];
+    auto weigh = [&]() {
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
             for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    score[qt][tt][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[qt][tt][i], a.scale_log2, -base));
-                    l[qt] += score[qt][tt][i];
+                for (int i = 0; i < 8; ++i) {
+                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(score[qt][tt][2 * i], a.scale_log2, shift[qt]));
+                    const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(score[qt][tt][2 * i + 1], a.scale_log2, shift[qt]));
+                    l[qt] += x;
+                    l[qt] += y;
+                    p[qt][tt][i] = pack16<DTYPE>(x, y);
                 }
-#pragma unroll
-            for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    p[qt][tt][i] = pack16<DTYPE>(score[qt][tt][2 * i], score[qt][tt][2 * i + 1]);
-        }
-        if (odd) {
-            // token by token, adding only what is seen
-#pragma unroll 1
-            for (int tok = 0; tok < kTokens; ++tok) {
-                const int i = tok % 32 / 8 * 4 + tok % 4;
-#pragma unroll
-                for (int qt = 0; qt < QT; ++qt) {
-                    float w = 0;
-#pragma unroll
-                    for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            w = tok / 32 == tt && i == j ? score[qt][tt][j] : w;
-                    w = __shfl(w, ql + 32 * (tok / 4 % 2));
-                    if (at + tok > ahead + first + 32 * qt + ql)
-                        continue;
-#pragma unroll
-                    for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            const int e = 32 * d + 8 * (j / 4) + 4 * half + j % 4;
-                            const uint16_t x = *(const uint16_t *)(vt + tok * D * 2 + value_piece<D>(tok, e / 8) * 16 + e % 8 * 2);
-                            out[qt][d][j] += w * value16<DTYPE>(x);
-                        }
-                }
-            }
-            continue;
-        }
-        // out^T += V^T P^T, 16 tokens at a time
-        const int tr = (lane & 15) / 4 + 4 * half, tc = 16 * (lane >> 4 & 1) + 4 * (lane & 3); // the lane's row and element
+    };
+    // out^T += V^T P^T, 16 tokens at a time
+    const int tr = (lane & 15) / 4 + 4 * half, tc = 16 * (lane >> 4 & 1) + 4 * (lane & 3); // the lane's row and element
+    auto gather = [&](int tile) {
+        const uint8_t *vt = lds[2 + (tile & 1)];
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
@@ -244,6 +220,80 @@ template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256) void attn_
                         out[qt][d] = mfma_32x32x16<DTYPE>(uint4{v[0].x, v[0].y, v[1].x, v[1].y},
                                                           uint4{p[qt][tt][4 * s], p[qt][tt][4 * s + 1], p[qt][tt][4 * s + 2], p[qt][tt][4 * s + 3]}, out[qt][d]);
                 }
+    };
+    auto arrive = [&]() { // what was requested is there, and nobody reads what will be overwritten
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    };
+
+    if (tiles > 0) {
+        load_keys(0);
+        load_values(0);
+    }
+    for (int tile = 0; tile < tiles; ++tile) {
+        arrive();
+        if (tile + 1 < tiles) {
+            load_keys(tile + 1);
+            load_values(tile + 1);
+        }
+        // A weight of 0 does not keep an infinite value out of a product, so tiles that some query sees a part of are
+        // looked through for values that are not finite.
+        bool odd = false;
+        if (tile >= whole) {
+            const uint8_t *vt = lds[2 + (tile & 1)];
+            uint32_t found = 0;
+#pragma unroll
+            for (int i = 0; i < kTile / 4096; ++i) {
+                const uint4 w = *(const uint4 *)(vt + (i * 256 + threadIdx.x) * 16);
+                const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) // all ones in the exponent: adding one to it carries
+                    found |= DTYPE == ABQ_BF16 ? (x[j] & 0x7f807f80u) + 0x00800080u : (x[j] & 0x7c007c00u) + 0x04000400u;
+            }
+            const bool any = __any((found & 0x80008000u) != 0);
+            if (lane == 0)
+                odd_values[wave] = any;
+            __syncthreads();
+            odd = odd_values[0] | odd_values[1] | odd_values[2] | odd_values[3];
+        }
+        if (tile < wave_tiles) {
+            scores(tile, score);
+            if (tile >= whole)
+                hide(tile);
+            find_most();
+            follow();
+            weigh();
+            if (odd) {
+                // token by token, adding only what is seen
+                const uint8_t *vt = lds[2 + (tile & 1)];
+#pragma unroll 1
+                for (int tok = 0; tok < kTokens; ++tok) {
+                    const int i = tok % 32 / 8 * 4 + tok % 4;
+#pragma unroll
+                    for (int qt = 0; qt < QT; ++qt) {
+                        uint32_t pair = 0;
+#pragma unroll
+                        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                pair = tok / 32 == tt && i / 2 == j ? p[qt][tt][j] : pair;
+                        pair = __shfl(pair, ql + 32 * (tok / 4 % 2));
+                        const float w = value16<DTYPE>(i & 1 ? pair >> 16 : pair);
+                        if (tile * kTokens + tok > ahead + first + 32 * qt + ql)
+                            continue;
+#pragma unroll
+                        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                const int e = 32 * d + 8 * (j / 4) + 4 * half + j % 4;
+                                const uint16_t x = *(const uint16_t *)(vt + tok * D * 2 + value_piece<D>(tok, e / 8) * 16 + e % 8 * 2);
+                                out[qt][d][j] += w * value16<DTYPE>(x);
+                            }
+                    }
+                }
+            } else
+                gather(tile);
+        }
     }
 
 #pragma unroll
@@ -283,9 +333,9 @@ void plan_attn_prompt(abq_attn_state *st, int most_parts)
 #define ABQ_PROMPT(T, D_, QT) hipLaunchKernelGGL((attn_prompt_kernel<T, D_, QT>), grid, dim3(256), 0, stream, a)
 #define ABQ_PROMPT_DIM(T)                    \
     do {                                     \
-        if (st.head_dim == 64)               \
+        if (st.head_dim == 64) {             \
             ABQ_PROMPT(T, 64, 1);            \
-        else                                 \
+        } else                               \
             ABQ_PROMPT(T, 128, 1);           \
     } while (0)
 
