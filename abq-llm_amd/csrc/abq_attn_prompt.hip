@@ -42,6 +42,12 @@ template <int DTYPE> __device__ __forceinline__ float16v mfma_32x32x16(uint4 a, 
 template <int D> __device__ __forceinline__ int key_piece(int r, int c) { return c ^ (D == 128 ? r & 15 : r >> 1 & 7); }
 template <int D> __device__ __forceinline__ int value_piece(int r, int c) { return c ^ (D == 128 ? 4 * (r & 3) : 4 * (r >> 1 & 1)); }
 
+// Of a pair of 16-bit floats, the sign bits of those whose exponent is all ones (adding one to it carries there)
+template <int DTYPE> __device__ __forceinline__ uint32_t not_finite(uint32_t pair)
+{
+    return (DTYPE == ABQ_BF16 ? (pair & 0x7f807f80u) + 0x00800080u : (pair & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+}
+
 template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256, 3 - QT) void attn_prompt_kernel(PromptArgs a)
 {
     constexpr int kBlock = 128 * QT;            // queries of the workgroup
@@ -104,23 +110,26 @@ template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256, 3 - QT) vo
     const unsigned lds_at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)&lds[0][0] + wave * kLoads * 1024;
     const int load_row = (wave * kLoads * 64 + lane) / kPieces, load_piece = lane % kPieces;
     constexpr int kRowStep = 64 / kPieces; // rows between a wave's loads
-    auto load_keys = [&](int tile) {
-        const int rows = ks.count - tile * kTokens - 1; // (rows behind the last one are copies of it, and never seen)
-        const uint16_t *src = k_src + (int64_t)tile * kTokens * a.k.row_stride;
+    const uint32_t k_row = load_row * (uint32_t)a.k.row_stride * 2, k_piece = 16 * key_piece<D>(load_row, load_piece);
+    const uint32_t v_at = load_row * (uint32_t)a.v.row_stride * 2 + 16 * value_piece<D>(load_row, load_piece);
+    auto load_tile = [&](int tile) {
+        const uint16_t *k = k_src + (int64_t)tile * kTokens * a.k.row_stride, *v = v_src + (int64_t)tile * kTokens * a.v.row_stride;
+        const unsigned to = lds_at + (tile & 1) * kTile;
+        const int rows = ks.count - tile * kTokens;
+        if (rows >= kTokens) { // kRowStep rows on, the pieces of keys change places by 4 and those of values not at all
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int r = load_row + i * kRowStep;
-            lds_dma16(src, (uint32_t)(min(r, rows) * (int)a.k.row_stride + 8 * key_piece<D>(r, load_piece)) * 2, lds_at + (tile & 1) * kTile + i * 1024);
-        }
-    };
-    auto load_values = [&](int tile) {
-        const int rows = ks.count - tile * kTokens - 1;
-        const uint16_t *src = v_src + (int64_t)tile * kTokens * a.v.row_stride;
+            for (int i = 0; i < kLoads; ++i)
+                lds_dma16(k + i * kRowStep * a.k.row_stride, k_row + (k_piece ^ 64 * i), to + i * 1024);
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int r = load_row + i * kRowStep;
-            lds_dma16(src, (uint32_t)(min(r, rows) * (int)a.v.row_stride + 8 * value_piece<D>(r, load_piece)) * 2, lds_at + (2 + (tile & 1)) * kTile + i * 1024);
-        }
+            for (int i = 0; i < kLoads; ++i)
+                lds_dma16(v + i * kRowStep * a.v.row_stride, v_at, to + 2 * kTile + i * 1024);
+        } else // rows behind the last one are copies of it, and never seen
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int r = load_row + i * kRowStep, from = min(r, rows - 1);
+                lds_dma16(k, from * (uint32_t)a.k.row_stride * 2 + 16 * key_piece<D>(r, load_piece), to + i * 1024);
+                lds_dma16(v, from * (uint32_t)a.v.row_stride * 2 + 16 * value_piece<D>(r, load_piece), to + 2 * kTile + i * 1024);
+            }
     };
 
     // S^T of a tile
@@ -226,35 +235,39 @@ template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256, 3 - QT) vo
         __syncthreads();
     };
 
-    if (tiles > 0) {
-        load_keys(0);
-        load_values(0);
-    }
+    if (tiles > 0)
+        load_tile(0);
     for (int tile = 0; tile < tiles; ++tile) {
         arrive();
-        if (tile + 1 < tiles) {
-            load_keys(tile + 1);
-            load_values(tile + 1);
-        }
-        // A weight of 0 does not keep an infinite value out of a product, so tiles that some query sees a part of are
-        // looked through for values that are not finite.
+        if (tile + 1 < tiles)
+            load_tile(tile + 1);
+        // A weight of 0 does not keep an infinite value out of a product.  Tiles that some query sees a part of are looked
+        // through for values that are not finite; where there are some, zeros take their places, and they are added after the
+        // product to the queries that see them.
         bool odd = false;
         if (tile >= whole) {
-            const uint8_t *vt = lds[2 + (tile & 1)];
+            uint4 *piece = (uint4 *)(lds[2 + (tile & 1)] + threadIdx.x * 16);
             uint32_t found = 0;
 #pragma unroll
             for (int i = 0; i < kTile / 4096; ++i) {
-                const uint4 w = *(const uint4 *)(vt + (i * 256 + threadIdx.x) * 16);
-                const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) // all ones in the exponent: adding one to it carries
-                    found |= DTYPE == ABQ_BF16 ? (x[j] & 0x7f807f80u) + 0x00800080u : (x[j] & 0x7c007c00u) + 0x04000400u;
+                const uint4 w = piece[i * 256];
+                found |= not_finite<DTYPE>(w.x) | not_finite<DTYPE>(w.y) | not_finite<DTYPE>(w.z) | not_finite<DTYPE>(w.w);
             }
-            const bool any = __any((found & 0x80008000u) != 0);
+            const bool any = __any(found != 0);
             if (lane == 0)
                 odd_values[wave] = any;
             __syncthreads();
             odd = odd_values[0] | odd_values[1] | odd_values[2] | odd_values[3];
+            if (odd) {
+#pragma unroll 1
+                for (int i = 0; i < kTile / 4096; ++i) {
+                    uint4 w = piece[i * 256];
+                    w.x &= ~(not_finite<DTYPE>(w.x) / 0x8000 * 0xffff), w.y &= ~(not_finite<DTYPE>(w.y) / 0x8000 * 0xffff);
+                    w.z &= ~(not_finite<DTYPE>(w.z) / 0x8000 * 0xffff), w.w &= ~(not_finite<DTYPE>(w.w) / 0x8000 * 0xffff);
+                    piece[i * 256] = w;
+                }
+                __syncthreads();
+            }
         }
         if (tile < wave_tiles) {
             scores(tile, score);
@@ -263,11 +276,11 @@ template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256, 3 - QT) vo
             find_most();
             follow();
             weigh();
+            gather(tile);
             if (odd) {
-                // token by token, adding only what is seen
-                const uint8_t *vt = lds[2 + (tile & 1)];
 #pragma unroll 1
-                for (int tok = 0; tok < kTokens; ++tok) {
+                for (int tok = 0; tok < min(kTokens, ks.count - tile * kTokens); ++tok) {
+                    const uint16_t *src = v_src + (int64_t)(tile * kTokens + tok) * a.v.row_stride + 4 * half;
                     const int i = tok % 32 / 8 * 4 + tok % 4;
 #pragma unroll
                     for (int qt = 0; qt < QT; ++qt) {
@@ -279,20 +292,23 @@ template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256, 3 - QT) vo
                                 pair = tok / 32 == tt && i / 2 == j ? p[qt][tt][j] : pair;
                         pair = __shfl(pair, ql + 32 * (tok / 4 % 2));
                         const float w = value16<DTYPE>(i & 1 ? pair >> 16 : pair);
-                        if (tile * kTokens + tok > ahead + first + 32 * qt + ql)
-                            continue;
+                        const bool seen = tile * kTokens + tok <= ahead + first + 32 * qt + ql;
 #pragma unroll
-                        for (int d = 0; d < D / 32; ++d)
+                        for (int d = 0; d < D / 32; ++d) {
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) {
-                                const int e = 32 * d + 8 * (j / 4) + 4 * half + j % 4;
-                                const uint16_t x = *(const uint16_t *)(vt + tok * D * 2 + value_piece<D>(tok, e / 8) * 16 + e % 8 * 2);
-                                out[qt][d][j] += w * value16<DTYPE>(x);
+                            for (int j = 0; j < 4; ++j) {
+                                const uint2 four = *(const uint2 *)(src + 32 * d + 8 * j);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const float x = value16<DTYPE>((e < 2 ? four.x : four.y) >> (16 * (e & 1)));
+                                    out[qt][d][4 * j + e] += seen && !(fabsf(x) < INFINITY) ? w * x : 0.f;
+                                }
                             }
+                            asm volatile("" ::: "memory"); // (a few loads at a time: rare, and not to cost registers)
+                        }
                     }
                 }
-            } else
-                gather(tile);
+            }
         }
     }
 
