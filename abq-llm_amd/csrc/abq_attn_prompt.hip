@@ -86,6 +86,12 @@ template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256, 3 - QT) vo
         for (int s = 0; s < D / 16; ++s)
             q[qt][s] = *(const uint4 *)(src + 16 * s);
     }
+    // (there before the loop: a wait for them inside it would be one for the tile that is being loaded)
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s)
+            asm volatile("" : "+v"(q[qt][s].x), "+v"(q[qt][s].y), "+v"(q[qt][s].z), "+v"(q[qt][s].w));
     // Weights are 2^(score - base + kLift): base follows the running maximum only when that has left it 2^kSlack behind, which
     // spares nearly every rescaling, and the lift leaves fp16 its normal range down to 2^-20 of the largest weight.
     constexpr float kSlack = 8, kLift = 6;
