@@ -143,21 +143,29 @@ template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256, 3 - QT) vo
     auto scores = [&](int tile, float16v (&sc)[QT][2]) {
         const uint8_t *kt = lds[tile & 1];
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt) {
+        for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     sc[qt][tt][i] = 0;
 #pragma unroll
-            for (int s = 0; s < D / 16; ++s) {
+        for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt) {
                 const int r = 32 * tt + ql;
                 const uint4 k = *(const uint4 *)(kt + r * D * 2 + key_piece<D>(r, 2 * s + half) * 16);
 #pragma unroll
                 for (int qt = 0; qt < QT; ++qt)
                     sc[qt][tt] = mfma_32x32x16<DTYPE>(k, q[qt][s], sc[qt][tt]);
             }
+        __builtin_amdgcn_sched_group_barrier(0x100, 8, 0); // eight reads, then a product and a read in turn
+#pragma unroll
+        for (int i = 0; i < D / 8 - 8; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
+        __builtin_amdgcn_sched_group_barrier(0x8, 8, 0);
     };
     auto hide = [&](int tile) { // what a query does not see
 #pragma unroll
@@ -198,43 +206,42 @@ template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256, 3 - QT) vo
                         out[qt][d][i] *= down;
             }
     };
-    uint32_t p[QT][2][8];
-    auto weigh = [&]() {
+    // Sixteen tokens at a time: their weights, their values, and out^T += V^T P^T
+    uint32_t p[QT][4][4];
+    auto weigh = [&](int s) {
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
-            for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(score[qt][tt][2 * i], a.scale_log2, shift[qt]));
-                    const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(score[qt][tt][2 * i + 1], a.scale_log2, shift[qt]));
-                    l[qt] += x;
-                    l[qt] += y;
-                    p[qt][tt][i] = pack16<DTYPE>(x, y);
-                }
+            for (int i = 0; i < 4; ++i) {
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(score[qt][s / 2][8 * (s % 2) + 2 * i], a.scale_log2, shift[qt]));
+                const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(score[qt][s / 2][8 * (s % 2) + 2 * i + 1], a.scale_log2, shift[qt]));
+                l[qt] += x;
+                l[qt] += y;
+                p[qt][s][i] = pack16<DTYPE>(x, y);
+            }
     };
-    // out^T += V^T P^T, 16 tokens at a time
     const int tr = (lane & 15) / 4 + 4 * half, tc = 16 * (lane >> 4 & 1) + 4 * (lane & 3); // the lane's row and element
-    auto gather = [&](int tile) {
+    uint4 v[2][D / 32];
+    auto fetch = [&](int tile, int s) {
         const uint8_t *vt = lds[2 + (tile & 1)];
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
+        for (int d = 0; d < D / 32; ++d) {
+            uint2 x[2];
 #pragma unroll
-            for (int s = 0; s < 2; ++s)
+            for (int j = 0; j < 2; ++j) {
+                const int r = 16 * s + 8 * j + tr, e = 32 * d + tc;
+                x[j] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) short4v *)(vt + r * D * 2 + value_piece<D>(r, e / 8) * 16 + e % 8 * 2)));
+            }
+            v[s & 1][d] = uint4{x[0].x, x[0].y, x[1].x, x[1].y};
+        }
+    };
+    auto gather = [&](int s) {
 #pragma unroll
-                for (int d = 0; d < D / 32; ++d) {
-                    uint2 v[2];
+        for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const int r = 32 * tt + 16 * s + 8 * x + tr, e = 32 * d + tc;
-                        v[x] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (__attribute__((address_space(3))) short4v *)(vt + r * D * 2 + value_piece<D>(r, e / 8) * 16 + e % 8 * 2)));
-                    }
-#pragma unroll
-                    for (int qt = 0; qt < QT; ++qt)
-                        out[qt][d] = mfma_32x32x16<DTYPE>(uint4{v[0].x, v[0].y, v[1].x, v[1].y},
-                                                          uint4{p[qt][tt][4 * s], p[qt][tt][4 * s + 1], p[qt][tt][4 * s + 2], p[qt][tt][4 * s + 3]}, out[qt][d]);
-                }
+            for (int qt = 0; qt < QT; ++qt)
+                out[qt][d] = mfma_32x32x16<DTYPE>(v[s & 1][d], uint4{p[qt][s][0], p[qt][s][1], p[qt][s][2], p[qt][s][3]}, out[qt][d]);
     };
     auto arrive = [&]() { // what was requested is there, and nobody reads what will be overwritten
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -281,8 +288,24 @@ template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256, 3 - QT) vo
                 hide(tile);
             find_most();
             follow();
-            weigh();
-            gather(tile);
+            fetch(tile, 0);
+            weigh(0);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) { // the next tokens' weights stand between the products
+                if (s < 3) {
+                    fetch(tile, s + 1);
+                    weigh(s + 1);
+                }
+                gather(s);
+                __builtin_amdgcn_sched_group_barrier(0x100, D / 16, 0);
+#pragma unroll
+                for (int i = 0; i < D / 32 * QT; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x402, 28 * 32 / D, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
             if (odd) {
 #pragma unroll 1
                 for (int tok = 0; tok < min(kTokens, ks.count - tile * kTokens); ++tok) {
@@ -292,10 +315,8 @@ template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256, 3 - QT) vo
                     for (int qt = 0; qt < QT; ++qt) {
                         uint32_t pair = 0;
 #pragma unroll
-                        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-                            for (int j = 0; j < 8; ++j)
-                                pair = tok / 32 == tt && i / 2 == j ? p[qt][tt][j] : pair;
+                        for (int j = 0; j < 16; ++j)
+                            pair = tok / 32 * 8 + i / 2 == j ? p[qt][j / 4][j % 4] : pair;
                         pair = __shfl(pair, ql + 32 * (tok / 4 % 2));
                         const float w = value16<DTYPE>(i & 1 ? pair >> 16 : pair);
                         const bool seen = tile * kTokens + tok <= ahead + first + 32 * qt + ql;
