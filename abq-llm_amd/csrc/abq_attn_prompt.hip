@@ -24,6 +24,7 @@ struct PromptArgs {
     const int32_t *q_starts, *k_starts;
     int heads, kv_heads, seqs, blocks; // blocks: of queries in the longest sequence
     float scale_log2;
+    AttnParts parts;
 };
 
 constexpr int kTokens = 64; // of a tile
@@ -48,21 +49,26 @@ template <int DTYPE> __device__ __forceinline__ uint32_t not_finite(uint32_t pai
     return (DTYPE == ABQ_BF16 ? (pair & 0x7f807f80u) + 0x00800080u : (pair & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
 }
 
-template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256, 3 - QT) void attn_prompt_kernel(PromptArgs a)
+// KG = 1: the four waves share the queries, 32 QT each.  KG = 2: two waves do, and the other two take the other 32 tokens of each
+// tile; their results are joined at the end.
+template <int DTYPE, int D, int QT, int KG> __global__ __launch_bounds__(256, 3 - QT) void attn_prompt_kernel(PromptArgs a)
 {
-    constexpr int kBlock = 128 * QT;            // queries of the workgroup
+    constexpr int kBlock = 128 * QT / KG;       // queries of the workgroup
+    constexpr int TT = 2 / KG;                  // a wave's 32-token parts of a tile
     constexpr int kPieces = D / 8;              // of a row
     constexpr int kTile = kTokens * D * 2;      // bytes
     constexpr int kLoads = kTile / 1024 / 4;    // of a wave per tile
     __shared__ __align__(1024) uint8_t lds[4][kTile]; // keys of even and odd tiles, values of even and odd tiles
     __shared__ int odd_values[4];
+    static_assert(KG == 1 || 4 * kTile >= 64 * QT * (D + 4) * 4, "the waves' sums fit where the tiles were");
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ql = lane & 31, half = lane >> 5;
     // Blocks with the most keys first.  Heads that share keys are kv_heads apart, so with 8 key heads (or a multiple) each
     // stays with one XCD's L2.
     const uint32_t per_block = a.heads * a.seqs;
-    const int block = a.blocks - 1 - (int)(blockIdx.x / per_block);
+    const int part = blockIdx.x / per_block % a.parts.parts, block = a.blocks - 1 - (int)(blockIdx.x / per_block / a.parts.parts);
+    const int kg = wave / (4 / KG);
     const int seq = blockIdx.x % per_block / a.heads, order = blockIdx.x % a.heads;
     const int kv_head = order % a.kv_heads, head = kv_head * (a.heads / a.kv_heads) + order / a.kv_heads;
 
@@ -70,12 +76,13 @@ template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256, 3 - QT) vo
     if (block * kBlock >= qs.count)
         return;
     const int ahead = ks.count - qs.count; // query i sees keys up to ahead + i
-    const int first = block * kBlock + wave * 32 * QT; // the wave's first query
+    const int first = block * kBlock + wave % (4 / KG) * 32 * QT; // the wave's first query
     const int last_key = ahead + min(block * kBlock + kBlock, qs.count) - 1; // seen by the block
     const int wave_last = ahead + min(first + 32 * QT, qs.count) - 1;        // seen by the wave (nothing if it has no queries)
     const int tiles = last_key < 0 ? 0 : last_key / kTokens + 1;
     const int wave_tiles = first >= qs.count || wave_last < 0 ? 0 : wave_last / kTokens + 1;
     const int whole = min(max(ahead + block * kBlock + 1, 0) / kTokens, tiles); // tiles that every query sees in full
+    const int tile0 = (int)((int64_t)tiles * part / a.parts.parts), tile1 = (int)((int64_t)tiles * (part + 1) / a.parts.parts);
 
     uint4 q[QT][D / 16];
 #pragma unroll
@@ -139,29 +146,29 @@ template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256, 3 - QT) vo
     };
 
     // S^T of a tile
-    float16v score[QT][2];
-    auto scores = [&](int tile, float16v (&sc)[QT][2]) {
-        const uint8_t *kt = lds[tile & 1];
+    float16v score[QT][TT];
+    auto scores = [&](int tile) {
+        const uint8_t *kt = lds[tile & 1] + kg * 32 * D * 2;
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
+        for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    sc[qt][tt][i] = 0;
+                    score[qt][tt][i] = 0;
 #pragma unroll
         for (int s = 0; s < D / 16; ++s)
 #pragma unroll
-            for (int tt = 0; tt < 2; ++tt) {
+            for (int tt = 0; tt < TT; ++tt) {
                 const int r = 32 * tt + ql;
                 const uint4 k = *(const uint4 *)(kt + r * D * 2 + key_piece<D>(r, 2 * s + half) * 16);
 #pragma unroll
                 for (int qt = 0; qt < QT; ++qt)
-                    sc[qt][tt] = mfma_32x32x16<DTYPE>(k, q[qt][s], sc[qt][tt]);
+                    score[qt][tt] = mfma_32x32x16<DTYPE>(k, q[qt][s], score[qt][tt]);
             }
         __builtin_amdgcn_sched_group_barrier(0x100, 8, 0); // eight reads, then a product and a read in turn
 #pragma unroll
-        for (int i = 0; i < D / 8 - 8; ++i) {
+        for (int i = 0; i < D / 16 * TT - 8; ++i) {
             __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
@@ -170,9 +177,9 @@ template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256, 3 - QT) vo
     auto hide = [&](int tile) { // what a query does not see
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
-            const int sees = ahead + first + 32 * qt + ql - tile * kTokens - 4 * half;
+            const int sees = ahead + first + 32 * qt + ql - tile * kTokens - 32 * kg - 4 * half;
 #pragma unroll
-            for (int tt = 0; tt < 2; ++tt)
+            for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     score[qt][tt][i] = 32 * tt + 8 * (i / 4) + i % 4 <= sees ? score[qt][tt][i] : -INFINITY;
@@ -183,7 +190,7 @@ template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256, 3 - QT) vo
         for (int qt = 0; qt < QT; ++qt) {
             float x = -INFINITY;
 #pragma unroll
-            for (int tt = 0; tt < 2; ++tt)
+            for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     x = fmaxf(x, score[qt][tt][i]);
@@ -207,7 +214,7 @@ template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256, 3 - QT) vo
             }
     };
     // Sixteen tokens at a time: their weights, their values, and out^T += V^T P^T
-    uint32_t p[QT][4][4];
+    uint32_t p[QT][2 * TT][4];
     auto weigh = [&](int s) {
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt)
@@ -229,7 +236,7 @@ template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256, 3 - QT) vo
             uint2 x[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const int r = 16 * s + 8 * j + tr, e = 32 * d + tc;
+                const int r = 32 * kg + 16 * s + 8 * j + tr, e = 32 * d + tc;
                 x[j] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                     (__attribute__((address_space(3))) short4v *)(vt + r * D * 2 + value_piece<D>(r, e / 8) * 16 + e % 8 * 2)));
             }
@@ -248,11 +255,11 @@ template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256, 3 - QT) vo
         __syncthreads();
     };
 
-    if (tiles > 0)
-        load_tile(0);
-    for (int tile = 0; tile < tiles; ++tile) {
+    if (tile0 < tile1)
+        load_tile(tile0);
+    for (int tile = tile0; tile < tile1; ++tile) {
         arrive();
-        if (tile + 1 < tiles)
+        if (tile + 1 < tile1)
             load_tile(tile + 1);
         // A weight of 0 does not keep an infinite value out of a product.  Tiles that some query sees a part of are looked
         // through for values that are not finite; where there are some, zeros take their places, and they are added after the
@@ -283,7 +290,7 @@ template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256, 3 - QT) vo
             }
         }
         if (tile < wave_tiles) {
-            scores(tile, score);
+            scores(tile);
             if (tile >= whole)
                 hide(tile);
             find_most();
@@ -292,8 +299,8 @@ template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256, 3 - QT) vo
             weigh(0);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int s = 0; s < 4; ++s) { // the next tokens' weights stand between the products
-                if (s < 3) {
+            for (int s = 0; s < 2 * TT; ++s) { // the next tokens' weights stand between the products
+                if (s < 2 * TT - 1) {
                     fetch(tile, s + 1);
                     weigh(s + 1);
                 }
@@ -308,15 +315,15 @@ template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256, 3 - QT) vo
             }
             if (odd) {
 #pragma unroll 1
-                for (int tok = 0; tok < min(kTokens, ks.count - tile * kTokens); ++tok) {
+                for (int tok = 32 * kg; tok < min(32 * kg + 32 * TT, ks.count - tile * kTokens); ++tok) {
                     const uint16_t *src = v_src + (int64_t)(tile * kTokens + tok) * a.v.row_stride + 4 * half;
                     const int i = tok % 32 / 8 * 4 + tok % 4;
 #pragma unroll
                     for (int qt = 0; qt < QT; ++qt) {
                         uint32_t pair = 0;
 #pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            pair = tok / 32 * 8 + i / 2 == j ? p[qt][j / 4][j % 4] : pair;
+                        for (int j = 0; j < 8 * TT; ++j)
+                            pair = (tok / 32 - kg) * 8 + i / 2 == j ? p[qt][j / 4][j % 4] : pair;
                         pair = __shfl(pair, ql + 32 * (tok / 4 % 2));
                         const float w = value16<DTYPE>(i & 1 ? pair >> 16 : pair);
                         const bool seen = tile * kTokens + tok <= ahead + first + 32 * qt + ql;
@@ -328,7 +335,7 @@ template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256, 3 - QT) vo
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) {
                                     const float x = value16<DTYPE>((e < 2 ? four.x : four.y) >> (16 * (e & 1)));
-                                    out[qt][d][4 * j + e] += seen && !(fabsf(x) < INFINITY) ? w * x : 0.f;
+                                    out[qt][d][4 * j + e] = __builtin_fmaf(w, seen && !(fabsf(x) < INFINITY) ? x : 0.f, out[qt][d][4 * j + e]);
                                 }
                             }
                             asm volatile("" ::: "memory"); // (a few loads at a time: rare, and not to cost registers)
@@ -339,11 +346,67 @@ template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256, 3 - QT) vo
         }
     }
 
+    // the sums of the waves with the other tokens
+    if constexpr (KG == 2) {
+        float *sums = (float *)&lds[0][0];
+        __shared__ float other[2][64 * QT];
+        const int at = wave % 2 * 32 * QT;
+        __syncthreads();
+        if (kg == 1)
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) {
+                const int r = at + 32 * qt + ql;
+                l[qt] = sum_across_halves(l[qt]);
+                if (half == 0) {
+                    other[0][r] = base[qt];
+                    other[1][r] = l[qt];
+                }
+#pragma unroll
+                for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        *(float4 *)&sums[r * (D + 4) + 32 * d + 8 * j + 4 * half] =
+                            float4{out[qt][d][4 * j], out[qt][d][4 * j + 1], out[qt][d][4 * j + 2], out[qt][d][4 * j + 3]};
+            }
+        __syncthreads();
+        if (kg == 1)
+            return;
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) {
+            const int r = at + 32 * qt + ql;
+            const float b = other[0][r], to = fmaxf(b, base[qt]);
+            const float mine = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((base[qt] - to) * a.scale_log2);
+            const float theirs = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((b - to) * a.scale_log2);
+            base[qt] = to;
+            shift[qt] = to == -INFINITY ? 0.f : kLift - to * a.scale_log2;
+            l[qt] = l[qt] * mine + (half ? 0.f : other[1][r] * theirs);
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    out[qt][d][j] = out[qt][d][j] * mine + sums[r * (D + 4) + 32 * d + 8 * (j / 4) + 4 * half + j % 4] * theirs;
+        }
+    }
+
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
         const float total = sum_across_halves(l[qt]);
-        const float f = total > 0 ? 1.f / total : total; // (a sum that is not a number stays one)
         const int i = first + 32 * qt + ql;
+        if (a.parts.parts > 1) {
+            if (i < qs.count) {
+                const int64_t at = ((int64_t)(qs.first + i) * a.heads + head) * a.parts.parts + part;
+#pragma unroll
+                for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        *(float4 *)(a.parts.sums + at * D + 32 * d + 8 * j + 4 * half) =
+                            float4{out[qt][d][4 * j], out[qt][d][4 * j + 1], out[qt][d][4 * j + 2], out[qt][d][4 * j + 3]};
+                if (half == 0)
+                    a.parts.stats[at] = float2{base[qt] == -INFINITY ? -INFINITY : -shift[qt], total};
+            }
+            continue;
+        }
+        const float f = total > 0 ? 1.f / total : total; // (a sum that is not a number stays one)
         uint16_t *to = (uint16_t *)a.out.data + (int64_t)(qs.first + i) * a.out.row_stride + (int64_t)head * a.out.head_stride;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
@@ -368,18 +431,29 @@ template <int DTYPE, int D, int QT> __global__ __launch_bounds__(256, 3 - QT) vo
 
 void plan_attn_prompt(abq_attn_state *st, int most_parts)
 {
-    (void)most_parts;
-    st->block_rows = 128;
-    st->parts = 1;
+    const int64_t each = (int64_t)st->heads * st->seqs;
+    // A compute unit holds two workgroups, so 512 run beside each other.  With fewer blocks of 128 queries, blocks of 64 ...
+    st->block_rows = ((int64_t)st->max_q + 127) / 128 * each >= 512 ? 128 : 64;
+    // ... and where those leave room as well, parts of the keys, of eight tiles at least
+    const int64_t groups = ((int64_t)st->max_q + st->block_rows - 1) / st->block_rows * each;
+    int64_t parts = 512 / groups;
+    parts = parts < st->max_k / (8 * kTokens) ? parts : st->max_k / (8 * kTokens);
+    parts = parts < most_parts ? parts : most_parts;
+    st->parts = parts < 2 ? 1 : (int)parts;
 }
 
-#define ABQ_PROMPT(T, D_, QT) hipLaunchKernelGGL((attn_prompt_kernel<T, D_, QT>), grid, dim3(256), 0, stream, a)
+#define ABQ_PROMPT(T, D_, KG) hipLaunchKernelGGL((attn_prompt_kernel<T, D_, 1, KG>), grid, dim3(256), 0, stream, a)
 #define ABQ_PROMPT_DIM(T)                    \
     do {                                     \
         if (st.head_dim == 64) {             \
-            ABQ_PROMPT(T, 64, 1);            \
-        } else                               \
+            if (st.block_rows == 128)        \
+                ABQ_PROMPT(T, 64, 1);        \
+            else                             \
+                ABQ_PROMPT(T, 64, 2);        \
+        } else if (st.block_rows == 128)     \
             ABQ_PROMPT(T, 128, 1);           \
+        else                                 \
+            ABQ_PROMPT(T, 128, 2);           \
     } while (0)
 
 hipError_t launch_attn_prompt(const abq_attn_state &st, hipStream_t stream)
@@ -396,12 +470,14 @@ hipError_t launch_attn_prompt(const abq_attn_state &st, hipStream_t stream)
     a.seqs = st.seqs;
     a.blocks = (st.max_q + st.block_rows - 1) / st.block_rows;
     a.scale_log2 = st.scale * kLog2e;
-    const dim3 grid((unsigned)((int64_t)a.blocks * st.heads * st.seqs));
+    a.parts = attn_parts(st);
+    const dim3 grid((unsigned)((int64_t)a.blocks * st.heads * st.seqs * st.parts));
     if (st.dtype == ABQ_BF16)
         ABQ_PROMPT_DIM(ABQ_BF16);
     else
         ABQ_PROMPT_DIM(ABQ_F16);
-    return hipGetLastError();
+    const hipError_t e = hipGetLastError();
+    return e != hipSuccess || st.parts < 2 ? e : launch_attn_join(st, stream);
 }
 
 } // namespace abq

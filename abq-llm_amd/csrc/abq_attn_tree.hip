@@ -135,7 +135,10 @@ template <int BITS, int D> __device__ __forceinline__ int query_offset(int ks, i
     return (ks / kPieces) * (32 * kPieces) + g * 8 * kPieces + (ks % kPieces) * 8;
 }
 
-template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(256) void attn_tree_kernel(TreeArgs a)
+// Waves per SIMD that the registers are kept to
+constexpr int tree_waves(int bits, bool asym, int d, int rt) { return rt > 1 ? 2 : bits == 8 && asym && d == 128 ? 3 : 4; }
+
+template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(256, tree_waves(BITS, ASYM, D, RT)) void attn_tree_kernel(TreeArgs a)
 {
     using S = Step<BITS, ASYM, D>;
     constexpr int kTiles = D / 16; // 16 x 16 tiles of out^T
@@ -225,16 +228,7 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(256) 
 
     const int steps = (len + kStep - 1) / kStep;
     const int step0 = (int)((int64_t)steps * part / a.parts.parts) + wave, step1 = (int)((int64_t)steps * (part + 1) / a.parts.parts);
-    S next;
-    uint32_t next_seen = 0;
-    if (step0 < step1)
-        load_step<BITS, ASYM, D>(next, a, pages, last_page, head, step0 * kStep, lane, &next_seen);
-    for (int step = step0; step < step1; step += kWaves) {
-        S s = next;
-        const uint32_t seen = next_seen;
-        if (step + kWaves < step1)
-            load_step<BITS, ASYM, D>(next, a, pages, last_page, head, (step + kWaves) * kStep, lane, &next_seen);
-
+    auto weigh_step = [&](S &s, int step, uint32_t seen) {
         // scores
         float score[RT][2][4];
 #pragma unroll
@@ -353,6 +347,30 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(256) 
                 }
             }
         }
+    };
+    // One row tile leaves registers for four waves per SIMD, which cover each other's loads; with more, a wave loads a step ahead.
+    if constexpr (RT == 1 || (ASYM && D == 128)) {
+        for (int step = step0; step < step1; step += kWaves) {
+            S s;
+            uint32_t seen;
+            load_step<BITS, ASYM, D>(s, a, pages, last_page, head, step * kStep, lane, &seen);
+            weigh_step(s, step, seen);
+        }
+    } else {
+        S s[2];
+        uint32_t seen[2];
+        if (step0 < step1)
+            load_step<BITS, ASYM, D>(s[0], a, pages, last_page, head, step0 * kStep, lane, &seen[0]);
+        for (int step = step0; step < step1; step += 2 * kWaves) {
+            if (step + kWaves < step1)
+                load_step<BITS, ASYM, D>(s[1], a, pages, last_page, head, (step + kWaves) * kStep, lane, &seen[1]);
+            weigh_step(s[0], step, seen[0]);
+            if (step + kWaves >= step1)
+                break;
+            if (step + 2 * kWaves < step1)
+                load_step<BITS, ASYM, D>(s[0], a, pages, last_page, head, (step + 2 * kWaves) * kStep, lane, &seen[0]);
+            weigh_step(s[1], step + kWaves, seen[1]);
+        }
     }
 
     // the waves' results joined
@@ -422,7 +440,7 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(256) 
     }
 }
 
-// The parts of one query row and head per wave: D / 64 elements a lane
+// The parts of one query row and head per wave
 struct JoinArgs {
     abq_rows out;
     AttnParts parts;
@@ -441,31 +459,35 @@ template <int D> __global__ __launch_bounds__(256) void attn_join_kernel(JoinArg
     if (draft >= own.count)
         return;
     const int64_t row = own.first + draft, at = (row * a.heads + head) * a.parts.parts;
-    float most = -INFINITY;
-    for (int p = lane; p < a.parts.parts; p += 64)
-        most = fmaxf(most, a.parts.stats[at + p].x);
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2)
-        most = fmaxf(most, __shfl_xor(most, o));
-    const float base = most == -INFINITY ? 0.f : most;
-    constexpr int kEach = D / 64;
-    float total = 0, acc[kEach] = {};
-    for (int p = 0; p < a.parts.parts; ++p) {
+    // D / 4 lanes a part, four elements each, so 2 (4) parts at a time, each with a maximum of its own
+    constexpr int kLanes = D / 4, kSide = 64 / kLanes;
+    const int e0 = lane % kLanes * 4;
+    float most = -INFINITY, total = 0, acc[4] = {};
+#pragma unroll 4
+    for (int p = lane / kLanes; p < a.parts.parts; p += kSide) {
         const float2 st = a.parts.stats[at + p];
-        const float f = __builtin_amdgcn_exp2f(st.x - base);
-        total += f * st.y;
-        const float *from = a.parts.sums + (at + p) * D + lane * kEach;
+        const float4 x = *(const float4 *)(a.parts.sums + (at + p) * D + e0);
+        const float to = fmaxf(most, st.x), base = to == -INFINITY ? 0.f : to;
+        const float f = __builtin_amdgcn_exp2f(most - base), g = __builtin_amdgcn_exp2f(st.x - base);
+        most = to;
+        total = total * f + st.y * g;
+        acc[0] = acc[0] * f + x.x * g, acc[1] = acc[1] * f + x.y * g, acc[2] = acc[2] * f + x.z * g, acc[3] = acc[3] * f + x.w * g;
+    }
 #pragma unroll
-        for (int e = 0; e < kEach; ++e)
-            acc[e] += f * from[e];
+    for (int o = kLanes; o < 64; o *= 2) {
+        const float other = __shfl_xor(most, o), to = fmaxf(most, other), base = to == -INFINITY ? 0.f : to;
+        const float f = __builtin_amdgcn_exp2f(most - base), g = __builtin_amdgcn_exp2f(other - base);
+        most = to;
+        total = total * f + __shfl_xor(total, o) * g;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            acc[e] = acc[e] * f + __shfl_xor(acc[e], o) * g;
     }
     const float f = total > 0 ? 1.f / total : total;
-    uint16_t *to = (uint16_t *)a.out.data + row * a.out.row_stride + (int64_t)head * a.out.head_stride + lane * kEach;
-    const uint32_t x = a.dtype == ABQ_BF16 ? pack16<ABQ_BF16>(acc[0] * f, acc[kEach - 1] * f) : pack16<ABQ_F16>(acc[0] * f, acc[kEach - 1] * f);
-    if (kEach == 2)
-        *(uint32_t *)to = x;
-    else
-        *to = (uint16_t)x;
+    uint16_t *to = (uint16_t *)a.out.data + row * a.out.row_stride + (int64_t)head * a.out.head_stride + e0;
+    if (lane < kLanes)
+        *(uint2 *)to = a.dtype == ABQ_BF16 ? uint2{pack16<ABQ_BF16>(acc[0] * f, acc[1] * f), pack16<ABQ_BF16>(acc[2] * f, acc[3] * f)}
+                                           : uint2{pack16<ABQ_F16>(acc[0] * f, acc[1] * f), pack16<ABQ_F16>(acc[2] * f, acc[3] * f)};
 }
 
 } // namespace
