@@ -48,8 +48,7 @@ template <int BITS, bool ASYM, int D> struct Step {
     static constexpr int kWords = D * BITS / 128;
     static constexpr int kLoad = kWords < 4 ? kWords : 4; // words per load
     uint32_t k[2][kWords], v[2][kWords];
-    float ks[2][4], vs[2][4];
-    float kz[ASYM ? 2 : 1][4], vz[ASYM ? 2 : 1][4];
+    float ks, vs, kz, vz; // of one token: lanes t = 4 h + i of the quarter g have token 4 g + i of half h, lanes 8 + t the same
 };
 
 template <int N> __device__ __forceinline__ void load_words(uint32_t *to, const void *from)
@@ -62,10 +61,14 @@ template <int N> __device__ __forceinline__ void load_words(uint32_t *to, const 
         to[0] = w.x, to[1] = w.y;
     }
 }
-__device__ __forceinline__ void load_floats(float *to, const float *from)
+// What lane K of the lane's row of sixteen has
+template <int K> __device__ __forceinline__ uint32_t of_lane(uint32_t x)
 {
-    const float4 w = *(const float4 *)from;
-    to[0] = w.x, to[1] = w.y, to[2] = w.z, to[3] = w.w;
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x150 + K, 0xf, 0xf, true);
+}
+template <int K> __device__ __forceinline__ float of_lane(float x)
+{
+    return __builtin_bit_cast(float, of_lane<K>(__builtin_bit_cast(uint32_t, x)));
 }
 
 // `seen`: bit h is cleared if half h lies on a page outside the cache
@@ -76,6 +79,7 @@ __device__ __forceinline__ void load_step(Step<BITS, ASYM, D> &s, const TreeArgs
     using S = Step<BITS, ASYM, D>;
     constexpr int R = D * BITS / 8;
     const int t = lane & 15, g = lane >> 4;
+    int64_t rows[2];
     *seen = 3;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -94,32 +98,70 @@ __device__ __forceinline__ void load_step(Step<BITS, ASYM, D> &s, const TreeArgs
             load_words<S::kLoad>(&s.k[h][l * S::kLoad], k + l * 64 + g * 4 * S::kLoad);
             load_words<S::kLoad>(&s.v[h][l * S::kLoad], v + l * 256 + t * 4 * S::kLoad);
         }
-        const int64_t at_scale = (ASYM ? 2 * row : row) + in_page + 4 * g;
-        load_floats(s.ks[h], a.c.k_scales + at_scale);
-        load_floats(s.vs[h], a.c.v_scales + at_scale);
-        if (ASYM) {
-            load_floats(s.kz[h], a.c.k_scales + at_scale + a.c.page_size);
-            load_floats(s.vz[h], a.c.v_scales + at_scale + a.c.page_size);
-        }
+        rows[h] = (ASYM ? 2 : 1) * row + in_page;
+    }
+    const int64_t at_scale = (t & 4 ? rows[1] : rows[0]) + 4 * g + (t & 3);
+    s.ks = a.c.k_scales[at_scale];
+    s.vs = a.c.v_scales[at_scale];
+    if (ASYM) {
+        s.kz = a.c.k_scales[at_scale + a.c.page_size];
+        s.vz = a.c.v_scales[at_scale + a.c.page_size];
     }
 }
 
-// Four codes of a word as whole numbers less half the range, in two pairs: 1024 + u is the fp16 number 0x6400 | u.
-__device__ __forceinline__ void four_codes(uint32_t w, uint32_t *lo, uint32_t *hi)
+// Codes to fp16: 1024 + u is the number 0x6400 | u.  The constants stand in registers of their own, one scalar and one vector, for
+// an operation to take both.
+struct Magic {
+    uint32_t bytes, halves; // 0x64 in every byte, 0x6400 in both halves
+};
+__device__ __forceinline__ Magic magic()
+{
+    Magic m = {0x64646464u, 0x64006400u};
+    asm("" : "+v"(m.bytes), "+v"(m.halves));
+    return m;
+}
+// Four codes of a word less half the range, in two pairs
+__device__ __forceinline__ void four_codes(const Magic &m, uint32_t w, uint32_t *lo, uint32_t *hi)
 {
     const half2v off = {(_Float16)1152, (_Float16)1152};
-    *lo = bits(half2_bits(__builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) - off);
-    *hi = bits(half2_bits(__builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) - off);
+    *lo = bits(half2_bits(__builtin_amdgcn_perm(m.bytes, w, 0x04010400u)) - off);
+    *hi = bits(half2_bits(__builtin_amdgcn_perm(m.bytes, w, 0x04030402u)) - off);
 }
 // Eight 4-bit codes of a word: nibbles (0, 4), (1, 5), (2, 6), (3, 7).  A nibble in bits 4 - 7 stands for 16 times its value.
-__device__ __forceinline__ void eight_codes(uint32_t w, uint32_t *out)
+__device__ __forceinline__ void eight_codes(const Magic &m, uint32_t w, uint32_t *out)
 {
     const half2v off = {(_Float16)1032, (_Float16)1032}, part = {(_Float16)0.0625f, (_Float16)0.0625f}, off16 = {(_Float16)72, (_Float16)72};
     const uint32_t w8 = w >> 8;
-    out[0] = bits(half2_bits((w & 0x000f000fu) | 0x64006400u) - off);
-    out[1] = bits(half2_bits((w & 0x00f000f0u) | 0x64006400u) * part - off16);
-    out[2] = bits(half2_bits((w8 & 0x000f000fu) | 0x64006400u) - off);
-    out[3] = bits(half2_bits((w8 & 0x00f000f0u) | 0x64006400u) * part - off16);
+    out[0] = bits(half2_bits((w & 0x000f000fu) | m.halves) - off);
+    out[1] = bits(half2_bits((w & 0x00f000f0u) | m.halves) * part - off16);
+    out[2] = bits(half2_bits((w8 & 0x000f000fu) | m.halves) - off);
+    out[3] = bits(half2_bits((w8 & 0x00f000f0u) | m.halves) * part - off16);
+}
+
+// score * k_factor + k_offset * qsum + v_log of token K of the lane's eight and of those behind it
+template <bool ASYM, int RT, int K>
+__device__ __forceinline__ void exponents(float (&score)[RT][2][4], float k_factor, float k_offset, float v_log, const float (&qsum)[RT])
+{
+    if constexpr (K < 8) {
+        const float f = of_lane<K>(k_factor), v = of_lane<K>(v_log), o = ASYM ? of_lane<K>(k_offset) : 0.f;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+            score[rt][K / 4][K % 4] = __builtin_fmaf(score[rt][K / 4][K % 4], f, ASYM ? __builtin_fmaf(o, qsum[rt], v) : v);
+        exponents<ASYM, RT, K + 1>(score, k_factor, k_offset, v_log, qsum);
+    }
+}
+// sum + the tokens' weights times their v
+template <int K> __device__ __forceinline__ float weighted_sum(const float (&w)[2][4], float v, float sum)
+{
+    if constexpr (K < 8)
+        return weighted_sum<K + 1>(w, v, __builtin_fmaf(of_lane<K>(v), w[K / 4][K % 4], sum));
+    return sum;
+}
+template <int K> __device__ __forceinline__ float pair_sum(const uint32_t (&w)[4], uint32_t v, float sum)
+{
+    if constexpr (K < 4)
+        return pair_sum<K + 1>(w, v, __builtin_amdgcn_fdot2(half2_bits(w[K]), half2_bits(of_lane<2 * K>(v)), sum, false));
+    return sum;
 }
 
 __device__ __forceinline__ half8v half8_bits(const uint32_t *w)
@@ -135,10 +177,7 @@ template <int BITS, int D> __device__ __forceinline__ int query_offset(int ks, i
     return (ks / kPieces) * (32 * kPieces) + g * 8 * kPieces + (ks % kPieces) * 8;
 }
 
-// Waves per SIMD that the registers are kept to
-constexpr int tree_waves(int bits, bool asym, int d, int rt) { return rt > 1 ? 2 : bits == 8 && asym && d == 128 ? 3 : 4; }
-
-template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(256, tree_waves(BITS, ASYM, D, RT)) void attn_tree_kernel(TreeArgs a)
+template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(256, RT == 1 ? 4 : 2) void attn_tree_kernel(TreeArgs a)
 {
     using S = Step<BITS, ASYM, D>;
     constexpr int kTiles = D / 16; // 16 x 16 tiles of out^T
@@ -167,7 +206,7 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(256, 
     const int32_t *pages = a.page_table + (int64_t)seq * a.max_pages;
     const int last_page = (len - 1) >> a.page_shift; // (len is 0 only without steps)
 
-    // the queries, and what turns their products into exponents of 2
+    // the queries, the power of two that they were divided by, and their sums
     half8v q[RT][D / 32];
     float factor[RT], qsum[RT];
     uint64_t sees[RT];
@@ -176,7 +215,7 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(256, 
         const int row = min(row0 + 16 * rt + t, rows - 1), draft = row / a.group;
         const uint16_t *src = (const uint16_t *)a.q.data + (int64_t)(own.first + draft) * a.q.row_stride + (int64_t)(head * a.group + row % a.group) * a.q.head_stride;
         sees[rt] = a.mask ? a.mask[own.first + draft] : ~0ull >> (63 - draft);
-        factor[rt] = a.scale_log2;
+        factor[rt] = 1.f;
         float sum = 0;
         uint4 w[D / 32];
 #pragma unroll
@@ -192,35 +231,41 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(256, 
                     most = fmaxf(most, fabsf(bf16_value(x[i / 2] >> (16 * (i & 1)) & 0xffff)));
             }
             most = max_across_quarters(most);
-            const int e = most > 0 && most < INFINITY ? 14 - (int)(__builtin_bit_cast(uint32_t, most) >> 23) + 127 : 0; // the largest becomes [2^14, 2^15)
-            factor[rt] = ldexpf(factor[rt], -e);
+            // the largest becomes [2^14, 2^15), if 2^126 gets it there
+            const int e = most > 0 && most < INFINITY ? min(14 + 127 - (int)(__builtin_bit_cast(uint32_t, most) >> 23), 126) : 0;
+            const float up = __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
+            factor[rt] = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
 #pragma unroll
             for (int ks = 0; ks < D / 32; ++ks) {
                 const uint32_t x[4] = {w[ks].x, w[ks].y, w[ks].z, w[ks].w};
                 uint32_t y[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    y[i] = pack16<ABQ_F16>(ldexpf(bf16_value(x[i] & 0xffff), e), ldexpf(bf16_value(x[i] >> 16), e));
+                    y[i] = pack16<ABQ_F16>(bf16_value(x[i] & 0xffff) * up, bf16_value(x[i] >> 16) * up);
                 q[rt][ks] = half8_bits(y);
             }
         } else
 #pragma unroll
             for (int ks = 0; ks < D / 32; ++ks)
                 q[rt][ks] = __builtin_bit_cast(half8v, w[ks]);
+        if (ASYM)
 #pragma unroll
-        for (int ks = 0; ks < D / 32; ++ks)
+            for (int ks = 0; ks < D / 32; ++ks)
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                sum += (float)q[rt][ks][i];
-        qsum[rt] = ASYM ? sum_across_quarters(sum) : 0;
+                for (int i = 0; i < 8; i += 2)
+                    sum = __builtin_amdgcn_fdot2(half2v{q[rt][ks][i], q[rt][ks][i + 1]}, half2v{(_Float16)1, (_Float16)1}, sum, false);
+        qsum[rt] = ASYM ? sum_across_quarters(sum) * factor[rt] : 0;
     }
 
     float4v out[RT][kTiles];
-    float m[RT], l[RT], z[RT];
+    // Weights are 2^(exponent - base + kLift): base follows the running maximum only when that has left it 2^kSlack behind, which
+    // spares nearly every rescaling, and the lift leaves fp16 its normal range down to 2^-24 of the largest weight.
+    constexpr float kSlack = 5, kLift = 10;
+    float base[RT], shift[RT], l[RT], z[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        m[rt] = -INFINITY;
-        l[rt] = z[rt] = 0;
+        base[rt] = -INFINITY;
+        shift[rt] = l[rt] = z[rt] = 0;
 #pragma unroll
         for (int i = 0; i < kTiles; ++i)
             out[rt][i] = float4v{0, 0, 0, 0};
@@ -228,6 +273,7 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(256, 
 
     const int steps = (len + kStep - 1) / kStep;
     const int step0 = (int)((int64_t)steps * part / a.parts.parts) + wave, step1 = (int)((int64_t)steps * (part + 1) / a.parts.parts);
+    const Magic mg = magic();
     auto weigh_step = [&](S &s, int step, uint32_t seen) {
         // scores
         float score[RT][2][4];
@@ -241,47 +287,61 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(256, 
             for (int ks = 0; ks < D / 32; ++ks) {
                 uint32_t w[4];
                 if (BITS == 8) {
-                    four_codes(s.k[h][2 * ks], &w[0], &w[1]);
-                    four_codes(s.k[h][2 * ks + 1], &w[2], &w[3]);
+                    four_codes(mg, s.k[h][2 * ks], &w[0], &w[1]);
+                    four_codes(mg, s.k[h][2 * ks + 1], &w[2], &w[3]);
                 } else
-                    eight_codes(s.k[h][ks], w);
+                    eight_codes(mg, s.k[h][ks], w);
                 const half8v k = half8_bits(w);
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt)
                     acc[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[rt][ks], acc[rt], 0, 0, 0);
             }
-            // (codes are less half their range here, and so is the zero point)
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    score[rt][h][i] = (ASYM ? acc[rt][i] - (s.kz[ASYM ? h : 0][i] - (float)(1 << (BITS - 1))) * qsum[rt] : acc[rt][i]) * (s.ks[h][i] * factor[rt]);
+                    score[rt][h][i] = acc[rt][i] * factor[rt];
         }
-        // what no row sees holds anything: its scales are replaced
+        // The lane's one token: factor and offset of the scores, logarithm and reciprocal of the value scale.  (Codes are less half
+        // their range here, and so are zero points.)  What no row sees holds anything, and is replaced.
         const int at = step * kStep;
-        if (at + kStep > context || seen != 3) {
+        const bool some = at + kStep > context || seen != 3; // (some row does not see some token of the step)
+        if (some) {
+            const int h = t >> 2 & 1;
+            const bool there = at + 16 * h + 4 * g + (t & 3) < len && (seen >> h & 1);
+            s.ks = there ? s.ks : 0.f;
+            s.vs = there ? s.vs : 1.f;
+            if (ASYM) {
+                s.kz = there ? s.kz : 0.f;
+                s.vz = there ? s.vz : 0.f;
+            }
+        }
+        constexpr float kHalf = (float)(1 << (BITS - 1));
+        const float k_factor = s.ks * a.scale_log2, k_offset = ASYM ? k_factor * (kHalf - s.kz) : 0.f;
+        const float v_log = __builtin_amdgcn_logf(s.vs), v_recip = __builtin_amdgcn_rcpf(s.vs);
+        // Zero points as fp16 pairs: whole numbers beyond fp16's 2048 in two parts, multiples of 2048 and the rest
+        uint32_t z_low = 0, z_high = 0;
+        bool high = false;
+        if constexpr (ASYM) {
+            const float x = s.vz - kHalf, xh = rintf(x * (1.f / 2048)) * 2048.f;
+            const float y = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0xb1, 0xf, 0xf, true)); // of lane t ^ 1
+            const float yh = rintf(y * (1.f / 2048)) * 2048.f;
+            z_low = pack16<ABQ_F16>(x - xh, y - yh); // (used of even lanes)
+            z_high = pack16<ABQ_F16>(xh, yh);
+            high = __any(xh != 0);
+        }
+        exponents<ASYM, RT, 0>(score, k_factor, k_offset, v_log, qsum);
+        if (some)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int pos = at + 16 * h + 4 * g + i;
                     const bool there = pos < len && (seen >> h & 1);
-                    s.vs[h][i] = there ? s.vs[h][i] : 1.f;
-                    if (ASYM)
-                        s.vz[ASYM ? h : 0][i] = there ? s.vz[ASYM ? h : 0][i] : 0.f;
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt)
                         score[rt][h][i] = there && (pos < context || (sees[rt] >> ((pos - context) & 63) & 1)) ? score[rt][h][i] : -INFINITY;
                 }
-        }
-        float v_log[2][4], v_recip[2][4];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v_log[h][i] = __builtin_amdgcn_logf(s.vs[h][i]);
-                v_recip[h][i] = __builtin_amdgcn_rcpf(s.vs[h][i]);
-            }
         // weights
         half8v w[RT];
 #pragma unroll
@@ -290,36 +350,34 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(256, 
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    score[rt][h][i] += v_log[h][i];
+                for (int i = 0; i < 4; ++i)
                     most = fmaxf(most, score[rt][h][i]);
-                }
-            most = fmaxf(max_across_quarters(most), m[rt]);
-            const float base = most == -INFINITY ? 0.f : most;
-            if (__any(most > m[rt])) {
-                const float down = __builtin_amdgcn_exp2f(m[rt] - base);
+            most = max_across_quarters(most);
+            if (__any(most > base[rt] + kSlack)) {
+                const float to = fmaxf(most, base[rt]);
+                const float down = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(base[rt] - to);
+                base[rt] = to;
+                shift[rt] = to == -INFINITY ? 0.f : kLift - to;
                 l[rt] *= down;
                 z[rt] *= down;
 #pragma unroll
                 for (int i = 0; i < kTiles; ++i)
                     out[rt][i] *= down;
             }
-            m[rt] = most;
             uint32_t pair[4];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                float x[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x[i] = __builtin_amdgcn_exp2f(score[rt][h][i] - base);
-                    l[rt] += x[i] * v_recip[h][i];
-                }
-                pair[2 * h] = pack16<ABQ_F16>(x[0], x[1]);
-                pair[2 * h + 1] = pack16<ABQ_F16>(x[2], x[3]);
-                if (ASYM) // with the weights as they are multiplied, so that the two sums' difference has no error of its own
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        z[rt] += f16_value(pair[2 * h + i / 2] >> (16 * (i & 1)) & 0xffff) * (s.vz[ASYM ? h : 0][i] - (float)(1 << (BITS - 1)));
+                for (int i = 0; i < 4; ++i)
+                    score[rt][h][i] = __builtin_amdgcn_exp2f(score[rt][h][i] + shift[rt]);
+                pair[2 * h] = pack16<ABQ_F16>(score[rt][h][0], score[rt][h][1]);
+                pair[2 * h + 1] = pack16<ABQ_F16>(score[rt][h][2], score[rt][h][3]);
+            }
+            l[rt] = weighted_sum<0>(score[rt], v_recip, l[rt]);
+            if constexpr (ASYM) { // with the weights as they are multiplied, so that the two sums' difference has no error of its own
+                z[rt] = pair_sum<0>(pair, z_low, z[rt]);
+                if (high)
+                    z[rt] = pair_sum<0>(pair, z_high, z[rt]);
             }
             w[rt] = half8_bits(pair);
         }
@@ -328,16 +386,16 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(256, 
         for (int j = 0; j < S::kWords; ++j) {
             if (BITS == 8) {
                 uint32_t x[4];
-                four_codes(s.v[0][j], &x[0], &x[1]);
-                four_codes(s.v[1][j], &x[2], &x[3]);
+                four_codes(mg, s.v[0][j], &x[0], &x[1]);
+                four_codes(mg, s.v[1][j], &x[2], &x[3]);
                 const half8v v = half8_bits(x);
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt)
                     out[rt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[rt], out[rt][j], 0, 0, 0);
             } else {
                 uint32_t x[4], y[4];
-                eight_codes(s.v[0][j], x);
-                eight_codes(s.v[1][j], y);
+                eight_codes(mg, s.v[0][j], x);
+                eight_codes(mg, s.v[1][j], y);
                 const uint32_t low[4] = {x[0], x[2], y[0], y[2]}, high[4] = {x[1], x[3], y[1], y[3]};
                 const half8v v0 = half8_bits(low), v1 = half8_bits(high);
 #pragma unroll
@@ -349,7 +407,7 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(256, 
         }
     };
     // One row tile leaves registers for four waves per SIMD, which cover each other's loads; with more, a wave loads a step ahead.
-    if constexpr (RT == 1 || (ASYM && D == 128)) {
+    if constexpr (RT == 1) {
         for (int step = step0; step < step1; step += kWaves) {
             S s;
             uint32_t seen;
@@ -378,7 +436,7 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(256, 
     for (int rt = 0; rt < RT; ++rt) {
         const float total = sum_across_quarters(l[rt]), zeros = ASYM ? sum_across_quarters(z[rt]) : 0;
         if (g == 0) {
-            stat_m[wave][16 * rt + t] = m[rt];
+            stat_m[wave][16 * rt + t] = base[rt] == -INFINITY ? -INFINITY : -shift[rt];
             stat_l[wave][16 * rt + t] = total;
             stat_z[wave][16 * rt + t] = zeros;
         }
@@ -401,13 +459,13 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(256, 
 #pragma unroll
         for (int w = 0; w < kWaves; ++w)
             most = fmaxf(most, stat_m[w][16 * rt + r]);
-        const float base = most == -INFINITY ? 0.f : most;
+        const float from = most == -INFINITY ? 0.f : most;
 #pragma unroll
         for (int e = 0; e < kEach; ++e)
             acc[e] = 0;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-            const float f = __builtin_amdgcn_exp2f(stat_m[w][16 * rt + r] - base);
+            const float f = __builtin_amdgcn_exp2f(stat_m[w][16 * rt + r] - from);
             total += f * stat_l[w][16 * rt + r];
 #pragma unroll
             for (int e = 0; e < kEach; ++e)
