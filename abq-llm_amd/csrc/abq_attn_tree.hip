@@ -567,8 +567,15 @@ void plan_attn_tree(abq_attn_state *st, int most_parts)
     st->block_rows = rows <= 16 ? 16 : 32;
     const int64_t units = (int64_t)st->seqs * st->kv_heads * ((rows + st->block_rows - 1) / st->block_rows);
     const int64_t steps = ((int64_t)st->max_k + kStep - 1) / kStep;
-    int64_t parts = units > 0 ? (1024 + units - 1) / units : 1;
+    // Two workgroups per compute unit, no wave without a step; below 24 steps the second launch costs more than parts save (20
+    // sequences of 700 tokens and 8 heads: 9.8 us, in three parts 10.9).  One sequence of 8000 and 32 heads: in 1, 4, 16, 32 parts
+    // 66, 25, 17, 18 us; 16 sequences of 1024 and 32 heads in 1, 2, 4: 24.8, 27.6, 29.9.
+    int64_t parts = steps > 24 ? 512 / units : 1;
     parts = parts < steps / kWaves ? parts : steps / kWaves;
+    // A wave has 32 steps at most, so that sequences much longer than the others are spread: 48 of up to 16384 tokens and 8 heads in
+    // 1, 3, 5, 8 parts 229, 163, 153, 147 us, while 30 of 4000 and 32 heads take 177 - 186 in any number.
+    const int64_t spread = (steps + 32 * kWaves - 1) / (32 * kWaves);
+    parts = parts > spread ? parts : spread;
     parts = parts < most_parts ? parts : most_parts;
     st->parts = parts < 1 ? 1 : (int)parts;
 }
