@@ -14,6 +14,7 @@ if "abq_gemm" not in sys.modules:
     sys.modules["abq_gemm"] = _module
     _spec.loader.exec_module(_module)
 import abq_gemm  # noqa: E402
+import torch  # noqa: E402
 
 AbqError = abq_gemm.AbqError
 F16, BF16 = 0, 1
@@ -78,22 +79,23 @@ def _check(status, what):
         raise AbqError(status, what)
 
 
+_DTYPES = {torch.float16: F16, torch.bfloat16: BF16}
+
+
 def _dtype(t):
-    import torch
-    if t.dtype == torch.float16:
-        return F16
-    if t.dtype == torch.bfloat16:
-        return BF16
-    raise TypeError("fp16 or bf16 is wanted, got %s" % t.dtype)
+    if t.dtype not in _DTYPES:
+        raise TypeError("fp16 or bf16 is wanted, got %s" % t.dtype)
+    return _DTYPES[t.dtype]
 
 
 def _rows(t):
     """A device tensor [rows, heads, head dim] as the library sees it"""
-    if not t.is_cuda or t.dim() != 3:
+    strides = t.stride()
+    if len(strides) != 3 or not t.is_cuda:
         raise ValueError("a device tensor [rows, heads, head dim] is wanted")
-    if t.shape[2] > 1 and t.stride(2) != 1:
+    if strides[2] != 1:
         raise ValueError("the elements of a head have to lie beside each other")
-    return Rows(t.data_ptr(), t.shape[0], t.stride(0), t.stride(1))
+    return Rows(t.data_ptr(), t.shape[0], strides[0], strides[1])
 
 
 def _index(t, dtype, numel, what):
@@ -108,7 +110,6 @@ class KvCache:
     A token's place is its slot, page * page_size + offset."""
 
     def __init__(self, num_pages, page_size, kv_heads, head_dim, bits=8, symmetric=True, device="cuda"):
-        import torch
         d = KvCacheDesc(bits, int(bool(symmetric)), kv_heads, head_dim, page_size, num_pages)
         codes, scales = lib().abq_kv_codes_bytes(ctypes.byref(d)), lib().abq_kv_scales_bytes(ctypes.byref(d))
         if not codes:
@@ -117,33 +118,33 @@ class KvCache:
         self.k_scales, self.v_scales = (torch.ones(scales // 4, dtype=torch.float32, device=device) for _ in range(2))
         d.k_codes, d.v_codes, d.k_scales, d.v_scales = (t.data_ptr() for t in (self.k_codes, self.v_codes, self.k_scales, self.v_scales))
         self.desc = d
+        self._ref, self._row = ctypes.byref(d), (kv_heads, head_dim)
+        self._append, self._read = lib().abq_kv_append, lib().abq_kv_read
 
-    def _call(self, name, k, v, slots, stream):
-        import torch
-        d = self.desc
-        if k.shape != v.shape or k.dtype != v.dtype or tuple(k.shape[1:]) != (d.kv_heads, d.head_dim):
-            raise ValueError("keys and values [tokens, %d, %d] of one type are wanted" % (d.kv_heads, d.head_dim))
-        rk, rv = _rows(k), _rows(v)
-        at = _index(slots, torch.int32, k.shape[0], "slots")
-        _check(getattr(lib(), name)(ctypes.byref(d), ctypes.byref(rk), ctypes.byref(rv), _dtype(k), at, abq_gemm._stream_ptr(stream)), name)
+    def _call(self, call, name, k, v, slots, stream):
+        shape = k.shape
+        if shape != v.shape or k.dtype is not v.dtype or shape[1:] != self._row:
+            raise ValueError("keys and values [tokens, %d, %d] of one type are wanted" % self._row)
+        at = _index(slots, torch.int32, shape[0], "slots")
+        status = call(self._ref, ctypes.byref(_rows(k)), ctypes.byref(_rows(v)), _dtype(k), at, abq_gemm._stream_ptr(stream))
+        if status:
+            raise AbqError(status, name)
 
     def append(self, k, v, slots, stream=None):
         """Quantises k and v [tokens, kv heads, head dim] and writes token i at slots[i] (int32; outside the cache: dropped)."""
-        self._call("abq_kv_append", k, v, slots, stream)
+        self._call(self._append, "abq_kv_append", k, v, slots, stream)
 
     def read(self, slots, dtype=None, out=None, stream=None):
         """(k, v) [tokens, kv heads, head dim] of the tokens at these slots, in fp16 (or dtype), or into out = (k, v)."""
-        import torch
         if out is None:
-            shape = (slots.numel(), self.desc.kv_heads, self.desc.head_dim)
+            shape = (slots.numel(),) + self._row
             out = tuple(torch.empty(shape, dtype=dtype or torch.float16, device=slots.device) for _ in range(2))
-        self._call("abq_kv_read", out[0], out[1], slots, stream)
+        self._call(self._read, "abq_kv_read", out[0], out[1], slots, stream)
         return out
 
 
 class _Attention:
     def _finish(self, out, workspace):
-        import torch
         self.out = out
         need = self.workspace_bytes
         if workspace is None and need:
@@ -160,7 +161,9 @@ class _Attention:
 
     def run(self, stream=None):
         """One pass over what the tensors hold now; returns out."""
-        _check(self._exec(self._state, abq_gemm._stream_ptr(stream)), "abq_attn_exec")
+        status = self._exec(self._state, abq_gemm._stream_ptr(stream))
+        if status:
+            raise AbqError(status, "abq_attn_exec")
         return self.out
 
 
@@ -171,7 +174,6 @@ class PromptAttention(_Attention):
     is made, an empty tensor means none."""
 
     def __init__(self, q, k, v, q_starts, k_starts=None, max_q=None, max_k=None, scale=None, out=None, workspace=None):
-        import torch
         if k.shape != v.shape or k.shape[2] != q.shape[2] or not (q.dtype == k.dtype == v.dtype):
             raise ValueError("q [tokens, heads, head dim], k and v [tokens, kv heads, head dim] of one type are wanted")
         if out is None:
@@ -196,7 +198,6 @@ class TreeAttention(_Attention):
     those before it and itself.  max_q, max_context: bounds of a sequence's drafts (at most 64) and context."""
 
     def __init__(self, q, cache, page_table, context, q_starts, max_q, max_context, mask=None, scale=None, out=None, workspace=None):
-        import torch
         d = cache.desc
         if q.dim() != 3 or q.shape[2] != d.head_dim:
             raise ValueError("q [drafts, heads, %d] is wanted" % d.head_dim)
