@@ -1,11 +1,10 @@
 // The quantised key / value cache: rows of new tokens quantised per token and head as they are written, and read back.
 // The layout and the formulas are those stated in abq_attention.h.
 //
-// A row (64 or 128 elements) is held by 8 or 16 lanes, 8 elements each, so a wave holds 8 or 4 consecutive tokens of one head.  It
-// takes their keys and values for two heads, all requested at once: four loads of 16 bytes per lane in flight, and a quarter of
-// the workgroups that one row each would take.  Extrema go over a row's lanes, and the four tokens that the values' layout puts
-// beside each other change places, by lane permutes without LDS.  Bound by memory: 2 bytes per element read and bits / 8 written
-// (and the other way round when read back).
+// A row (64 or 128 elements) is held by 8 or 16 lanes, 8 elements each, so a wave holds 8 or 4 consecutive tokens of one head, and
+// takes their keys and their values, requested together.  Extrema go over a row's lanes, and the four tokens that the values'
+// layout puts beside each other change places, by lane permutes without LDS.  Bound by memory: 2 bytes per element read and
+// bits / 8 written (and the other way round when read back).
 #include "abq_attn.h"
 #include "abq_quant.h"
 
@@ -18,11 +17,8 @@ struct CacheArgs {
     abq_rows k, v;
     const int32_t *slots;
     int tokens, groups;  // groups: of the consecutive tokens that a wave holds
-    int head_groups;     // of kHeads heads
     int page_shift;
 };
-
-constexpr int kHeads = 2;
 
 template <int CTRL> __device__ __forceinline__ uint32_t dpp(uint32_t x)
 {
@@ -60,13 +56,13 @@ template <int D> __device__ __forceinline__ uint32_t transpose_bytes(uint32_t ow
     }
 }
 
-// The lane's token and its wave's first head; heads come first, so that the waves of a workgroup read neighbouring heads of
+// The lane's token and its wave's head; heads come first, so that the waves of a workgroup read neighbouring heads of
 // the same tokens.
 template <int D> __device__ __forceinline__ bool place(const CacheArgs &a, int lane, int *token, int *head)
 {
-    const uint32_t unit = blockIdx.x * 4 + (threadIdx.x >> 6), group = unit / a.head_groups;
+    const uint32_t unit = blockIdx.x * 4 + (threadIdx.x >> 6), group = unit / a.c.kv_heads;
     *token = group * (512 / D) + lane / (D / 8);
-    *head = unit % a.head_groups * kHeads;
+    *head = unit % a.c.kv_heads;
     return group < (uint32_t)a.groups;
 }
 
@@ -80,13 +76,8 @@ template <int DTYPE, int BITS, int D> __global__ __launch_bounds__(256) void kv_
     if (!place<D>(a, lane, &token, &head))
         return;
     const int from = min(token, a.tokens - 1);
-    uint4 w[kHeads][2];
-#pragma unroll
-    for (int h = 0; h < kHeads; ++h) {
-        const int at = min(head + h, a.c.kv_heads - 1);
-        w[h][0] = *(const uint4 *)((const uint16_t *)a.k.data + (int64_t)from * a.k.row_stride + (int64_t)at * a.k.head_stride + 8 * li);
-        w[h][1] = *(const uint4 *)((const uint16_t *)a.v.data + (int64_t)from * a.v.row_stride + (int64_t)at * a.v.head_stride + 8 * li);
-    }
+    const uint4 w[2] = {*(const uint4 *)((const uint16_t *)a.k.data + (int64_t)from * a.k.row_stride + (int64_t)head * a.k.head_stride + 8 * li),
+                        *(const uint4 *)((const uint16_t *)a.v.data + (int64_t)from * a.v.row_stride + (int64_t)head * a.v.head_stride + 8 * li)};
     const int slot = token < a.tokens ? a.slots[from] : -1;
     const bool there = slot >= 0 && (slot >> a.page_shift) < a.c.num_pages;
     const int page = slot >> a.page_shift, t = slot & (a.c.page_size - 1);
@@ -98,90 +89,87 @@ template <int DTYPE, int BITS, int D> __global__ __launch_bounds__(256) void kv_
     const bool whole = (wholes & quad_lanes) == quad_lanes;
 
 #pragma unroll
-    for (int h = 0; h < kHeads; ++h)
+    for (int kv = 0; kv < 2; ++kv) {
+        const uint32_t words[4] = {w[kv].x, w[kv].y, w[kv].z, w[kv].w};
+        float x[8];
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-            const uint32_t words[4] = {w[h][kv].x, w[h][kv].y, w[h][kv].z, w[h][kv].w};
-            float x[8];
+        for (int i = 0; i < 8; ++i)
+            x[i] = value16<DTYPE>(words[i / 2] >> (16 * (i & 1)));
+        uint32_t code[8];
+        QuantRow q;
+        if (a.c.symmetric) {
+            float mx = 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                x[i] = value16<DTYPE>(words[i / 2] >> (16 * (i & 1)));
-            uint32_t code[8];
-            QuantRow q;
-            if (a.c.symmetric) {
-                float mx = 0;
+                mx = fmaxf(mx, fabsf(x[i]));
+            q = quant_row_params(max_of_row<D>(mx), 0.f, BITS, 1);
+        } else {
+            float mx = x[0], mn = -x[0];
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    mx = fmaxf(mx, fabsf(x[i]));
-                q = quant_row_params(max_of_row<D>(mx), 0.f, BITS, 1);
-            } else {
-                float mx = x[0], mn = -x[0];
-#pragma unroll
-                for (int i = 1; i < 8; ++i) {
-                    mx = fmaxf(mx, x[i]);
-                    mn = fmaxf(mn, -x[i]);
-                }
-                q = quant_row_params(max_of_row<D>(mx), -max_of_row<D>(mn), BITS, 0);
+            for (int i = 1; i < 8; ++i) {
+                mx = fmaxf(mx, x[i]);
+                mn = fmaxf(mn, -x[i]);
             }
+            q = quant_row_params(max_of_row<D>(mx), -max_of_row<D>(mn), BITS, 0);
+        }
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                code[i] = (quant_code_bits(x[i], q) ^ kHalf) & (2 * kHalf - 1);
+        for (int i = 0; i < 8; ++i)
+            code[i] = (quant_code_bits(x[i], q) ^ kHalf) & (2 * kHalf - 1);
 
-            const bool mine = there && head + h < a.c.kv_heads;
-            const int64_t row = ((int64_t)page * a.c.kv_heads + head + h) * a.c.page_size; // the head's first row in its page
-            if (mine && li == 0) {
-                float *scales = kv ? a.c.v_scales : a.c.k_scales;
-                if (a.c.symmetric)
-                    scales[row + t] = q.scale;
-                else {
-                    scales[2 * row + t] = q.scale;
-                    scales[2 * row + a.c.page_size + t] = q.zero_out + (float)kHalf;
-                }
-            }
-            if (kv == 0) {
-                uint8_t *dst = (uint8_t *)a.c.k_codes + (row + t) * R;
-                if (BITS == 8) {
-                    if (mine)
-                        *(uint2 *)(dst + 8 * li) = uint2{code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24,
-                                                         code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24};
-                } else if (mine) // nibbles 0, 4, 1, 5, 2, 6, 3, 7
-                    *(uint32_t *)(dst + 4 * li) =
-                        code[0] | code[1] << 16 | code[2] << 4 | code[3] << 20 | code[4] << 8 | code[5] << 24 | code[6] << 12 | code[7] << 28;
-                continue;
-            }
-            // values: byte columns, four tokens beside each other
-            constexpr int kCols = BITS == 8 ? 8 : 4; // columns of a lane
-            uint32_t cols[2];
-            int c0; // the lane's first column
-            cols[0] = code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24;
-            cols[1] = code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24;
-            if (BITS == 8)
-                c0 = 8 * li;
+        const int64_t row = ((int64_t)page * a.c.kv_heads + head) * a.c.page_size; // the head's first row in its page
+        if (there && li == 0) {
+            float *scales = kv ? a.c.v_scales : a.c.k_scales;
+            if (a.c.symmetric)
+                scales[row + t] = q.scale;
             else {
-                // a column holds elements d and d + D / 2: of the eight columns that this lane and its partner share, the lower
-                // lane takes the first four
-                const uint32_t low2 = __shfl_xor(cols[0], kLanes / 2), high2 = __shfl_xor(cols[1], kLanes / 2);
-                const bool upper = li >= kLanes / 2;
-                cols[0] = upper ? high2 | cols[1] << 4 : cols[0] | low2 << 4;
-                c0 = 8 * (li % (kLanes / 2)) + (upper ? 4 : 0);
-            }
-            uint8_t *dst = (uint8_t *)a.c.v_codes + (row + (t & ~3)) * R; // the four tokens' columns
-            if (whole) {
-#pragma unroll
-                for (int j = 0; j < kCols / 4; ++j) {
-                    uint32_t word = transpose_bytes<D>(cols[j], quad);
-                    if (BITS == 4)
-                        word = __builtin_amdgcn_perm(word, word, 0x03010200u);
-                    if (mine)
-                        *(uint32_t *)(dst + (c0 + 4 * j + quad) * 4) = word;
-                }
-            } else if (mine) {
-                const int at = BITS == 8 ? t & 3 : (t & 1) << 1 | (t >> 1 & 1);
-#pragma unroll
-                for (int j = 0; j < kCols; ++j)
-                    dst[(c0 + j) * 4 + at] = (uint8_t)(cols[j / 4] >> (8 * (j & 3)));
+                scales[2 * row + t] = q.scale;
+                scales[2 * row + a.c.page_size + t] = q.zero_out + (float)kHalf;
             }
         }
+        if (kv == 0) {
+            uint8_t *dst = (uint8_t *)a.c.k_codes + (row + t) * R;
+            if (BITS == 8) {
+                if (there)
+                    *(uint2 *)(dst + 8 * li) = uint2{code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24,
+                                                     code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24};
+            } else if (there) // nibbles 0, 4, 1, 5, 2, 6, 3, 7
+                *(uint32_t *)(dst + 4 * li) =
+                    code[0] | code[1] << 16 | code[2] << 4 | code[3] << 20 | code[4] << 8 | code[5] << 24 | code[6] << 12 | code[7] << 28;
+            continue;
+        }
+        // values: byte columns, four tokens beside each other
+        constexpr int kCols = BITS == 8 ? 8 : 4; // columns of a lane
+        uint32_t cols[2];
+        int c0; // the lane's first column
+        cols[0] = code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24;
+        cols[1] = code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24;
+        if (BITS == 8)
+            c0 = 8 * li;
+        else {
+            // a column holds elements d and d + D / 2: of the eight columns that this lane and its partner share, the lower
+            // lane takes the first four
+            const uint32_t low2 = __shfl_xor(cols[0], kLanes / 2), high2 = __shfl_xor(cols[1], kLanes / 2);
+            const bool upper = li >= kLanes / 2;
+            cols[0] = upper ? high2 | cols[1] << 4 : cols[0] | low2 << 4;
+            c0 = 8 * (li % (kLanes / 2)) + (upper ? 4 : 0);
+        }
+        uint8_t *dst = (uint8_t *)a.c.v_codes + (row + (t & ~3)) * R; // the four tokens' columns
+        if (whole) {
+#pragma unroll
+            for (int j = 0; j < kCols / 4; ++j) {
+                uint32_t word = transpose_bytes<D>(cols[j], quad);
+                if (BITS == 4)
+                    word = __builtin_amdgcn_perm(word, word, 0x03010200u);
+                if (there)
+                    *(uint32_t *)(dst + (c0 + 4 * j + quad) * 4) = word;
+            }
+        } else if (there) {
+            const int at = BITS == 8 ? t & 3 : (t & 1) << 1 | (t >> 1 & 1);
+#pragma unroll
+            for (int j = 0; j < kCols; ++j)
+                dst[(c0 + j) * 4 + at] = (uint8_t)(cols[j / 4] >> (8 * (j & 3)));
+        }
+    }
 }
 
 template <int DTYPE, int BITS, int D> __global__ __launch_bounds__(256) void kv_read_kernel(CacheArgs a)
@@ -196,49 +184,40 @@ template <int DTYPE, int BITS, int D> __global__ __launch_bounds__(256) void kv_
     const bool there = slot >= 0 && (slot >> a.page_shift) < a.c.num_pages;
     const int page = there ? slot >> a.page_shift : 0, t = slot & (a.c.page_size - 1);
     const int c0 = BITS == 8 ? 8 * li : 8 * (li % (kLanes / 2)); // the first of the lane's eight columns of values
-    uint2 kw[kHeads];
-    uint4 vw[kHeads][2]; // (the lanes of the neighbouring tokens read the same words)
-    float scale[kHeads][2], zero[kHeads][2];
-#pragma unroll
-    for (int h = 0; h < kHeads; ++h) {
-        const int64_t row = ((int64_t)page * a.c.kv_heads + min(head + h, a.c.kv_heads - 1)) * a.c.page_size;
-        const uint8_t *k = (const uint8_t *)a.c.k_codes + (row + t) * R, *v = (const uint8_t *)a.c.v_codes + (row + (t & ~3)) * R + c0 * 4;
-        kw[h] = BITS == 8 ? *(const uint2 *)(k + 8 * li) : uint2{*(const uint32_t *)(k + 4 * li), 0};
-        vw[h][0] = *(const uint4 *)v;
-        vw[h][1] = *(const uint4 *)(v + 16);
-        const int64_t at = a.c.symmetric ? row + t : 2 * row + t;
-        scale[h][0] = a.c.k_scales[at];
-        scale[h][1] = a.c.v_scales[at];
-        zero[h][0] = a.c.symmetric ? (float)(1 << (BITS - 1)) : a.c.k_scales[at + a.c.page_size];
-        zero[h][1] = a.c.symmetric ? (float)(1 << (BITS - 1)) : a.c.v_scales[at + a.c.page_size];
+    const int64_t row = ((int64_t)page * a.c.kv_heads + head) * a.c.page_size;
+    const uint8_t *k = (const uint8_t *)a.c.k_codes + (row + t) * R, *v = (const uint8_t *)a.c.v_codes + (row + (t & ~3)) * R + c0 * 4;
+    const uint2 kw = BITS == 8 ? *(const uint2 *)(k + 8 * li) : uint2{*(const uint32_t *)(k + 4 * li), 0};
+    const uint4 vw[2] = {*(const uint4 *)v, *(const uint4 *)(v + 16)}; // (the lanes of the neighbouring tokens read the same words)
+    const int64_t at_scale = a.c.symmetric ? row + t : 2 * row + t;
+    const float scale[2] = {a.c.k_scales[at_scale], a.c.v_scales[at_scale]};
+    float zero[2] = {(float)(1 << (BITS - 1)), (float)(1 << (BITS - 1))};
+    if (!a.c.symmetric) {
+        zero[0] = a.c.k_scales[at_scale + a.c.page_size];
+        zero[1] = a.c.v_scales[at_scale + a.c.page_size];
     }
 #pragma unroll
-    for (int h = 0; h < kHeads; ++h)
+    for (int kv = 0; kv < 2; ++kv) {
+        uint32_t code[8];
+        if (kv == 0) {
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-            uint32_t code[8];
-            if (kv == 0) {
+            for (int i = 0; i < 8; ++i)
+                code[i] = BITS == 8 ? (i < 4 ? kw.x : kw.y) >> (8 * (i & 3)) & 255 : kw.x >> (16 * (i & 1) + 4 * (i / 2)) & 15;
+        } else {
+            const uint32_t w[8] = {vw[0].x, vw[0].y, vw[0].z, vw[0].w, vw[1].x, vw[1].y, vw[1].z, vw[1].w};
+            const int at = BITS == 8 ? 8 * (t & 3) : 8 * ((t & 1) << 1 | (t >> 1 & 1)) + (li >= kLanes / 2 ? 4 : 0);
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    code[i] = BITS == 8 ? (i < 4 ? kw[h].x : kw[h].y) >> (8 * (i & 3)) & 255 : kw[h].x >> (16 * (i & 1) + 4 * (i / 2)) & 15;
-            } else {
-                const uint32_t w[8] = {vw[h][0].x, vw[h][0].y, vw[h][0].z, vw[h][0].w, vw[h][1].x, vw[h][1].y, vw[h][1].z, vw[h][1].w};
-                const int at = BITS == 8 ? 8 * (t & 3) : 8 * ((t & 1) << 1 | (t >> 1 & 1)) + (li >= kLanes / 2 ? 4 : 0);
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    code[i] = w[i] >> at & ((1 << BITS) - 1);
-            }
-            uint32_t out[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t two = pack16<DTYPE>(((float)code[2 * i] - zero[h][kv]) * scale[h][kv], ((float)code[2 * i + 1] - zero[h][kv]) * scale[h][kv]);
-                out[i] = there ? two : 0;
-            }
-            const abq_rows &dst = kv ? a.v : a.k;
-            if (head + h < a.c.kv_heads)
-                *(uint4 *)((uint16_t *)dst.data + (int64_t)token * dst.row_stride + (int64_t)(head + h) * dst.head_stride + 8 * li) =
-                    uint4{out[0], out[1], out[2], out[3]};
+            for (int i = 0; i < 8; ++i)
+                code[i] = w[i] >> at & ((1 << BITS) - 1);
         }
+        uint32_t out[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t two = pack16<DTYPE>(((float)code[2 * i] - zero[kv]) * scale[kv], ((float)code[2 * i + 1] - zero[kv]) * scale[kv]);
+            out[i] = there ? two : 0;
+        }
+        const abq_rows &dst = kv ? a.v : a.k;
+        *(uint4 *)((uint16_t *)dst.data + (int64_t)token * dst.row_stride + (int64_t)head * dst.head_stride + 8 * li) = uint4{out[0], out[1], out[2], out[3]};
+    }
 }
 
 bool cache_args(const abq_kv_cache &c, const abq_rows &k, const abq_rows &v, const int32_t *slots, CacheArgs *a, dim3 *grid)
@@ -251,8 +230,7 @@ bool cache_args(const abq_kv_cache &c, const abq_rows &k, const abq_rows &v, con
     const int rows = 512 / c.head_dim;
     a->groups = (a->tokens + rows - 1) / rows;
     a->page_shift = __builtin_ctz((unsigned)c.page_size);
-    a->head_groups = (c.kv_heads + kHeads - 1) / kHeads;
-    *grid = dim3((unsigned)(((int64_t)a->groups * a->head_groups + 3) / 4));
+    *grid = dim3((unsigned)(((int64_t)a->groups * c.kv_heads + 3) / 4));
     return a->tokens > 0;
 }
 
