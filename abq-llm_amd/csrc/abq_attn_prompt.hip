@@ -1,7 +1,6 @@
 // Causal attention of packed prompts with grouped heads.
 //
-// A workgroup takes a block of one sequence's queries and one head, its four waves 32 (or 64) queries each, and goes over the
-// keys in tiles of 64 tokens with the running maximum and sum of the softmax.  Both products are taken transposed,
+// A workgroup takes a block of one sequence's queries and one head, a wave 32 queries, and goes over the keys in tiles of 64 tokens with the running maximum and sum of the softmax.  Both products are taken transposed,
 // S^T = K q^T and out^T = V^T P^T (32 x 32 x 16 MFMA): lane (i, h) of the first result holds the scores of query i for tokens
 // 8 j + 4 h .. + 3, which are, eight at a time, an operand of the second product as they are, if the values' tokens
 // come in the same order; so P never leaves its registers, and a query's statistics are two lanes'.  The values are
@@ -14,6 +13,8 @@
 // P is rounded to the type of the inputs for the second product; its sum is taken in fp32 before that.
 #include "abq_attn.h"
 #include "abq_lds_dma.h"
+
+#include <type_traits>
 
 namespace abq {
 
@@ -49,188 +50,170 @@ template <int DTYPE> __device__ __forceinline__ uint32_t not_finite(uint32_t pai
     return (DTYPE == ABQ_BF16 ? (pair & 0x7f807f80u) + 0x00800080u : (pair & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
 }
 
-// KG = 1: the four waves share the queries, 32 QT each.  KG = 2: two waves do, and the other two take the other 32 tokens of each
-// tile; their results are joined at the end.
-template <int DTYPE, int D, int QT, int KG> __global__ __launch_bounds__(256, 3 - QT) void attn_prompt_kernel(PromptArgs a)
+// KG = 1: the four waves share 128 queries, 32 each.  KG = 2: two waves share 64, and the other two take the other 32 tokens of
+// each tile; their results are joined at the end.
+template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(PromptArgs a)
 {
-    constexpr int kBlock = 128 * QT / KG;       // queries of the workgroup
+    constexpr int kBlock = 128 / KG;            // queries of the workgroup
     constexpr int TT = 2 / KG;                  // a wave's 32-token parts of a tile
     constexpr int kPieces = D / 8;              // of a row
     constexpr int kTile = kTokens * D * 2;      // bytes
     constexpr int kLoads = kTile / 1024 / 4;    // of a wave per tile
-    __shared__ __align__(1024) uint8_t lds[4][kTile]; // keys of even and odd tiles, values of even and odd tiles
+    __shared__ __align__(1024) uint8_t lds[4][kTile]; // keys of two tiles, values of two tiles
     __shared__ int odd_values[4];
-    static_assert(KG == 1 || 4 * kTile >= 64 * QT * (D + 4) * 4, "the waves' sums fit where the tiles were");
+    static_assert(KG == 1 || 4 * kTile >= 64 * (D + 4) * 4, "the waves' sums fit where the tiles were");
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ql = lane & 31, half = lane >> 5;
-    // Blocks with the most keys first.  Heads that share keys are kv_heads apart, so with 8 key heads (or a multiple) each
+    // Blocks with the most keys first.  Where all run beside each other, two to a compute unit, the second half comes the other way
+    // round, so that every unit has the same.  Heads that share keys are kv_heads apart, so with 8 key heads (or a multiple) each
     // stays with one XCD's L2.
+    const uint32_t at = gridDim.x <= 512 && blockIdx.x >= 256 ? 255 + gridDim.x - blockIdx.x : blockIdx.x;
     const uint32_t per_block = a.heads * a.seqs;
-    const int part = blockIdx.x / per_block % a.parts.parts, block = a.blocks - 1 - (int)(blockIdx.x / per_block / a.parts.parts);
+    const int part = at / per_block % a.parts.parts, block = a.blocks - 1 - (int)(at / per_block / a.parts.parts);
     const int kg = wave / (4 / KG);
-    const int seq = blockIdx.x % per_block / a.heads, order = blockIdx.x % a.heads;
+    const int seq = at % per_block / a.heads, order = at % a.heads;
     const int kv_head = order % a.kv_heads, head = kv_head * (a.heads / a.kv_heads) + order / a.kv_heads;
 
     const SeqRows qs = seq_rows(a.q_starts, seq, a.q.rows), ks = seq_rows(a.k_starts, seq, a.k.rows);
     if (block * kBlock >= qs.count)
         return;
     const int ahead = ks.count - qs.count; // query i sees keys up to ahead + i
-    const int first = block * kBlock + wave % (4 / KG) * 32 * QT; // the wave's first query
+    const int first = block * kBlock + wave % (4 / KG) * 32; // the wave's first query
     const int last_key = ahead + min(block * kBlock + kBlock, qs.count) - 1; // seen by the block
-    const int wave_last = ahead + min(first + 32 * QT, qs.count) - 1;        // seen by the wave (nothing if it has no queries)
+    const int wave_last = ahead + min(first + 32, qs.count) - 1;             // seen by the wave (nothing if it has no queries)
     const int tiles = last_key < 0 ? 0 : last_key / kTokens + 1;
     const int wave_tiles = first >= qs.count || wave_last < 0 ? 0 : wave_last / kTokens + 1;
     const int whole = min(max(ahead + block * kBlock + 1, 0) / kTokens, tiles); // tiles that every query sees in full
     const int tile0 = (int)((int64_t)tiles * part / a.parts.parts), tile1 = (int)((int64_t)tiles * (part + 1) / a.parts.parts);
 
-    uint4 q[QT][D / 16];
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-        const int64_t row = qs.first + min(first + 32 * qt + ql, qs.count - 1);
+    uint4 q[D / 16];
+    {
+        const int64_t row = qs.first + min(first + ql, qs.count - 1);
         const uint16_t *src = (const uint16_t *)a.q.data + row * a.q.row_stride + (int64_t)head * a.q.head_stride + 8 * half;
 #pragma unroll
         for (int s = 0; s < D / 16; ++s)
-            q[qt][s] = *(const uint4 *)(src + 16 * s);
-    }
-    // (there before the loop: a wait for them inside it would be one for the tile that is being loaded)
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt)
+            q[s] = *(const uint4 *)(src + 16 * s);
+        // (there before the loop: a wait for them inside it would be one for the tiles that are being loaded)
 #pragma unroll
         for (int s = 0; s < D / 16; ++s)
-            asm volatile("" : "+v"(q[qt][s].x), "+v"(q[qt][s].y), "+v"(q[qt][s].z), "+v"(q[qt][s].w));
+            asm volatile("" : "+v"(q[s].x), "+v"(q[s].y), "+v"(q[s].z), "+v"(q[s].w));
+    }
     // Weights are 2^(score - base + kLift): base follows the running maximum only when that has left it 2^kSlack behind, which
     // spares nearly every rescaling, and the lift leaves fp16 its normal range down to 2^-20 of the largest weight.
     constexpr float kSlack = 8, kLift = 6;
     const float slack = kSlack / a.scale_log2;
-    float16v out[QT][D / 32];
-    float base[QT], shift[QT], l[QT], most[QT]; // base: in scores; shift: what is added to scores in powers of two
+    float16v out[D / 32];
+    float base = -INFINITY, shift = 0, l = 0, most = -INFINITY; // base: in scores; shift: what is added to scores in powers of two
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-        base[qt] = -INFINITY;
-        shift[qt] = 0;
-        l[qt] = 0;
+    for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                out[qt][d][i] = 0;
-    }
+        for (int i = 0; i < 16; ++i)
+            out[d][i] = 0;
 
-    // loads of a tile: the lane's place in it, in bytes
+    // Loads of a tile: the lane's place in it, in bytes
     const uint16_t *k_src = (const uint16_t *)a.k.data + (int64_t)ks.first * a.k.row_stride + (int64_t)kv_head * a.k.head_stride;
     const uint16_t *v_src = (const uint16_t *)a.v.data + (int64_t)ks.first * a.v.row_stride + (int64_t)kv_head * a.v.head_stride;
     const unsigned lds_at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)&lds[0][0] + wave * kLoads * 1024;
     const int load_row = (wave * kLoads * 64 + lane) / kPieces, load_piece = lane % kPieces;
     constexpr int kRowStep = 64 / kPieces; // rows between a wave's loads
     const uint32_t k_row = load_row * (uint32_t)a.k.row_stride * 2, k_piece = 16 * key_piece<D>(load_row, load_piece);
-    const uint32_t v_at = load_row * (uint32_t)a.v.row_stride * 2 + 16 * value_piece<D>(load_row, load_piece);
-    auto load_tile = [&](int tile) {
-        const uint16_t *k = k_src + (int64_t)tile * kTokens * a.k.row_stride, *v = v_src + (int64_t)tile * kTokens * a.v.row_stride;
-        const unsigned to = lds_at + (tile & 1) * kTile;
-        const int rows = ks.count - tile * kTokens;
-        if (rows >= kTokens) { // kRowStep rows on, the pieces of keys change places by 4 and those of values not at all
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i)
-                lds_dma16(k + i * kRowStep * a.k.row_stride, k_row + (k_piece ^ 64 * i), to + i * 1024);
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i)
-                lds_dma16(v + i * kRowStep * a.v.row_stride, v_at, to + 2 * kTile + i * 1024);
-        } else // rows behind the last one are copies of it, and never seen
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                const int r = load_row + i * kRowStep, from = min(r, rows - 1);
-                lds_dma16(k, from * (uint32_t)a.k.row_stride * 2 + 16 * key_piece<D>(r, load_piece), to + i * 1024);
-                lds_dma16(v, from * (uint32_t)a.v.row_stride * 2 + 16 * value_piece<D>(r, load_piece), to + 2 * kTile + i * 1024);
-            }
+    const uint32_t v_row = load_row * (uint32_t)a.v.row_stride * 2, v_piece = 16 * value_piece<D>(load_row, load_piece);
+    // Load i of a tile's keys (values), into the first or second place for them.  Behind the last tile: the last one again, so that a
+    // wave can count what is on its way.
+    auto load = [&](bool keys, int tile, int place, int i) {
+        tile = min(tile, tile1 - 1);
+        const int64_t stride = keys ? a.k.row_stride : a.v.row_stride;
+        const uint32_t last = (min(ks.count - tile * kTokens, kTokens) - 1) * (uint32_t)stride * 2;
+        // kRowStep rows on, the pieces of keys change places by 4 and those of values not at all; rows behind the last one are
+        // copies of it, and never seen
+        const uint32_t row = min((keys ? k_row : v_row) + i * kRowStep * (uint32_t)stride * 2, last);
+        lds_dma16((keys ? k_src : v_src) + (int64_t)tile * kTokens * stride, row + (keys ? k_piece ^ 64 * i : v_piece),
+                        lds_at + ((keys ? 0 : 2) + place) * kTile + i * 1024);
     };
+    auto load_keys = [&](int tile, int place) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+            load(true, tile, place, i);
+    };
+    auto load_values = [&](int tile, int place) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+            load(false, tile, place, i);
+    };
+    // All but the newest `newer` loads have arrived, every wave's, and nobody reads what will be overwritten
+    auto arrive = [&](auto newer) {
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(decltype(newer)::value) : "memory");
+        __syncthreads();
+    };
+    typedef std::integral_constant<int, 0> None;
+    typedef std::integral_constant<int, kLoads> OneTile;
 
+    typedef float16v Scores[TT];
     // S^T of a tile
-    float16v score[QT][TT];
-    auto scores = [&](int tile) {
-        const uint8_t *kt = lds[tile & 1] + kg * 32 * D * 2;
+    auto scores = [&](int place, Scores &score) {
+        const uint8_t *kt = lds[place] + kg * 32 * D * 2;
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    score[qt][tt][i] = 0;
+            for (int i = 0; i < 16; ++i)
+                score[tt][i] = 0;
 #pragma unroll
         for (int s = 0; s < D / 16; ++s)
 #pragma unroll
             for (int tt = 0; tt < TT; ++tt) {
                 const int r = 32 * tt + ql;
                 const uint4 k = *(const uint4 *)(kt + r * D * 2 + key_piece<D>(r, 2 * s + half) * 16);
-#pragma unroll
-                for (int qt = 0; qt < QT; ++qt)
-                    score[qt][tt] = mfma_32x32x16<DTYPE>(k, q[qt][s], score[qt][tt]);
+                score[tt] = mfma_32x32x16<DTYPE>(k, q[s], score[tt]);
             }
-        __builtin_amdgcn_sched_group_barrier(0x100, 8, 0); // eight reads, then a product and a read in turn
-#pragma unroll
-        for (int i = 0; i < D / 16 * TT - 8; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        }
-        __builtin_amdgcn_sched_group_barrier(0x8, 8, 0);
     };
-    auto hide = [&](int tile) { // what a query does not see
+    auto hide = [&](int tile, Scores &score) { // what a query does not see
+        const int sees = ahead + first + ql - tile * kTokens - 32 * kg - 4 * half;
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
-            const int sees = ahead + first + 32 * qt + ql - tile * kTokens - 32 * kg - 4 * half;
+        for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
-            for (int tt = 0; tt < TT; ++tt)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    score[qt][tt][i] = 32 * tt + 8 * (i / 4) + i % 4 <= sees ? score[qt][tt][i] : -INFINITY;
-        }
+            for (int i = 0; i < 16; ++i)
+                score[tt][i] = 32 * tt + 8 * (i / 4) + i % 4 <= sees ? score[tt][i] : -INFINITY;
     };
-    auto find_most = [&]() {
+    auto find_most = [&](const Scores &score) {
+        float x = -INFINITY;
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
-            float x = -INFINITY;
+        for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
-            for (int tt = 0; tt < TT; ++tt)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    x = fmaxf(x, score[qt][tt][i]);
-            most[qt] = max_across_halves(x);
-        }
+            for (int i = 0; i < 16; ++i)
+                x = fmaxf(x, score[tt][i]);
+        most = max_across_halves(x);
     };
     auto follow = [&]() {
+        if (__any(most > base + slack)) {
+            const float to = fmaxf(most, base);
+            const float down = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((base - to) * a.scale_log2);
+            base = to;
+            shift = to == -INFINITY ? 0.f : kLift - to * a.scale_log2;
+            l *= down;
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt)
-            if (__any(most[qt] > base[qt] + slack)) {
-                const float to = fmaxf(most[qt], base[qt]);
-                const float down = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((base[qt] - to) * a.scale_log2);
-                base[qt] = to;
-                shift[qt] = to == -INFINITY ? 0.f : kLift - to * a.scale_log2;
-                l[qt] *= down;
+            for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-                for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        out[qt][d][i] *= down;
-            }
+                for (int i = 0; i < 16; ++i)
+                    out[d][i] *= down;
+        }
     };
     // Sixteen tokens at a time: their weights, their values, and out^T += V^T P^T
-    uint32_t p[QT][2 * TT][4];
-    auto weigh = [&](int s) {
+    uint32_t p[2 * TT][4];
+    auto weigh = [&](int s, const Scores &score) {
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(score[qt][s / 2][8 * (s % 2) + 2 * i], a.scale_log2, shift[qt]));
-                const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(score[qt][s / 2][8 * (s % 2) + 2 * i + 1], a.scale_log2, shift[qt]));
-                l[qt] += x;
-                l[qt] += y;
-                p[qt][s][i] = pack16<DTYPE>(x, y);
-            }
+        for (int i = 0; i < 4; ++i) {
+            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(score[s / 2][8 * (s % 2) + 2 * i], a.scale_log2, shift));
+            const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(score[s / 2][8 * (s % 2) + 2 * i + 1], a.scale_log2, shift));
+            l += x;
+            l += y;
+            p[s][i] = pack16<DTYPE>(x, y);
+        }
     };
     const int tr = (lane & 15) / 4 + 4 * half, tc = 16 * (lane >> 4 & 1) + 4 * (lane & 3); // the lane's row and element
     uint4 v[2][D / 32];
-    auto fetch = [&](int tile, int s) {
-        const uint8_t *vt = lds[2 + (tile & 1)];
+    auto fetch = [&](int place, int s) {
+        const uint8_t *vt = lds[2 + place];
 #pragma unroll
         for (int d = 0; d < D / 32; ++d) {
             uint2 x[2];
@@ -246,27 +229,102 @@ template <int DTYPE, int D, int QT, int KG> __global__ __launch_bounds__(256, 3 
     auto gather = [&](int s) {
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-            for (int qt = 0; qt < QT; ++qt)
-                out[qt][d] = mfma_32x32x16<DTYPE>(v[s & 1][d], uint4{p[qt][s][0], p[qt][s][1], p[qt][s][2], p[qt][s][3]}, out[qt][d]);
-    };
-    auto arrive = [&]() { // what was requested is there, and nobody reads what will be overwritten
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
+            out[d] = mfma_32x32x16<DTYPE>(v[s & 1][d], uint4{p[s][0], p[s][1], p[s][2], p[s][3]}, out[d]);
     };
 
-    if (tile0 < tile1)
-        load_tile(tile0);
-    for (int tile = tile0; tile < tile1; ++tile) {
-        arrive();
-        if (tile + 1 < tile1)
-            load_tile(tile + 1);
+    // The scores of a tile are taken while the one before is weighed, and its maximum is found while that one's values are gathered.
+    // Loads stand between the products: eight at once would hold a wave up for as long as a quarter of the tile's products take.
+    // A tile's keys and values are requested one step before they are needed, keys in a step's first half and values in its second.
+    Scores even, odd_ones;
+    if (tile0 < tile1) {
+        load_keys(tile0, 0);
+        arrive(None());
+        load_keys(tile0 + 1, 1);
+        load_values(tile0, 0);
+        if (tile0 < wave_tiles) {
+            scores(0, even);
+            if (tile0 >= whole)
+                hide(tile0, even);
+            find_most(even);
+        }
+    }
+    auto step = [&](int tile, auto place, const Scores &score, Scores &next) {
+        constexpr int b = decltype(place)::value;
+        arrive(OneTile());
+        if (wave_tiles > 0) // (a wave that has queries sees every whole tile)
+            follow();
+        __builtin_amdgcn_sched_barrier(0);
+        const uint8_t *kt = lds[1 - b] + kg * 32 * D * 2;
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                next[tt][i] = 0;
+        constexpr int kParts = D / 16;
+#pragma unroll
+        for (int s = 0; s < kParts; ++s) {
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt) {
+                const int r = 32 * tt + ql;
+                const uint4 k = *(const uint4 *)(kt + r * D * 2 + key_piece<D>(r, 2 * s + half) * 16);
+                next[tt] = mfma_32x32x16<DTYPE>(k, q[s], next[tt]);
+            }
+            if (s % 2 == 1)
+                load(true, tile + 2, b, s / 2);
+        }
+#pragma unroll
+        for (int s = 0; s < 2 * TT; ++s)
+            weigh(s, score);
+        __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+        for (int i = 0; i < D / 16 * TT; ++i) { // a product, a read, two weights
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x402, 7 * 128 / D, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        arrive(OneTile());
+        float x = -INFINITY;
+        fetch(b, 0);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int s = 0; s < 2 * TT; ++s) { // the next sixteen tokens' values and a quarter (half) of the maximum beside the products
+            if (s < 2 * TT - 1)
+                fetch(b, s + 1);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                x = fmaxf(x, next[s / 2][8 * (s % 2) + i]);
+            gather(s);
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i)
+                if (i * 2 * TT / kLoads == s)
+                    load(false, tile + 1, 1 - b, i);
+            __builtin_amdgcn_sched_group_barrier(0x100, D / 16, 0);
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x2, 2, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        most = max_across_halves(x);
+    };
+    int tile = tile0;
+    for (; tile + 2 < min(whole, tile1); tile += 2) {
+        step(tile, std::integral_constant<int, 0>(), even, odd_ones);
+        step(tile + 1, std::integral_constant<int, 1>(), odd_ones, even);
+    }
+    for (; tile < tile1; ++tile) {
+        const int b = tile - tile0 & 1;
+        arrive(None());
+        load_keys(tile + 2, b);
+        load_values(tile + 1, 1 - b);
         // A weight of 0 does not keep an infinite value out of a product.  Tiles that some query sees a part of are looked
         // through for values that are not finite; where there are some, zeros take their places, and they are added after the
         // product to the queries that see them.
         bool odd = false;
         if (tile >= whole) {
-            uint4 *piece = (uint4 *)(lds[2 + (tile & 1)] + threadIdx.x * 16);
+            uint4 *piece = (uint4 *)(lds[2 + b] + threadIdx.x * 16);
             uint32_t found = 0;
 #pragma unroll
             for (int i = 0; i < kTile / 4096; ++i) {
@@ -277,7 +335,7 @@ template <int DTYPE, int D, int QT, int KG> __global__ __launch_bounds__(256, 3 
             if (lane == 0)
                 odd_values[wave] = any;
             __syncthreads();
-            odd = odd_values[0] | odd_values[1] | odd_values[2] | odd_values[3];
+            odd = (odd_values[0] | odd_values[1] | odd_values[2] | odd_values[3]) != 0;
             if (odd) {
 #pragma unroll 1
                 for (int i = 0; i < kTile / 4096; ++i) {
@@ -290,141 +348,119 @@ template <int DTYPE, int D, int QT, int KG> __global__ __launch_bounds__(256, 3 
             }
         }
         if (tile < wave_tiles) {
-            scores(tile);
-            if (tile >= whole)
-                hide(tile);
-            find_most();
             follow();
-            fetch(tile, 0);
-            weigh(0);
-            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int s = 0; s < 2 * TT; ++s) { // the next tokens' weights stand between the products
-                if (s < 2 * TT - 1) {
-                    fetch(tile, s + 1);
-                    weigh(s + 1);
-                }
+            for (int s = 0; s < 2 * TT; ++s)
+                weigh(s, even);
+#pragma unroll
+            for (int s = 0; s < 2 * TT; ++s) {
+                fetch(b, s);
                 gather(s);
-                __builtin_amdgcn_sched_group_barrier(0x100, D / 16, 0);
-#pragma unroll
-                for (int i = 0; i < D / 32 * QT; ++i) {
-                    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x402, 28 * 32 / D, 0);
-                }
-                __builtin_amdgcn_sched_barrier(0);
             }
             if (odd) {
 #pragma unroll 1
                 for (int tok = 32 * kg; tok < min(32 * kg + 32 * TT, ks.count - tile * kTokens); ++tok) {
                     const uint16_t *src = v_src + (int64_t)(tile * kTokens + tok) * a.v.row_stride + 4 * half;
                     const int i = tok % 32 / 8 * 4 + tok % 4;
+                    uint32_t pair = 0;
 #pragma unroll
-                    for (int qt = 0; qt < QT; ++qt) {
-                        uint32_t pair = 0;
+                    for (int j = 0; j < 8 * TT; ++j)
+                        pair = (tok / 32 - kg) * 8 + i / 2 == j ? p[j / 4][j % 4] : pair;
+                    pair = __shfl(pair, ql + 32 * (tok / 4 % 2));
+                    const float w = value16<DTYPE>(i & 1 ? pair >> 16 : pair);
+                    const bool seen = tile * kTokens + tok <= ahead + first + ql;
 #pragma unroll
-                        for (int j = 0; j < 8 * TT; ++j)
-                            pair = (tok / 32 - kg) * 8 + i / 2 == j ? p[qt][j / 4][j % 4] : pair;
-                        pair = __shfl(pair, ql + 32 * (tok / 4 % 2));
-                        const float w = value16<DTYPE>(i & 1 ? pair >> 16 : pair);
-                        const bool seen = tile * kTokens + tok <= ahead + first + 32 * qt + ql;
+                    for (int d = 0; d < D / 32; ++d) {
 #pragma unroll
-                        for (int d = 0; d < D / 32; ++d) {
+                        for (int j = 0; j < 4; ++j) {
+                            const uint2 four = *(const uint2 *)(src + 32 * d + 8 * j);
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const uint2 four = *(const uint2 *)(src + 32 * d + 8 * j);
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    const float x = value16<DTYPE>((e < 2 ? four.x : four.y) >> (16 * (e & 1)));
-                                    out[qt][d][4 * j + e] = __builtin_fmaf(w, seen && !(fabsf(x) < INFINITY) ? x : 0.f, out[qt][d][4 * j + e]);
-                                }
+                            for (int e = 0; e < 4; ++e) {
+                                const float x = value16<DTYPE>((e < 2 ? four.x : four.y) >> (16 * (e & 1)));
+                                out[d][4 * j + e] = __builtin_fmaf(w, seen && !(fabsf(x) < INFINITY) ? x : 0.f, out[d][4 * j + e]);
                             }
-                            asm volatile("" ::: "memory"); // (a few loads at a time: rare, and not to cost registers)
                         }
+                        asm volatile("" ::: "memory"); // (a few loads at a time: rare, and not to cost registers)
                     }
                 }
             }
         }
+        if (tile + 1 < min(tile1, wave_tiles)) {
+            scores(1 - b, even);
+            if (tile + 1 >= whole)
+                hide(tile + 1, even);
+            find_most(even);
+        }
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // (nothing may arrive in LDS that is another's, or holds sums)
 
     // the sums of the waves with the other tokens
     if constexpr (KG == 2) {
         float *sums = (float *)&lds[0][0];
-        __shared__ float other[2][64 * QT];
-        const int at = wave % 2 * 32 * QT;
+        __shared__ float other[2][64];
+        const int r = wave % 2 * 32 + ql;
         __syncthreads();
-        if (kg == 1)
-#pragma unroll
-            for (int qt = 0; qt < QT; ++qt) {
-                const int r = at + 32 * qt + ql;
-                l[qt] = sum_across_halves(l[qt]);
-                if (half == 0) {
-                    other[0][r] = base[qt];
-                    other[1][r] = l[qt];
-                }
-#pragma unroll
-                for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        *(float4 *)&sums[r * (D + 4) + 32 * d + 8 * j + 4 * half] =
-                            float4{out[qt][d][4 * j], out[qt][d][4 * j + 1], out[qt][d][4 * j + 2], out[qt][d][4 * j + 3]};
+        if (kg == 1) {
+            l = sum_across_halves(l);
+            if (half == 0) {
+                other[0][r] = base;
+                other[1][r] = l;
             }
-        __syncthreads();
-        if (kg == 1)
-            return;
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
-            const int r = at + 32 * qt + ql;
-            const float b = other[0][r], to = fmaxf(b, base[qt]);
-            const float mine = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((base[qt] - to) * a.scale_log2);
-            const float theirs = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((b - to) * a.scale_log2);
-            base[qt] = to;
-            shift[qt] = to == -INFINITY ? 0.f : kLift - to * a.scale_log2;
-            l[qt] = l[qt] * mine + (half ? 0.f : other[1][r] * theirs);
 #pragma unroll
             for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    out[qt][d][j] = out[qt][d][j] * mine + sums[r * (D + 4) + 32 * d + 8 * (j / 4) + 4 * half + j % 4] * theirs;
+                for (int j = 0; j < 4; ++j)
+                    *(float4 *)&sums[r * (D + 4) + 32 * d + 8 * j + 4 * half] = float4{out[d][4 * j], out[d][4 * j + 1], out[d][4 * j + 2], out[d][4 * j + 3]};
         }
-    }
-
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-        const float total = sum_across_halves(l[qt]);
-        const int i = first + 32 * qt + ql;
-        if (a.parts.parts > 1) {
-            if (i < qs.count) {
-                const int64_t at = ((int64_t)(qs.first + i) * a.heads + head) * a.parts.parts + part;
-#pragma unroll
-                for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        *(float4 *)(a.parts.sums + at * D + 32 * d + 8 * j + 4 * half) =
-                            float4{out[qt][d][4 * j], out[qt][d][4 * j + 1], out[qt][d][4 * j + 2], out[qt][d][4 * j + 3]};
-                if (half == 0)
-                    a.parts.stats[at] = float2{base[qt] == -INFINITY ? -INFINITY : -shift[qt], total};
-            }
-            continue;
-        }
-        const float f = total > 0 ? 1.f / total : total; // (a sum that is not a number stays one)
-        uint16_t *to = (uint16_t *)a.out.data + (int64_t)(qs.first + i) * a.out.row_stride + (int64_t)head * a.out.head_stride;
+        __syncthreads();
+        if (kg == 1)
+            return;
+        const float b = other[0][r], to = fmaxf(b, base);
+        const float mine = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((base - to) * a.scale_log2);
+        const float theirs = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((b - to) * a.scale_log2);
+        base = to;
+        shift = to == -INFINITY ? 0.f : kLift - to * a.scale_log2;
+        l = l * mine + (half ? 0.f : other[1][r] * theirs);
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                // elements 8 x + 4 h .. + 3 of the lanes h = 0, 1: eight neighbours per lane after an exchange
-                uint32_t x[2][2];
-#pragma unroll
-                for (int y = 0; y < 2; ++y)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        x[y][e] = pack16<DTYPE>(out[qt][d][8 * j + 4 * y + 2 * e] * f, out[qt][d][8 * j + 4 * y + 2 * e + 1] * f);
-                const auto r0 = __builtin_amdgcn_permlane32_swap(x[0][0], x[1][0], false, false);
-                const auto r1 = __builtin_amdgcn_permlane32_swap(x[0][1], x[1][1], false, false);
-                if (i < qs.count)
-                    *(uint4 *)(to + 32 * d + 16 * j + 8 * half) = uint4{r0[0], r1[0], r0[1], r1[1]};
-            }
+            for (int j = 0; j < 16; ++j)
+                out[d][j] = out[d][j] * mine + sums[r * (D + 4) + 32 * d + 8 * (j / 4) + 4 * half + j % 4] * theirs;
     }
+
+    const float total = sum_across_halves(l);
+    const int i = first + ql;
+    if (a.parts.parts > 1) {
+        if (i < qs.count) {
+            const int64_t at = ((int64_t)(qs.first + i) * a.heads + head) * a.parts.parts + part;
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    *(float4 *)(a.parts.sums + at * D + 32 * d + 8 * j + 4 * half) = float4{out[d][4 * j], out[d][4 * j + 1], out[d][4 * j + 2], out[d][4 * j + 3]};
+            if (half == 0)
+                a.parts.stats[at] = float2{base == -INFINITY ? -INFINITY : -shift, total};
+        }
+        return;
+    }
+    const float f = total > 0 ? 1.f / total : total; // (a sum that is not a number stays one)
+    uint16_t *to = (uint16_t *)a.out.data + (int64_t)(qs.first + i) * a.out.row_stride + (int64_t)head * a.out.head_stride;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            // elements 8 x + 4 h .. + 3 of the lanes h = 0, 1: eight neighbours per lane after an exchange
+            uint32_t x[2][2];
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    x[y][e] = pack16<DTYPE>(out[d][8 * j + 4 * y + 2 * e] * f, out[d][8 * j + 4 * y + 2 * e + 1] * f);
+            const auto r0 = __builtin_amdgcn_permlane32_swap(x[0][0], x[1][0], false, false);
+            const auto r1 = __builtin_amdgcn_permlane32_swap(x[0][1], x[1][1], false, false);
+            if (i < qs.count)
+                *(uint4 *)(to + 32 * d + 16 * j + 8 * half) = uint4{r0[0], r1[0], r0[1], r1[1]};
+        }
 }
 
 } // namespace
@@ -432,17 +468,20 @@ template <int DTYPE, int D, int QT, int KG> __global__ __launch_bounds__(256, 3 
 void plan_attn_prompt(abq_attn_state *st, int most_parts)
 {
     const int64_t each = (int64_t)st->heads * st->seqs;
-    // A compute unit holds two workgroups, so 512 run beside each other.  With fewer blocks of 128 queries, blocks of 64 ...
+    // A compute unit holds two workgroups, so 512 run beside each other.  With fewer blocks of 128 queries, blocks of 64 whose
+    // waves share the tokens (1024 tokens, heads of 128, fp16: 32 heads 23.6 -> 19.9 us, 8 heads 21.3 -> 15.5; 64 heads, which
+    // fill the chip, 29.5 -> 34) ...
     st->block_rows = ((int64_t)st->max_q + 127) / 128 * each >= 512 ? 128 : 64;
-    // ... and where those leave room as well, parts of the keys, of eight tiles at least
+    // ... and where those leave room as well, parts of the keys, of sixteen tiles at least (64 queries behind 8128 keys, 8 heads in
+    // 1, 4, 16 parts: 77, 29, 16 us; 1024 tokens, 16 heads in 1, 2: 16.9, 23.1)
     const int64_t groups = ((int64_t)st->max_q + st->block_rows - 1) / st->block_rows * each;
     int64_t parts = 512 / groups;
-    parts = parts < st->max_k / (8 * kTokens) ? parts : st->max_k / (8 * kTokens);
+    parts = parts < st->max_k / (16 * kTokens) ? parts : st->max_k / (16 * kTokens);
     parts = parts < most_parts ? parts : most_parts;
     st->parts = parts < 2 ? 1 : (int)parts;
 }
 
-#define ABQ_PROMPT(T, D_, KG) hipLaunchKernelGGL((attn_prompt_kernel<T, D_, 1, KG>), grid, dim3(256), 0, stream, a)
+#define ABQ_PROMPT(T, D_, KG) hipLaunchKernelGGL((attn_prompt_kernel<T, D_, KG>), grid, dim3(256), 0, stream, a)
 #define ABQ_PROMPT_DIM(T)                    \
     do {                                     \
         if (st.head_dim == 64) {             \
