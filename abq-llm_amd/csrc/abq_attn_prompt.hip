@@ -81,9 +81,7 @@ template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void at
     const int ahead = ks.count - qs.count; // query i sees keys up to ahead + i
     const int first = block * kBlock + wave % (4 / KG) * 32; // the wave's first query
     const int last_key = ahead + min(block * kBlock + kBlock, qs.count) - 1; // seen by the block
-    const int wave_last = ahead + min(first + 32, qs.count) - 1;             // seen by the wave (nothing if it has no queries)
     const int tiles = last_key < 0 ? 0 : last_key / kTokens + 1;
-    const int wave_tiles = first >= qs.count || wave_last < 0 ? 0 : wave_last / kTokens + 1;
     const int whole = min(max(ahead + block * kBlock + 1, 0) / kTokens, tiles); // tiles that every query sees in full
     const int tile0 = (int)((int64_t)tiles * part / a.parts.parts), tile1 = (int)((int64_t)tiles * (part + 1) / a.parts.parts);
 
@@ -198,18 +196,16 @@ template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void at
                     out[d][i] *= down;
         }
     };
-    // Sixteen tokens at a time: their weights, their values, and out^T += V^T P^T
+    // Weights, two at a time
     uint32_t p[2 * TT][4];
-    auto weigh = [&](int s, const Scores &score) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(score[s / 2][8 * (s % 2) + 2 * i], a.scale_log2, shift));
-            const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(score[s / 2][8 * (s % 2) + 2 * i + 1], a.scale_log2, shift));
-            l += x;
-            l += y;
-            p[s][i] = pack16<DTYPE>(x, y);
-        }
+    auto weigh = [&](int pair, const Scores &score) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(score[pair / 8][2 * (pair % 8)], a.scale_log2, shift));
+        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(score[pair / 8][2 * (pair % 8) + 1], a.scale_log2, shift));
+        l += x;
+        l += y;
+        p[pair / 4][pair % 4] = pack16<DTYPE>(x, y);
     };
+    // Sixteen tokens at a time: their values, and out^T += V^T P^T
     const int tr = (lane & 15) / 4 + 4 * half, tc = 16 * (lane >> 4 & 1) + 4 * (lane & 3); // the lane's row and element
     uint4 v[2][D / 32];
     auto fetch = [&](int place, int s) {
@@ -235,54 +231,53 @@ template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void at
     // The scores of a tile are taken while the one before is weighed, and its maximum is found while that one's values are gathered.
     // Loads stand between the products: eight at once would hold a wave up for as long as a quarter of the tile's products take.
     // A tile's keys and values are requested one step before they are needed, keys in a step's first half and values in its second.
-    Scores even, odd_ones;
-    if (tile0 < tile1) {
-        load_keys(tile0, 0);
-        arrive(None());
-        load_keys(tile0 + 1, 1);
-        load_values(tile0, 0);
-        if (tile0 < wave_tiles) {
-            scores(0, even);
-            if (tile0 >= whole)
-                hide(tile0, even);
-            find_most(even);
-        }
-    }
     auto step = [&](int tile, auto place, const Scores &score, Scores &next) {
         constexpr int b = decltype(place)::value;
         arrive(OneTile());
-        if (wave_tiles > 0) // (a wave that has queries sees every whole tile)
-            follow();
+        // Sixteen elements at a time: their products, the next ones' keys, and a share of the weights beside each other
+        constexpr int kShares = D / 16, kPairs = 8 * TT / kShares;
+        uint4 k[2][TT];
+        auto read_keys = [&](int c) {
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt) {
+                const int r = 32 * tt + ql;
+                k[c & 1][tt] = *(const uint4 *)(lds[1 - b] + (32 * kg + r) * D * 2 + key_piece<D>(r, 2 * c + half) * 16);
+            }
+        };
+        read_keys(0);
+        follow();
         __builtin_amdgcn_sched_barrier(0);
-        const uint8_t *kt = lds[1 - b] + kg * 32 * D * 2;
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 next[tt][i] = 0;
-        constexpr int kParts = D / 16;
 #pragma unroll
-        for (int s = 0; s < kParts; ++s) {
+        for (int c = 0; c < kShares; ++c) {
+            if (c < kShares - 1)
+                read_keys(c + 1);
 #pragma unroll
-            for (int tt = 0; tt < TT; ++tt) {
-                const int r = 32 * tt + ql;
-                const uint4 k = *(const uint4 *)(kt + r * D * 2 + key_piece<D>(r, 2 * s + half) * 16);
-                next[tt] = mfma_32x32x16<DTYPE>(k, q[s], next[tt]);
+            for (int tt = 0; tt < TT; ++tt)
+                next[tt] = mfma_32x32x16<DTYPE>(k[c & 1][tt], q[c], next[tt]);
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i)
+                weigh(kPairs * c + i, score);
+            if (c % 2 == 1)
+                load(true, tile + 2, b, c / 2);
+            __builtin_amdgcn_sched_group_barrier(0x100, TT, 0);
+#pragma unroll
+            for (int i = 0; i < TT; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x402, 7 * 128 / D, 0);
             }
-            if (s % 2 == 1)
-                load(true, tile + 2, b, s / 2);
+            __builtin_amdgcn_sched_barrier(0);
         }
+        // (all weights are taken here, not behind the branch)
 #pragma unroll
         for (int s = 0; s < 2 * TT; ++s)
-            weigh(s, score);
-        __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
-#pragma unroll
-        for (int i = 0; i < D / 16 * TT; ++i) { // a product, a read, two weights
-            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x402, 7 * 128 / D, 0);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+            asm volatile("" : "+v"(p[s][0]), "+v"(p[s][1]), "+v"(p[s][2]), "+v"(p[s][3]));
+        if (tile + 1 >= whole)
+            hide(tile + 1, next);
         arrive(OneTile());
         float x = -INFINITY;
         fetch(b, 0);
@@ -309,58 +304,103 @@ template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void at
         }
         most = max_across_halves(x);
     };
-    int tile = tile0;
-    for (; tile + 2 < min(whole, tile1); tile += 2) {
-        step(tile, std::integral_constant<int, 0>(), even, odd_ones);
-        step(tile + 1, std::integral_constant<int, 1>(), odd_ones, even);
-    }
-    for (; tile < tile1; ++tile) {
-        const int b = tile - tile0 & 1;
+    if (tile0 < tile1) {
+        Scores even, uneven;
+        load_keys(tile0, 0);
         arrive(None());
-        load_keys(tile + 2, b);
-        load_values(tile + 1, 1 - b);
-        // A weight of 0 does not keep an infinite value out of a product.  Tiles that some query sees a part of are looked
-        // through for values that are not finite; where there are some, zeros take their places, and they are added after the
-        // product to the queries that see them.
-        bool odd = false;
-        if (tile >= whole) {
-            uint4 *piece = (uint4 *)(lds[2 + b] + threadIdx.x * 16);
-            uint32_t found = 0;
-#pragma unroll
-            for (int i = 0; i < kTile / 4096; ++i) {
-                const uint4 w = piece[i * 256];
-                found |= not_finite<DTYPE>(w.x) | not_finite<DTYPE>(w.y) | not_finite<DTYPE>(w.z) | not_finite<DTYPE>(w.w);
-            }
-            const bool any = __any(found != 0);
-            if (lane == 0)
-                odd_values[wave] = any;
-            __syncthreads();
-            odd = (odd_values[0] | odd_values[1] | odd_values[2] | odd_values[3]) != 0;
-            if (odd) {
-#pragma unroll 1
-                for (int i = 0; i < kTile / 4096; ++i) {
-                    uint4 w = piece[i * 256];
-                    w.x &= ~(not_finite<DTYPE>(w.x) / 0x8000 * 0xffff), w.y &= ~(not_finite<DTYPE>(w.y) / 0x8000 * 0xffff);
-                    w.z &= ~(not_finite<DTYPE>(w.z) / 0x8000 * 0xffff), w.w &= ~(not_finite<DTYPE>(w.w) / 0x8000 * 0xffff);
-                    piece[i * 256] = w;
-                }
-                __syncthreads();
-            }
+        load_keys(tile0 + 1, 1);
+        load_values(tile0, 0);
+        scores(0, even);
+        if (tile0 >= whole)
+            hide(tile0, even);
+        find_most(even);
+        int tile = tile0;
+        for (; tile + 2 < tile1; tile += 2) {
+            step(tile, std::integral_constant<int, 0>(), even, uneven);
+            step(tile + 1, std::integral_constant<int, 1>(), uneven, even);
         }
-        if (tile < wave_tiles) {
-            follow();
+        if (tile + 1 < tile1) {
+            step(tile, std::integral_constant<int, 0>(), even, uneven);
 #pragma unroll
-            for (int s = 0; s < 2 * TT; ++s)
-                weigh(s, even);
+            for (int tt = 0; tt < TT; ++tt)
+                even[tt] = uneven[tt];
+            ++tile;
+        }
+        arrive(None()); // the last one
+        follow();
 #pragma unroll
-            for (int s = 0; s < 2 * TT; ++s) {
-                fetch(b, s);
-                gather(s);
-            }
-            if (odd) {
+        for (int i = 0; i < 8 * TT; ++i)
+            weigh(i, even);
+#pragma unroll
+        for (int s = 0; s < 2 * TT; ++s) {
+            fetch(tile - tile0 & 1, s);
+            gather(s);
+        }
+    }
+
+    // (what the lane is, taken anew: the loop needs every register)
+    int none = 0;
+    asm volatile("" : "+v"(none));
+    const int upper = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, none)) >> 5;
+
+    // A weight of 0 does not keep a value that is not finite out of a product, so one that no query may see can have come into the
+    // sums.  A block whose sums are not all finite is done again, step by step: where a tile that some query does not see all of
+    // holds such values, zeros take their places, and they are added after the product to the queries that see them.
+    if (whole < tiles) {
+        float any = 0;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                any = __builtin_fmaf(out[d][i], 0.f, any);
+        const bool found = __any(!(any == 0));
+        if (lane == 0)
+            odd_values[wave] = found;
+        __syncthreads();
+        if (odd_values[0] | odd_values[1] | odd_values[2] | odd_values[3]) {
+            base = -INFINITY;
+            shift = l = 0;
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    out[d][i] = 0;
+            Scores score;
+#pragma unroll 1
+            for (int tile = tile0; tile < tile1; ++tile) {
+                __syncthreads(); // (nobody reads the tile before)
+                load_keys(tile, 0);
+                load_values(tile, 0);
+                arrive(None());
+                if (tile >= whole) {
+                    uint4 *piece = (uint4 *)(lds[2] + (wave * 64 + lane) * 16);
+#pragma unroll 1
+                    for (int i = 0; i < kTile / 4096; ++i) {
+                        uint4 w = piece[i * 256];
+                        w.x &= ~(not_finite<DTYPE>(w.x) / 0x8000 * 0xffff), w.y &= ~(not_finite<DTYPE>(w.y) / 0x8000 * 0xffff);
+                        w.z &= ~(not_finite<DTYPE>(w.z) / 0x8000 * 0xffff), w.w &= ~(not_finite<DTYPE>(w.w) / 0x8000 * 0xffff);
+                        piece[i * 256] = w;
+                    }
+                    __syncthreads();
+                }
+                scores(0, score);
+                if (tile >= whole)
+                    hide(tile, score);
+                find_most(score);
+                follow();
+#pragma unroll
+                for (int i = 0; i < 8 * TT; ++i)
+                    weigh(i, score);
+#pragma unroll
+                for (int s = 0; s < 2 * TT; ++s) {
+                    fetch(0, s);
+                    gather(s);
+                }
+                if (tile < whole)
+                    continue;
 #pragma unroll 1
                 for (int tok = 32 * kg; tok < min(32 * kg + 32 * TT, ks.count - tile * kTokens); ++tok) {
-                    const uint16_t *src = v_src + (int64_t)(tile * kTokens + tok) * a.v.row_stride + 4 * half;
+                    const uint16_t *src = v_src + (int64_t)(tile * kTokens + tok) * a.v.row_stride + 4 * upper;
                     const int i = tok % 32 / 8 * 4 + tok % 4;
                     uint32_t pair = 0;
 #pragma unroll
@@ -368,7 +408,7 @@ template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void at
                         pair = (tok / 32 - kg) * 8 + i / 2 == j ? p[j / 4][j % 4] : pair;
                     pair = __shfl(pair, ql + 32 * (tok / 4 % 2));
                     const float w = value16<DTYPE>(i & 1 ? pair >> 16 : pair);
-                    const bool seen = tile * kTokens + tok <= ahead + first + ql;
+                    const bool seen = tile * kTokens + tok - ahead - first <= ql;
 #pragma unroll
                     for (int d = 0; d < D / 32; ++d) {
 #pragma unroll
@@ -380,16 +420,10 @@ template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void at
                                 out[d][4 * j + e] = __builtin_fmaf(w, seen && !(fabsf(x) < INFINITY) ? x : 0.f, out[d][4 * j + e]);
                             }
                         }
-                        asm volatile("" ::: "memory"); // (a few loads at a time: rare, and not to cost registers)
+                        asm volatile("" ::: "memory"); // (a few loads at a time)
                     }
                 }
             }
-        }
-        if (tile + 1 < min(tile1, wave_tiles)) {
-            scores(1 - b, even);
-            if (tile + 1 >= whole)
-                hide(tile + 1, even);
-            find_most(even);
         }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // (nothing may arrive in LDS that is another's, or holds sums)
@@ -402,7 +436,7 @@ template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void at
         __syncthreads();
         if (kg == 1) {
             l = sum_across_halves(l);
-            if (half == 0) {
+            if (upper == 0) {
                 other[0][r] = base;
                 other[1][r] = l;
             }
@@ -410,7 +444,7 @@ template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void at
             for (int d = 0; d < D / 32; ++d)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    *(float4 *)&sums[r * (D + 4) + 32 * d + 8 * j + 4 * half] = float4{out[d][4 * j], out[d][4 * j + 1], out[d][4 * j + 2], out[d][4 * j + 3]};
+                    *(float4 *)&sums[r * (D + 4) + 32 * d + 8 * j + 4 * upper] = float4{out[d][4 * j], out[d][4 * j + 1], out[d][4 * j + 2], out[d][4 * j + 3]};
         }
         __syncthreads();
         if (kg == 1)
@@ -420,12 +454,12 @@ template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void at
         const float theirs = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((b - to) * a.scale_log2);
         base = to;
         shift = to == -INFINITY ? 0.f : kLift - to * a.scale_log2;
-        l = l * mine + (half ? 0.f : other[1][r] * theirs);
+        l = l * mine + (upper ? 0.f : other[1][r] * theirs);
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
 #pragma unroll
             for (int j = 0; j < 16; ++j)
-                out[d][j] = out[d][j] * mine + sums[r * (D + 4) + 32 * d + 8 * (j / 4) + 4 * half + j % 4] * theirs;
+                out[d][j] = out[d][j] * mine + sums[r * (D + 4) + 32 * d + 8 * (j / 4) + 4 * upper + j % 4] * theirs;
     }
 
     const float total = sum_across_halves(l);
@@ -437,8 +471,8 @@ template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void at
             for (int d = 0; d < D / 32; ++d)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    *(float4 *)(a.parts.sums + at * D + 32 * d + 8 * j + 4 * half) = float4{out[d][4 * j], out[d][4 * j + 1], out[d][4 * j + 2], out[d][4 * j + 3]};
-            if (half == 0)
+                    *(float4 *)(a.parts.sums + at * D + 32 * d + 8 * j + 4 * upper) = float4{out[d][4 * j], out[d][4 * j + 1], out[d][4 * j + 2], out[d][4 * j + 3]};
+            if (upper == 0)
                 a.parts.stats[at] = float2{base == -INFINITY ? -INFINITY : -shift, total};
         }
         return;
@@ -459,7 +493,7 @@ template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void at
             const auto r0 = __builtin_amdgcn_permlane32_swap(x[0][0], x[1][0], false, false);
             const auto r1 = __builtin_amdgcn_permlane32_swap(x[0][1], x[1][1], false, false);
             if (i < qs.count)
-                *(uint4 *)(to + 32 * d + 16 * j + 8 * half) = uint4{r0[0], r1[0], r0[1], r1[1]};
+                *(uint4 *)(to + 32 * d + 16 * j + 8 * upper) = uint4{r0[0], r1[0], r0[1], r1[1]};
         }
 }
 
