@@ -235,16 +235,18 @@ template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void at
         constexpr int b = decltype(place)::value;
         arrive(OneTile());
         // Sixteen elements at a time: their products, the next ones' keys, and a share of the weights beside each other
-        constexpr int kShares = D / 16, kPairs = 8 * TT / kShares;
-        uint4 k[2][TT];
+        constexpr int kShares = D / 16, kPairs = 8 * TT / kShares, kAhead = 4 / TT - 1; // (keys on their way)
+        uint4 k[kAhead + 1][TT];
         auto read_keys = [&](int c) {
 #pragma unroll
             for (int tt = 0; tt < TT; ++tt) {
                 const int r = 32 * tt + ql;
-                k[c & 1][tt] = *(const uint4 *)(lds[1 - b] + (32 * kg + r) * D * 2 + key_piece<D>(r, 2 * c + half) * 16);
+                k[c % (kAhead + 1)][tt] = *(const uint4 *)(lds[1 - b] + (32 * kg + r) * D * 2 + key_piece<D>(r, 2 * c + half) * 16);
             }
         };
-        read_keys(0);
+#pragma unroll
+        for (int c = 0; c < kAhead; ++c)
+            read_keys(c);
         follow();
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -254,11 +256,11 @@ template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void at
                 next[tt][i] = 0;
 #pragma unroll
         for (int c = 0; c < kShares; ++c) {
-            if (c < kShares - 1)
-                read_keys(c + 1);
+            if (c + kAhead < kShares)
+                read_keys(c + kAhead);
 #pragma unroll
             for (int tt = 0; tt < TT; ++tt)
-                next[tt] = mfma_32x32x16<DTYPE>(k[c & 1][tt], q[c], next[tt]);
+                next[tt] = mfma_32x32x16<DTYPE>(k[c % (kAhead + 1)][tt], q[c], next[tt]);
 #pragma unroll
             for (int i = 0; i < kPairs; ++i)
                 weigh(kPairs * c + i, score);
