@@ -508,13 +508,29 @@ void plan_attn_prompt(abq_attn_state *st, int most_parts)
     // waves share the tokens (1024 tokens, heads of 128, fp16: 32 heads 23.6 -> 19.9 us, 8 heads 21.3 -> 15.5; 64 heads, which
     // fill the chip, 29.5 -> 34) ...
     st->block_rows = ((int64_t)st->max_q + 127) / 128 * each >= 512 ? 128 : 64;
-    // ... and where those leave room as well, parts of the keys, of sixteen tiles at least (64 queries behind 8128 keys, 8 heads in
-    // 1, 4, 16 parts: 77, 29, 16 us; 1024 tokens, 16 heads in 1, 2: 16.9, 23.1)
+    // ... and where those leave room as well, parts of the keys: one workgroup per compute unit, or two with heads of 64.  A part
+    // saves its share of the steps, 0.6 us (0.5) each; the parts' results cost a launch, 3 us, and their way through memory.
+    //   us in parts                               1     2     4     8    16    32
+    //   64 queries behind 8128, 4 heads of 128   78    46    28    19    15    14   (taken: 32)
+    //   the same, 16 heads                       79    47    29    20    20    24   (16)
+    //   512 behind 3584, 16 heads of 128         44    34    34    44    71         (2)
+    //   1024 alone, 8 heads of 128               15    17    18                     (1)
+    //   333 behind 7000, 8 heads of 64           62    38    24    20    22    25   (10)
     const int64_t groups = ((int64_t)st->max_q + st->block_rows - 1) / st->block_rows * each;
-    int64_t parts = 512 / groups;
-    parts = parts < st->max_k / (16 * kTokens) ? parts : st->max_k / (16 * kTokens);
-    parts = parts < most_parts ? parts : most_parts;
-    st->parts = parts < 2 ? 1 : (int)parts;
+    const double steps = (st->max_k + kTokens - 1) / kTokens, step_us = st->head_dim == 64 ? 0.5 : 0.6;
+    const double result_us = (double)st->q.rows * st->heads * st->head_dim * 8 / 4e6;
+    int64_t most = (st->head_dim == 64 ? 512 : 256) / groups, parts = 1;
+    most = most < steps / 4 ? most : (int64_t)(steps / 4);
+    most = most < most_parts ? most : most_parts;
+    double least = steps * step_us;
+    for (int64_t p = 2; p <= most; ++p) {
+        const double us = steps / p * step_us + 3 + p * result_us;
+        if (us < least) {
+            least = us;
+            parts = p;
+        }
+    }
+    st->parts = (int)parts;
 }
 
 #define ABQ_PROMPT(T, D_, KG) hipLaunchKernelGGL((attn_prompt_kernel<T, D_, KG>), grid, dim3(256), 0, stream, a)
