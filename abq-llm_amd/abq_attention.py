@@ -187,7 +187,7 @@ class PromptAttention(_Attention):
         self.held = (q, k, v, q_starts, k_starts)
         self.state = AttnState()
         _check(lib().abq_attn_prompt_init(*[ctypes.byref(r) for r in rows], _dtype(q), q.shape[1], k.shape[1], q.shape[2], at[0], at[1],
-                                          seqs, max_q, max_k, scale or q.shape[2] ** -0.5, ctypes.byref(self.state)), "abq_attn_prompt_init")
+                                          seqs, max_q, max_k, q.shape[2] ** -0.5 if scale is None else scale, ctypes.byref(self.state)), "abq_attn_prompt_init")
         self._finish(out, workspace)
 
 
@@ -213,5 +213,5 @@ class TreeAttention(_Attention):
         _check(lib().abq_attn_tree_init(ctypes.byref(d), ctypes.byref(rows[0]), ctypes.byref(rows[1]), _dtype(q), q.shape[1], table, page_table.shape[-1],
                                         _index(context, torch.int32, seqs, "context"), _index(q_starts, torch.int32, seqs + 1, "q_starts"),
                                         None if mask is None else _index(mask, torch.int64, q.shape[0], "mask"), seqs, max_q, max_context,
-                                        scale or q.shape[2] ** -0.5, ctypes.byref(self.state)), "abq_attn_tree_init")
+                                        q.shape[2] ** -0.5 if scale is None else scale, ctypes.byref(self.state)), "abq_attn_tree_init")
         self._finish(out, workspace)

@@ -14,8 +14,15 @@ namespace {
 
 constexpr int kPromptKind = 1, kTreeKind = 2;
 
-// HIP counts the threads of a launch in 32 bits
-constexpr int64_t kMostBlocks = 0xffffffffll / 256;
+// A tile of keys or values is addressed from its first row in 32 bits: 63 strides of 2-byte elements and a row
+constexpr int64_t kMostTileStride = 1 << 25;
+
+// a * b * c, none of them negative, or more than any limit here where that does not fit
+int64_t product(int64_t a, int64_t b, int64_t c)
+{
+    int64_t x;
+    return __builtin_mul_overflow(a, b, &x) || __builtin_mul_overflow(x, c, &x) ? INT64_MAX : x;
+}
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -75,7 +82,7 @@ abq_status init_common(int kind, const abq_rows *q, const abq_rows *out, int dty
     abq_status s;
     if ((s = check_rows(q, q->rows, heads, head_dim)) != ABQ_OK || (s = check_rows(out, q->rows, heads, head_dim)) != ABQ_OK)
         return s;
-    if (q->rows > 0x7ffffff0)
+    if (q->rows > 0x7ffffff0 || product(q->rows, heads, 1) > 1ll << 42) // (so that bytes of a workspace fit 64 bits)
         return ABQ_ERR_TOO_LARGE;
     st->kind = kind;
     st->dtype = dtype;
@@ -151,9 +158,10 @@ abq_status abq_attn_prompt_init(const abq_rows *q, const abq_rows *k, const abq_
     state->v = *v;
     state->k_starts = k_starts ? k_starts : q_starts;
     state->max_k = max_k;
-    plan(state, 1);
-    if (k->rows > 0x7ffffff0 || ((int64_t)max_q + 31) / 32 * heads * seqs > kMostBlocks)
+    if (k->rows > 0x7ffffff0 || k->row_stride > kMostTileStride || v->row_stride > kMostTileStride ||
+        product(((int64_t)max_q + 31) / 32, heads, seqs) > kMostBlocks)
         return ABQ_ERR_TOO_LARGE;
+    plan(state, 1);
     state->init_success = 1;
     return ABQ_OK;
 }
@@ -181,9 +189,9 @@ abq_status abq_attn_tree_init(const abq_kv_cache *cache, const abq_rows *q, cons
     state->context = context;
     state->mask = mask;
     state->max_k = max_context + max_q;
-    plan(state, 1);
-    if (((int64_t)seqs * cache->kv_heads + 8) * ((int64_t)max_q * (heads / cache->kv_heads) + 15) / 16 > kMostBlocks)
+    if (product((int64_t)seqs * cache->kv_heads + 8, ((int64_t)max_q * (heads / cache->kv_heads) + 15) / 16, 1) > kMostBlocks)
         return ABQ_ERR_TOO_LARGE;
+    plan(state, 1);
     state->init_success = 1;
     return ABQ_OK;
 }

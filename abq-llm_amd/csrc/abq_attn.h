@@ -19,6 +19,9 @@ hipError_t launch_attn_tree(const abq_attn_state &st, hipStream_t stream);
 void plan_attn_prompt(abq_attn_state *st, int most_parts);
 void plan_attn_tree(abq_attn_state *st, int most_parts);
 
+// HIP counts the threads of a launch in 32 bits
+constexpr int64_t kMostBlocks = 0xffffffffll / 256;
+
 // Bytes of the parts' results: per query row and head, `parts` sums of head_dim floats and as many pairs (maximum, sum)
 inline size_t attn_parts_bytes(const abq_attn_state &st, int parts)
 {

@@ -17,8 +17,14 @@
 // values beside each other for the same reason.  A wave goes from global memory to registers in 16-byte loads and needs no
 // LDS until its tokens are done.
 //
-// Bound by the cache's bytes.  A sequence's tokens are split over workgroups (parts) until the chip is covered, and inside
-// one over its four waves, step by step; the waves' results are joined in LDS, the parts' by a second launch.
+// A sequence's tokens are split over workgroups (parts) until the chip is covered, and inside one over its four waves, step by
+// step; the waves' results are joined in LDS, the parts' by a second launch.
+//
+// Up to 16 rows, bound by the cache's bytes: one query for each of 32 heads on 16 x 1024 tokens of 8 bits, 29 us for 138 MB,
+// 4.8 TB/s of the 5.1 that a copy reaches; four waves per SIMD cover each other's loads, so none keeps a second buffer.  With more
+// rows a step's vector work (400 operations beside 32 MFMA: codes to fp16, factors, exponentials) and the loads share the time:
+// two waves per SIMD, each with a step under way while it works at another.  20 rows on 48 ragged contexts, 630 MB: 148 us,
+// 4.3 TB/s; 108 rows on 3 x 5500 tokens of 4 bits, 25 us, bound by that work and, at 12 steps a wave, by its start and end.
 #include "abq_attn.h"
 
 namespace abq {
@@ -564,19 +570,28 @@ hipError_t launch_attn_join(const abq_attn_state &st, hipStream_t stream)
 void plan_attn_tree(abq_attn_state *st, int most_parts)
 {
     const int rows = st->max_q * (st->heads / st->kv_heads);
+    // Blocks of 32 rows read a code once for two products, where there are two: 27 drafts of 4 heads per key head on 3 x 5500 tokens of
+    // 4 bits 30.5 us, in blocks of 16 rows 32; 48 ragged contexts, 20 rows, 147.5 and 173.  (64 drafts on 4000 tokens, or 16 of 4 heads
+    // on 4 x 2000, take the same in either: 20.8, 15.)  Up to 16 rows the second half would be empty.
     st->block_rows = rows <= 16 ? 16 : 32;
     const int64_t units = (int64_t)st->seqs * st->kv_heads * ((rows + st->block_rows - 1) / st->block_rows);
     const int64_t steps = ((int64_t)st->max_k + kStep - 1) / kStep;
     // Two workgroups per compute unit, no wave without a step; below 24 steps the second launch costs more than parts save (20
-    // sequences of 700 tokens and 8 heads: 9.8 us, in three parts 10.9).  One sequence of 8000 and 32 heads: in 1, 4, 16, 32 parts
-    // 66, 25, 17, 18 us; 16 sequences of 1024 and 32 heads in 1, 2, 4: 24.8, 27.6, 29.9.
+    // sequences of 700 tokens and 8 heads: 11.6 us, in three parts 11.7, and a workspace).  With the cache's bytes from memory, one
+    // sequence of 8000 tokens and 32 heads takes in 1, 4, 16, 32 parts 64, 25, 18, 18.5 us, and 16 of 1024 in 1, 2, 4: 29.1, 32.5,
+    // 34.4.
     int64_t parts = steps > 24 ? 512 / units : 1;
     parts = parts < steps / kWaves ? parts : steps / kWaves;
     // A wave has 32 steps at most, so that sequences much longer than the others are spread: 48 of up to 16384 tokens and 8 heads in
-    // 1, 3, 5, 8 parts 229, 163, 153, 147 us, while 30 of 4000 and 32 heads take 177 - 186 in any number.
+    // 1, 3, 5, 8 parts 230, 164, 153, 148 us, while 30 of 4000 and 32 heads take 177 - 186 in any number.
     const int64_t spread = (steps + 32 * kWaves - 1) / (32 * kWaves);
     parts = parts > spread ? parts : spread;
     parts = parts < most_parts ? parts : most_parts;
+    // (launches within their limit: this one, rounded up, and the one that joins the parts, four rows of heads per workgroup)
+    const int64_t row_blocks = (rows + st->block_rows - 1) / st->block_rows, most = kMostBlocks / (units + 8 * row_blocks);
+    parts = parts < most ? parts : most;
+    if ((int64_t)st->seqs * st->max_q > 4 * kMostBlocks / st->heads)
+        parts = 1;
     st->parts = parts < 1 ? 1 : (int)parts;
 }
 

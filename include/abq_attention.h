@@ -107,7 +107,8 @@ typedef struct abq_attn_state {
 } abq_attn_state;
 
 /* Causal attention of packed prompts.  Sequence s owns rows q_starts[s] .. q_starts[s + 1] - 1 of q and out and rows
- * k_starts[s] .. k_starts[s + 1] - 1 of k and v (k_starts NULL: the same as q_starts); starts are device arrays of seqs + 1
+ * k_starts[s] .. k_starts[s + 1] - 1 of k and v (k_starts NULL: the same as q_starts); rows of k and v are at most 2^25
+ * elements apart; starts are device arrays of seqs + 1
  * ascending offsets.  The queries are the last of the sequence's tokens: query i of n sees keys 0 .. m - n + i of m, so with
  * fewer keys than queries the first n - m queries see nothing.  max_q, max_k: bounds of a sequence's queries and keys
  * on the host; queries beyond max_q are not computed, max_k only guides how the work is split.  scale > 0.  out must not

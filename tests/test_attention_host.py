@@ -136,3 +136,41 @@ def test_parts_follow_the_workspace(attn):
         assert L.abq_attn_set_workspace(ctypes.byref(st), A, parts * per_part + 5) == 0 and st.parts == parts
     assert L.abq_attn_set_workspace(ctypes.byref(st), None, 0) == 0 and st.parts == 1
     assert L.abq_attn_workspace_bytes(ctypes.byref(st)) == need  # what it would take is not what it has
+
+
+def test_sizes_beyond_32_and_64_bits_are_refused(attn):
+    ok = attn.abq_gemm
+    most = 1 << 25  # 63 strides of 2-byte elements, a tile's last row, stay below 2^32
+    assert prompt(attn, k={"row_stride": most}, v={"row_stride": most})[0] == ok.ABQ_OK
+    for name in ("k", "v"):
+        assert prompt(attn, **{name: {"row_stride": most + 8}})[0] == ok.ABQ_ERR_TOO_LARGE
+    assert prompt(attn, q={"row_stride": 1 << 40}, out={"row_stride": 1 << 40})[0] == ok.ABQ_OK  # (addressed in 64 bits)
+    top = 2 ** 31 - 1
+    for kw in ({"max_q": top, "heads": top, "kv_heads": top, "seqs": top}, {"max_q": 1 << 26, "heads": 1 << 25, "kv_heads": 1, "seqs": 1 << 18},
+               {"heads": top, "kv_heads": top, "seqs": top}):  # (the second is 2^64 blocks)
+        assert prompt(attn, **kw)[0] == ok.ABQ_ERR_TOO_LARGE, kw
+    for kw in ({"max_q": 64, "heads": top - 1, "seqs": top}, {"max_q": 64, "heads": 1 << 31 - 6, "cache": {"kv_heads": 1}, "seqs": top}):
+        assert tree(attn, **kw)[0] == ok.ABQ_ERR_TOO_LARGE, kw
+
+
+def test_parts_keep_launches_within_their_limit(attn):
+    L, blocks = attn.lib(), 0xffffffff // 256
+    # a generous bound of the contexts asks for many parts; many sequences leave room for few
+    for seqs, max_q, heads, kv_heads in ((2000, 1, 32, 32), (70000, 1, 32, 8), (300, 64, 32, 8), (20000, 64, 32, 8), (1 << 20, 1, 8, 8)):
+        s, st = tree(attn, cache={"kv_heads": kv_heads}, heads=heads, seqs=seqs, max_q=max_q, max_context=2 ** 31 - 100)
+        assert s == attn.abq_gemm.ABQ_OK, (seqs, max_q)
+        need = L.abq_attn_workspace_bytes(ctypes.byref(st))
+        assert L.abq_attn_set_workspace(ctypes.byref(st), A, need) == 0
+        rows = (max_q * heads // kv_heads + st.block_rows - 1) // st.block_rows
+        assert (seqs * kv_heads * st.parts + 7) // 8 * 8 * rows <= blocks, (seqs, st.parts)
+        assert st.parts == 1 or (seqs * max_q * heads + 3) // 4 <= blocks, (seqs, st.parts)
+
+
+def test_a_scale_of_zero_is_refused_not_replaced(attn):
+    class Fake(attn.torch.Tensor):  # a CPU tensor that says it is on the device: no launch is made
+        is_cuda = True
+    def fake(*shape, dtype=attn.torch.float16):
+        return attn.torch.zeros(shape, dtype=dtype).as_subclass(Fake)
+    q, starts = fake(4, 2, 64), fake(2, dtype=attn.torch.int32)
+    with pytest.raises(attn.AbqError):
+        attn.PromptAttention(q, q, q, starts, scale=0.0, out=q)
