@@ -17,7 +17,7 @@
 // values beside each other for the same reason.  A wave goes from global memory to registers in 16-byte loads and needs no
 // LDS until its tokens are done.
 //
-// A sequence's tokens are split over workgroups (parts) until the chip is covered, and inside one over its four waves, step by
+// A sequence's tokens are split over workgroups (parts) until the chip is covered, and inside one over its waves, step by
 // step; the waves' results are joined in LDS, the parts' by a second launch.
 //
 // Up to 16 rows, bound by the cache's bytes: one query for each of 32 heads on 16 x 1024 tokens of 8 bits, 29 us for 138 MB,
@@ -42,8 +42,8 @@ struct TreeArgs {
     AttnParts parts;
 };
 
-constexpr int kStep = 32;  // tokens of a wave's step
-constexpr int kWaves = 4;
+constexpr int kStep = 32; // tokens of a wave's step
+constexpr int tree_waves(int row_tiles) { return row_tiles == 1 ? 8 : 4; }
 
 __device__ __forceinline__ half2v half2_bits(uint32_t w) { return __builtin_bit_cast(half2v, w); }
 __device__ __forceinline__ uint32_t bits(half2v h) { return __builtin_bit_cast(uint32_t, h); }
@@ -183,9 +183,10 @@ template <int BITS, int D> __device__ __forceinline__ int query_offset(int ks, i
     return (ks / kPieces) * (32 * kPieces) + g * 8 * kPieces + (ks % kPieces) * 8;
 }
 
-template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(256, RT == 1 ? 4 : 2) void attn_tree_kernel(TreeArgs a)
+template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(64 * tree_waves(RT), RT == 1 ? 4 : 2) void attn_tree_kernel(TreeArgs a)
 {
     using S = Step<BITS, ASYM, D>;
+    constexpr int kWaves = tree_waves(RT);
     constexpr int kTiles = D / 16; // 16 x 16 tiles of out^T
     constexpr int kPad = D + 4;
     __shared__ __align__(16) float sums[kWaves][16][kPad];
@@ -413,6 +414,8 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(256, 
         }
     };
     // One row tile leaves registers for four waves per SIMD, which cover each other's loads; with more, a wave loads a step ahead.
+    // Eight waves in a workgroup keep them there where there are few workgroups (of four and of eight: 32768 tokens, 8 heads 25 and 20
+    // us, 20 x 700 tokens 11.3 and 10.2, 16 x 1024 of 32 heads 29 either way; sixteen 20, 10.6, 34).
     if constexpr (RT == 1) {
         for (int step = step0; step < step1; step += kWaves) {
             S s;
@@ -452,7 +455,7 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(256, 
     for (int rt = 0; rt < RT; ++rt) {
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < kTiles; j += kSpan)
+        for (int j = 0; j < kTiles && row0 + 16 * rt + t < rows; j += kSpan)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -461,6 +464,8 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(256, 
         __syncthreads();
         constexpr int kEach = D / 16;
         const int r = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * kEach, row = row0 + 16 * rt + r;
+        if (r >= 16 || row >= rows)
+            continue;
         float most = -INFINITY, total = 0, acc[kEach];
 #pragma unroll
         for (int w = 0; w < kWaves; ++w)
@@ -477,29 +482,27 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(256, 
             for (int e = 0; e < kEach; ++e)
                 acc[e] += f * (sums[w][r][d0 + e] - (ASYM ? stat_z[w][16 * rt + r] : 0.f));
         }
-        if (row < rows) {
-            const int64_t q_row = own.first + row / a.group;
-            const int q_head = head * a.group + row % a.group;
-            if (a.parts.parts > 1) {
-                const int64_t at = (q_row * a.heads + q_head) * a.parts.parts + part;
-                float *to = a.parts.sums + at * D + d0;
+        const int64_t q_row = own.first + row / a.group;
+        const int q_head = head * a.group + row % a.group;
+        if (a.parts.parts > 1) {
+            const int64_t at = (q_row * a.heads + q_head) * a.parts.parts + part;
+            float *to = a.parts.sums + at * D + d0;
 #pragma unroll
-                for (int e = 0; e < kEach; e += 4)
-                    *(float4 *)(to + e) = float4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
-                if ((threadIdx.x & 15) == 0)
-                    a.parts.stats[at] = float2{most, total};
-            } else {
-                const float f = total > 0 ? 1.f / total : total; // (a sum that is not a number stays one)
-                uint16_t *to = (uint16_t *)a.out.data + q_row * a.out.row_stride + (int64_t)q_head * a.out.head_stride + d0;
-                uint32_t x[kEach / 2];
+            for (int e = 0; e < kEach; e += 4)
+                *(float4 *)(to + e) = float4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
+            if ((threadIdx.x & 15) == 0)
+                a.parts.stats[at] = float2{most, total};
+        } else {
+            const float f = total > 0 ? 1.f / total : total; // (a sum that is not a number stays one)
+            uint16_t *to = (uint16_t *)a.out.data + q_row * a.out.row_stride + (int64_t)q_head * a.out.head_stride + d0;
+            uint32_t x[kEach / 2];
 #pragma unroll
-                for (int e = 0; e < kEach / 2; ++e)
-                    x[e] = a.dtype == ABQ_BF16 ? pack16<ABQ_BF16>(acc[2 * e] * f, acc[2 * e + 1] * f) : pack16<ABQ_F16>(acc[2 * e] * f, acc[2 * e + 1] * f);
-                if constexpr (kEach == 8)
-                    *(uint4 *)to = uint4{x[0], x[1], x[2], x[3]};
-                else
-                    *(uint2 *)to = uint2{x[0], x[1]};
-            }
+            for (int e = 0; e < kEach / 2; ++e)
+                x[e] = a.dtype == ABQ_BF16 ? pack16<ABQ_BF16>(acc[2 * e] * f, acc[2 * e + 1] * f) : pack16<ABQ_F16>(acc[2 * e] * f, acc[2 * e + 1] * f);
+            if constexpr (kEach == 8)
+                *(uint4 *)to = uint4{x[0], x[1], x[2], x[3]};
+            else
+                *(uint2 *)to = uint2{x[0], x[1]};
         }
     }
 }
@@ -576,15 +579,23 @@ void plan_attn_tree(abq_attn_state *st, int most_parts)
     st->block_rows = rows <= 16 ? 16 : 32;
     const int64_t units = (int64_t)st->seqs * st->kv_heads * ((rows + st->block_rows - 1) / st->block_rows);
     const int64_t steps = ((int64_t)st->max_k + kStep - 1) / kStep;
-    // Two workgroups per compute unit, no wave without a step; below 24 steps the second launch costs more than parts save (20
-    // sequences of 700 tokens and 8 heads: 11.6 us, in three parts 11.7, and a workspace).  With the cache's bytes from memory, one
-    // sequence of 8000 tokens and 32 heads takes in 1, 4, 16, 32 parts 64, 25, 18, 18.5 us, and 16 of 1024 in 1, 2, 4: 29.1, 32.5,
-    // 34.4.
-    int64_t parts = steps > 24 ? 512 / units : 1;
-    parts = parts < steps / kWaves ? parts : steps / kWaves;
-    // A wave has 32 steps at most, so that sequences much longer than the others are spread: 48 of up to 16384 tokens and 8 heads in
-    // 1, 3, 5, 8 parts 230, 164, 153, 148 us, while 30 of 4000 and 32 heads take 177 - 186 in any number.
-    const int64_t spread = (steps + 32 * kWaves - 1) / (32 * kWaves);
+    // Eight waves of 16 rows, or two times four of 32, per compute unit, the more of a part's waves with a step or two the better: with
+    // the cache's bytes from memory, and up to 16 rows, one sequence takes
+    //   us in parts                        1     2     4     8    16    32
+    //   1000 tokens, 32 key heads         11    10   9.3   8.2               (taken: 8)
+    //   8000 tokens, 32                   46    29    20  17.7  18.4         (8)
+    //   32768 tokens, 8                  168    90    50    29    20    19   (32)
+    //   2 x 2000 tokens, 8                15    13    11     9    11         (8)
+    //   4 x 4096 tokens, 32               33    31    32                     (2)
+    // Up to three steps a wave the second launch costs as much as parts save, or more: one sequence of 8 key heads and one row, 500 tokens
+    // in 1, 2 parts 7.3, 8.5 us, 700 tokens 8.6, 8.8; of 40 rows, 400 tokens in 1, 3 parts 10.5, 10.9, 500 in 1, 4 10.8, 9.8.
+    const int waves = tree_waves(st->block_rows / 16);
+    int64_t parts = steps > (waves == 8 ? 24 : 15) ? 2048 / waves / units : 1;
+    const int64_t busy = steps / 4 < 8 || waves == 4 ? steps / 4 : steps / 8 > 8 ? steps / 8 : 8;
+    parts = parts < busy ? parts : busy;
+    // A wave has 32 steps at most, so that sequences much longer than the others are spread: 48 of up to 16384 tokens and 8 heads, 20
+    // rows, in 1, 3, 5, 8 parts 230, 164, 153, 148 us, while 30 of 4000 and 32 heads, one row, take 175 in any number.
+    const int64_t spread = (steps + 32 * waves - 1) / (32 * waves);
     parts = parts > spread ? parts : spread;
     parts = parts < most_parts ? parts : most_parts;
     // (launches within their limit: this one, rounded up, and the one that joins the parts, four rows of heads per workgroup)
@@ -595,7 +606,7 @@ void plan_attn_tree(abq_attn_state *st, int most_parts)
     st->parts = parts < 1 ? 1 : (int)parts;
 }
 
-#define ABQ_TREE(B, A, D_, RT_) hipLaunchKernelGGL((attn_tree_kernel<B, A, D_, RT_>), grid, dim3(256), 0, stream, a)
+#define ABQ_TREE(B, A, D_, RT_) hipLaunchKernelGGL((attn_tree_kernel<B, A, D_, RT_>), grid, dim3(64 * tree_waves(RT_)), 0, stream, a)
 #define ABQ_TREE_ROWS(B, A, D_)           \
     do {                                  \
         if (st.block_rows == 16)          \
