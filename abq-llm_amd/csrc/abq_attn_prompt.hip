@@ -17,7 +17,7 @@
 // Long prompts are bound by the matrix cores, at the clock that the power left to the chip allows: 16384 tokens, 32 heads of 128
 // on 8 key heads, bf16, 2.2 TFLOP of what queries see, take 1.92 - 2.09 ms (1.05 - 1.15 PFLOP/s; a large matrix product reaches
 // 1.38) with the matrix cores busy in 67 % of clocks, of which there are 1.6 - 1.9 GHz.  Short ones are bound by the chain of
-// steps: a tile's 64 tokens take 0.6 us whatever the grid, so 1024 tokens of 32 heads, 16 tiles, 20 us.
+// steps: a tile's 64 tokens take 0.6 us whatever the grid, so 1024 tokens of 32 heads, 16 tiles, 18 - 20 us.
 #include "abq_attn.h"
 #include "abq_lds_dma.h"
 
