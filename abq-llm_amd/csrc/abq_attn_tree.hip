@@ -24,7 +24,7 @@
 // 4.8 TB/s of the 5.1 that a copy reaches; four waves per SIMD cover each other's loads, so none keeps a second buffer.  With more
 // rows a step's vector work (400 operations beside 32 MFMA: codes to fp16, factors, exponentials) and the loads share the time:
 // two waves per SIMD, each with a step under way while it works at another.  20 rows on 48 ragged contexts, 630 MB: 148 us,
-// 4.3 TB/s; 108 rows on 3 x 5500 tokens of 4 bits, 25 us, bound by that work and, at 12 steps a wave, by its start and end.
+// 4.3 TB/s; 108 rows on 3 x 5500 tokens of 4 bits, 25 us, bound by that work and, at 9 steps a wave, by its start and end.
 #include "abq_attn.h"
 
 namespace abq {
