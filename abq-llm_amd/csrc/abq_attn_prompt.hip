@@ -102,9 +102,12 @@ template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void at
         for (int s = 0; s < D / 16; ++s)
             asm volatile("" : "+v"(q[s].x), "+v"(q[s].y), "+v"(q[s].z), "+v"(q[s].w));
     }
-    // Weights are 2^(score - base + kLift): base follows the running maximum only when that has left it 2^kSlack behind, which
-    // spares nearly every rescaling, and the lift leaves fp16 its normal range down to 2^-20 of the largest weight.
-    constexpr float kSlack = 8, kLift = 6;
+    // Weights are 2^(score - base + lift): base follows the running maximum only when that has left it 2^kSlack behind, which
+    // spares nearly every rescaling.  In fp16 the lift leaves weights their normal range down to 2^-20 of the largest one.  bf16 has
+    // the exponents of the sums, and its values may stand at their end: there the lift keeps the sum of all weights below 1/2, so
+    // that a sum of weights times values stays below the largest of the values.  (At the other end, values below 2^-100 lose digits.)
+    constexpr float kSlack = 8;
+    const float lift = DTYPE == ABQ_BF16 ? -kSlack - 1 - (float)(32 - __builtin_clz((unsigned)ks.count | 1)) : 6.f;
     const float slack = fminf(kSlack / a.scale_log2, 3e38f); // (finite, so that any score is more than that above none)
     float16v out[D / 32];
     float base = -INFINITY, shift = 0, l = 0, most = -INFINITY; // base: in scores; shift: what is added to scores in powers of two
@@ -192,7 +195,7 @@ template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void at
             const float to = fmaxf(most, base);
             const float down = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((base - to) * a.scale_log2);
             base = to;
-            shift = to == -INFINITY ? 0.f : kLift - to * a.scale_log2;
+            shift = to == -INFINITY ? 0.f : lift - to * a.scale_log2;
             l *= down;
 #pragma unroll
             for (int d = 0; d < D / 32; ++d)
@@ -460,7 +463,7 @@ template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void at
         const float mine = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((base - to) * a.scale_log2);
         const float theirs = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((b - to) * a.scale_log2);
         base = to;
-        shift = to == -INFINITY ? 0.f : kLift - to * a.scale_log2;
+        shift = to == -INFINITY ? 0.f : lift - to * a.scale_log2;
         l = l * mine + (upper ? 0.f : other[1][r] * theirs);
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
