@@ -87,7 +87,7 @@ template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void at
     const int first = block * kBlock + wave % (4 / KG) * 32; // the wave's first query
     const int last_key = ahead + min(block * kBlock + kBlock, qs.count) - 1; // seen by the block
     const int tiles = last_key < 0 ? 0 : last_key / kTokens + 1;
-    const int whole = min(max(ahead + block * kBlock + 1, 0) / kTokens, tiles); // tiles that every query sees in full
+    const int whole = min(max(ahead + block * kBlock + 1, 0) / kTokens, last_key / kTokens); // tiles in front of the last that every query sees in full
     const int tile0 = (int)((int64_t)tiles * part / a.parts.parts), tile1 = (int)((int64_t)tiles * (part + 1) / a.parts.parts);
 
     uint4 q[D / 16];
@@ -191,7 +191,7 @@ template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void at
         most = max_across_halves(x);
     };
     auto follow = [&]() {
-        if (__any(most > base + slack)) {
+        if (__any(most - base > slack)) { // (the difference has no rounding, base + slack would)
             const float to = fmaxf(most, base);
             const float down = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((base - to) * a.scale_log2);
             base = to;
@@ -353,9 +353,12 @@ template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void at
     asm volatile("" : "+v"(none));
     const int upper = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, none)) >> 5;
 
+    // A block is done again, step by step, in two cases.
     // A weight of 0 does not keep a value that is not finite out of a product, so one that no query may see can have come into the
-    // sums.  A block whose sums are not all finite is done again, step by step: where a tile that some query does not see all of
-    // holds such values, zeros take their places, and they are added after the product to the queries that see them.
+    // sums.  Where they are not all finite, and a tile that some query does not see all of holds such values, zeros take their
+    // places, and they are added after the product to the queries that see them.
+    // Scores from 2^24 powers of two on leave no room for a lift that is added to them: fp32 has steps of 2 and more there.  The base
+    // is taken off them first, which has no rounding near it.
     if (whole < tiles) {
         float any = 0;
 #pragma unroll
@@ -363,7 +366,7 @@ template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void at
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 any = __builtin_fmaf(out[d][i], 0.f, any);
-        const bool found = __any(!(any == 0));
+        const bool found = __any(!(any == 0) || (fabsf(base) < INFINITY && fabsf(base) * a.scale_log2 >= 0x1p24f));
         if (lane == 0)
             odd_values[wave] = found;
         __syncthreads();
@@ -398,6 +401,15 @@ template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void at
                     hide(tile, score);
                 find_most(score);
                 follow();
+                shift = lift;
+                {
+                    const float from = fabsf(base) < INFINITY ? base : 0.f;
+#pragma unroll
+                    for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            score[tt][i] -= from;
+                }
 #pragma unroll
                 for (int i = 0; i < 8 * TT; ++i)
                     weigh(i, score);
@@ -434,6 +446,7 @@ template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void at
                     }
                 }
             }
+            shift = base == -INFINITY ? 0.f : lift - base * a.scale_log2;
         }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // (nothing may arrive in LDS that is another's, or holds sums)

@@ -35,3 +35,62 @@ def test_values_of_any_size_in_bf16(attn, top, dim, lens, k_lens, heads, block, 
     down = 2.0 ** -100
     want, allowed = prompt_reference(q[:, some], k, (v.double() * down).float(), lens, k_lens, dim ** -0.5)
     check((got.double() * down).float(), want, allowed, top)
+
+
+def equal_keys(dtype, dim, T, gen):
+    """(q row, key row, scale): scores of T in powers of two"""
+    q = (1 + torch.rand(dim, generator=gen)).to(dtype)
+    k = (1 + torch.rand(dim, generator=gen)).to(dtype)
+    scale = T / float(q.double() @ k.double()) / 1.4426950408889634
+    return q, k, scale
+
+
+def mean_bound(v, dtype, u_weight):
+    """Mean of the first 1, 2, .. tokens' values, and what may be off it: equal weights are rounded alike (u_weight), their sum in fp32
+    is off by 2^-23 a term, and the result is rounded once"""
+    count = torch.arange(1, v.shape[0] + 1, dtype=torch.float64)[:, None]
+    mean, size = v.double().cumsum(0) / count, v.double().abs().cumsum(0) / count
+    u = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[dtype]
+    return mean, size * (u_weight + count * 2.0 ** -23) + mean.abs() * u * 1.01 + 2.0 ** -24
+
+
+# (between them, steps of fp32 at such scores are 1, 2, 4 .. in powers of two)
+LEVELS = [2.0 ** e * x for e in (18, 23, 24, 25, 26, 27, 28, 30, 33, 40) for x in (1.13, 1.71)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("heads,tokens,m,split", [(2, 150, 150, False), (2, 150, 1500, True), (256, 150, 150, False), (2, 1, 128, False)])
+def test_prompts_whose_scores_are_large_and_equal(attn, dtype, sign, heads, tokens, m, split):
+    """Equal scores mean equal weights, whatever their size: every query gets the mean of the values that it sees"""
+    gen = torch.Generator().manual_seed(22)
+    dim = 64
+    v = torch.randn(m, 1, dim, generator=gen).to(dtype)
+    want, allowed = mean_bound(v[:, 0], dtype, {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[dtype])
+    for T in LEVELS:
+        q, k, scale = equal_keys(dtype, dim, T, gen)
+        call = attn.PromptAttention((sign * q).expand(tokens, heads, dim).contiguous().cuda(), k.expand(m, 1, dim).contiguous().cuda(), v.cuda(),
+                                    starts([tokens]), starts([m]), tokens, m, scale=scale)
+        assert (call.state.block_rows, call.state.parts > 1) == (128 if heads > 2 else 64, split)
+        got = call.run().cpu()
+        for h in (0, heads - 1):
+            check(got[:, h], want[m - tokens:], allowed[m - tokens:], (T, h))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("split", [False, True])
+def test_prompts_whose_scores_are_large_and_far_apart(attn, dtype, split):
+    """One key ahead of the others by a quarter of its score takes all"""
+    gen = torch.Generator().manual_seed(23)
+    dim, tokens, m, at = 128, 30, 1000, 333
+    v = torch.randn(m, 1, dim, generator=gen).to(dtype)
+    for T in LEVELS:
+        q, k, scale = equal_keys(dtype, dim, T, gen)
+        keys = (k * (0.25 + 0.5 * torch.rand(m, 1, 1, generator=gen))).to(dtype)
+        keys[at, 0] = k
+        call = attn.PromptAttention(q.expand(tokens, 1, dim).contiguous().cuda(), keys.cuda(), v.cuda(), starts([tokens]), starts([m]), tokens, m, scale=scale,
+                                    workspace=None if split else torch.empty(0, device="cuda"))
+        assert (call.state.parts > 1) == split
+        want = v[at].double().expand(tokens, 1, dim)
+        u = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[dtype]
+        check(call.run().cpu(), want, want.abs() * 2.1 * u + 2.0 ** -24, T)
