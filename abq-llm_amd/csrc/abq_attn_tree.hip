@@ -360,11 +360,13 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(64 * 
                 for (int i = 0; i < 4; ++i)
                     most = fmaxf(most, score[rt][h][i]);
             most = max_across_quarters(most);
-            if (__any(most > base[rt] + kSlack)) {
+            if (__any(most - base[rt] > kSlack)) { // (the difference has no rounding)
                 const float to = fmaxf(most, base[rt]);
                 const float down = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(base[rt] - to);
                 base[rt] = to;
-                shift[rt] = to == -INFINITY ? 0.f : kLift - to;
+                // (from 2^24 on the lift is rounded to steps of 2 and more: never to more than it is)
+                const float lifted = kLift - to;
+                shift[rt] = to == -INFINITY ? 0.f : lifted + to > kLift ? -to : lifted;
                 l[rt] *= down;
                 z[rt] *= down;
 #pragma unroll

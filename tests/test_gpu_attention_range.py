@@ -4,7 +4,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from attention_reference import check, load_abq_attention  # noqa: E402
+from attention_reference import cache_contents, check, load_abq_attention  # noqa: E402
 from test_gpu_attention import prompt_reference, starts  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -94,3 +94,30 @@ def test_prompts_whose_scores_are_large_and_far_apart(attn, dtype, split):
         want = v[at].double().expand(tokens, 1, dim)
         u = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[dtype]
         check(call.run().cpu(), want, want.abs() * 2.1 * u + 2.0 ** -24, T)
+
+
+def tree_of(attn, v, k, bits, symmetric, dtype):
+    tokens, _, dim = v.shape
+    cache = attn.KvCache((tokens + 63) // 64, 64, 1, dim, bits=bits, symmetric=symmetric)
+    cache.append(k.to(dtype).cuda(), v.to(dtype).cuda(), torch.arange(tokens, dtype=torch.int32).cuda())
+    _, vc, _, (vs, vz) = cache_contents(cache)
+    held = torch.from_numpy((vc[:tokens, 0] - vz[:tokens, 0, None]) * vs[:tokens, 0, None].astype("float64"))
+    return cache, torch.arange((tokens + 63) // 64, dtype=torch.int32).cuda()[None], held
+
+
+@pytest.mark.parametrize("bits,symmetric", [(8, True), (8, False), (4, True), (4, False)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads,tokens", [(3, 70), (3, 1500), (40, 300)])
+def test_drafts_whose_scores_are_large_and_equal(attn, bits, symmetric, dtype, heads, tokens):
+    gen = torch.Generator().manual_seed(24)
+    dim = 128
+    v = torch.randn(tokens, 1, dim, generator=gen)
+    v[:, :, 0], v[:, :, 1] = 4, -4  # (one range, so one scale and one zero point: then the weights are alike too)
+    for T in LEVELS:
+        q, k, scale = equal_keys(dtype, dim, T, gen)
+        cache, table, held = tree_of(attn, v.clamp(-4, 4), k.expand(tokens, 1, dim), bits, symmetric, dtype)
+        mean, allowed = mean_bound(held, dtype, 2.0 ** -11)
+        call = attn.TreeAttention(q.expand(1, heads, dim).contiguous().cuda(), cache, table, torch.tensor([tokens - 1], dtype=torch.int32).cuda(), starts([1]), 1,
+                                  tokens - 1, scale=scale)
+        assert call.state.block_rows == (16 if heads <= 16 else 32) and (call.state.parts > 1 or tokens < 1000)
+        check(call.run().cpu()[0], mean[-1].expand(heads, dim), allowed[-1].expand(heads, dim), T)
