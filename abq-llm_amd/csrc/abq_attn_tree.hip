@@ -144,16 +144,20 @@ __device__ __forceinline__ void eight_codes(const Magic &m, uint32_t w, uint32_t
     out[3] = bits(half2_bits((w8 & 0x00f000f0u) | m.halves) * part - off16);
 }
 
-// score * k_factor + k_offset * qsum + v_log of token K of the lane's eight and of those behind it
+// (score * k_factor + k_offset * qsum) * factor + v_log of token K of the lane's eight and of those behind it.  The row's power of
+// two comes last: in units of codes a score that fp32 holds may be beyond it.
 template <bool ASYM, int RT, int K>
-__device__ __forceinline__ void exponents(float (&score)[RT][2][4], float k_factor, float k_offset, float v_log, const float (&qsum)[RT])
+__device__ __forceinline__ void exponents(float (&score)[RT][2][4], float k_factor, float k_offset, float v_log, const float (&qsum)[RT],
+                                          const float (&factor)[RT])
 {
     if constexpr (K < 8) {
         const float f = of_lane<K>(k_factor), v = of_lane<K>(v_log), o = ASYM ? of_lane<K>(k_offset) : 0.f;
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-            score[rt][K / 4][K % 4] = __builtin_fmaf(score[rt][K / 4][K % 4], f, ASYM ? __builtin_fmaf(o, qsum[rt], v) : v);
-        exponents<ASYM, RT, K + 1>(score, k_factor, k_offset, v_log, qsum);
+        for (int rt = 0; rt < RT; ++rt) {
+            const float x = score[rt][K / 4][K % 4] * f;
+            score[rt][K / 4][K % 4] = __builtin_fmaf(ASYM ? __builtin_fmaf(o, qsum[rt], x) : x, factor[rt], v);
+        }
+        exponents<ASYM, RT, K + 1>(score, k_factor, k_offset, v_log, qsum, factor);
     }
 }
 // sum + the tokens' weights times their v
@@ -213,7 +217,7 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(64 * 
     const int32_t *pages = a.page_table + (int64_t)seq * a.max_pages;
     const int last_page = (len - 1) >> a.page_shift; // (len is 0 only without steps)
 
-    // the queries, the power of two that they were divided by, and their sums
+    // the queries as the products take them, the power of two that they were divided by, and their sums
     half8v q[RT][D / 32];
     float factor[RT], qsum[RT];
     uint64_t sees[RT];
@@ -261,7 +265,7 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(64 * 
 #pragma unroll
                 for (int i = 0; i < 8; i += 2)
                     sum = __builtin_amdgcn_fdot2(half2v{q[rt][ks][i], q[rt][ks][i + 1]}, half2v{(_Float16)1, (_Float16)1}, sum, false);
-        qsum[rt] = ASYM ? sum_across_quarters(sum) * factor[rt] : 0;
+        qsum[rt] = ASYM ? sum_across_quarters(sum) : 0;
     }
 
     float4v out[RT][kTiles];
@@ -307,7 +311,7 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(64 * 
             for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    score[rt][h][i] = acc[rt][i] * factor[rt];
+                    score[rt][h][i] = acc[rt][i];
         }
         // The lane's one token: factor and offset of the scores, logarithm and reciprocal of the value scale.  (Codes are less half
         // their range here, and so are zero points.)  What no row sees holds anything, and is replaced.
@@ -337,7 +341,7 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(64 * 
             z_high = pack16<ABQ_F16>(xh, yh);
             high = __any(xh != 0);
         }
-        exponents<ASYM, RT, 0>(score, k_factor, k_offset, v_log, qsum);
+        exponents<ASYM, RT, 0>(score, k_factor, k_offset, v_log, qsum, factor);
         if (some)
 #pragma unroll
             for (int h = 0; h < 2; ++h)

@@ -121,3 +121,20 @@ def test_drafts_whose_scores_are_large_and_equal(attn, bits, symmetric, dtype, h
                                   tokens - 1, scale=scale)
         assert call.state.block_rows == (16 if heads <= 16 else 32) and (call.state.parts > 1 or tokens < 1000)
         check(call.run().cpu()[0], mean[-1].expand(heads, dim), allowed[-1].expand(heads, dim), T)
+
+
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("size", [1e30, 1e34, 1e35])
+def test_bf16_queries_near_the_types_end_on_the_cache(attn, symmetric, size):
+    """Scores that fp32 holds, of queries that in units of the keys' codes it does not"""
+    gen = torch.Generator().manual_seed(25)
+    dim, tokens, at = 128, 100, 41
+    v = torch.randn(tokens, 1, dim, generator=gen)
+    keys = 0.5 * torch.rand(tokens, 1, dim, generator=gen)
+    keys[at] = 0.75 + 0.25 * torch.rand(dim, generator=gen)
+    keys[:, :, 0], keys[:, :, 1] = 1, 0.01
+    cache, table, held = tree_of(attn, v, keys, 8, symmetric, torch.bfloat16)
+    q = (size * (0.5 + 0.5 * torch.rand(1, 2, dim, generator=gen))).bfloat16()
+    got = attn.TreeAttention(q.cuda(), cache, table, torch.tensor([tokens - 1], dtype=torch.int32).cuda(), starts([1]), 1, tokens - 1).run()
+    want = held[at].expand(1, 2, dim)
+    check(got.cpu(), want, want.abs() * 2.0 ** -8 * 1.1 + held.abs().max() * 2.0 ** -18, size)
