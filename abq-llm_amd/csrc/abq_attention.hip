@@ -17,6 +17,9 @@ constexpr int kPromptKind = 1, kTreeKind = 2;
 // A tile of keys or values is addressed from its first row in 32 bits: 63 strides of 2-byte elements and a row
 constexpr int64_t kMostTileStride = 1 << 25;
 
+// Scales that fp32 holds times log2(e), and for drafts times a token's scale and zero point, of up to 1e4 each, as well
+constexpr float kMostPromptScale = 2e38f, kMostTreeScale = 2e30f;
+
 // a * b * c, none of them negative, or more than any limit here where that does not fit
 int64_t product(int64_t a, int64_t b, int64_t c)
 {
@@ -73,7 +76,7 @@ abq_status init_common(int kind, const abq_rows *q, const abq_rows *out, int dty
                        int seqs, int max_q, float scale, abq_attn_state *st)
 {
     if (!q || !out || !q_starts || (dtype != ABQ_F16 && dtype != ABQ_BF16) || heads <= 0 || kv_heads <= 0 || seqs <= 0 || max_q <= 0 ||
-        q->rows < 0 || !(scale > 0) || !(scale <= 3e38f))
+        q->rows < 0 || !(scale > 0) || !(scale <= (kind == kTreeKind ? kMostTreeScale : kMostPromptScale)))
         return ABQ_ERR_INVALID_ARG;
     if (head_dim != 64 && head_dim != 128)
         return ABQ_ERR_UNSUPPORTED;

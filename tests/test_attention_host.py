@@ -174,3 +174,13 @@ def test_a_scale_of_zero_is_refused_not_replaced(attn):
     q, starts = fake(4, 2, 64), fake(2, dtype=attn.torch.int32)
     with pytest.raises(attn.AbqError):
         attn.PromptAttention(q, q, q, starts, scale=0.0, out=q)
+
+
+def test_scales_whose_product_with_a_tokens_is_beyond_fp32_are_refused(attn):
+    ok = attn.abq_gemm
+    for scale in (1e-38, 1e20, 2e30):
+        assert prompt(attn, scale=scale)[0] == ok.ABQ_OK and tree(attn, scale=scale)[0] == ok.ABQ_OK, scale
+    for scale in (3e30, 2e38):  # a token's scale and zero point may be 1e4 each
+        assert prompt(attn, scale=scale)[0] == ok.ABQ_OK and tree(attn, scale=scale)[0] == ok.ABQ_ERR_INVALID_ARG, scale
+    for scale in (2.5e38, 3e38):  # beyond fp32 once it is taken in powers of two
+        assert prompt(attn, scale=scale)[0] == ok.ABQ_ERR_INVALID_ARG and tree(attn, scale=scale)[0] == ok.ABQ_ERR_INVALID_ARG, scale
