@@ -19,8 +19,8 @@ hipError_t launch_attn_tree(const abq_attn_state &st, hipStream_t stream);
 void plan_attn_prompt(abq_attn_state *st, int most_parts);
 void plan_attn_tree(abq_attn_state *st, int most_parts);
 
-// HIP counts the threads of a launch in 32 bits
-constexpr int64_t kMostBlocks = 0xffffffffll / 256;
+// HIP counts the threads of a launch in 32 bits; workgroups have 256, where nothing else is said
+constexpr int64_t kMostThreads = 0xffffffffll, kMostBlocks = kMostThreads / 256;
 
 // Bytes of the parts' results: per query row and head, `parts` sums of head_dim floats and as many pairs (maximum, sum)
 inline size_t attn_parts_bytes(const abq_attn_state &st, int parts)

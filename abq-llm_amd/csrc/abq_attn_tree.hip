@@ -581,9 +581,11 @@ void plan_attn_tree(abq_attn_state *st, int most_parts)
     const int rows = st->max_q * (st->heads / st->kv_heads);
     // Blocks of 32 rows read a code once for two products, where there are two: 27 drafts of 4 heads per key head on 3 x 5500 tokens of
     // 4 bits 30.5 us, in blocks of 16 rows 32; 48 ragged contexts, 20 rows, 147.5 and 173.  (64 drafts on 4000 tokens, or 16 of 4 heads
-    // on 4 x 2000, take the same in either: 20.8, 15.)  Up to 16 rows the second half would be empty.
-    st->block_rows = rows <= 16 ? 16 : 32;
-    const int64_t units = (int64_t)st->seqs * st->kv_heads * ((rows + st->block_rows - 1) / st->block_rows);
+    // on 4 x 2000, take the same in either: 20.8, 15.)  Up to 16 rows the second half would be empty, but the workgroups have half as many
+    // threads, and twice as many of them fit a launch.
+    const int64_t key_heads = (int64_t)st->seqs * st->kv_heads;
+    st->block_rows = rows <= 16 && key_heads + 8 <= kMostThreads / (64 * tree_waves(1)) ? 16 : 32;
+    const int64_t units = key_heads * ((rows + st->block_rows - 1) / st->block_rows);
     const int64_t steps = ((int64_t)st->max_k + kStep - 1) / kStep;
     // Eight waves of 16 rows, or two times four of 32, per compute unit, the more of a part's waves with a step or two the better: with
     // the cache's bytes from memory, and up to 16 rows, one sequence takes
@@ -605,7 +607,7 @@ void plan_attn_tree(abq_attn_state *st, int most_parts)
     parts = parts > spread ? parts : spread;
     parts = parts < most_parts ? parts : most_parts;
     // (launches within their limit: this one, rounded up, and the one that joins the parts, four rows of heads per workgroup)
-    const int64_t row_blocks = (rows + st->block_rows - 1) / st->block_rows, most = kMostBlocks / (units + 8 * row_blocks);
+    const int64_t row_blocks = (rows + st->block_rows - 1) / st->block_rows, most = kMostThreads / (64 * waves) / (units + 8 * row_blocks);
     parts = parts < most ? parts : most;
     if ((int64_t)st->seqs * st->max_q > 4 * kMostBlocks / st->heads)
         parts = 1;

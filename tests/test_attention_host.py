@@ -8,6 +8,7 @@ import pytest
 
 pytest.importorskip("torch")
 
+from attention_launch_probe import launches  # noqa: E402
 from attention_reference import load_abq_attention  # noqa: E402
 from conftest import ROOT  # noqa: E402
 
@@ -184,3 +185,20 @@ def test_scales_whose_product_with_a_tokens_is_beyond_fp32_are_refused(attn):
         assert prompt(attn, scale=scale)[0] == ok.ABQ_OK and tree(attn, scale=scale)[0] == ok.ABQ_ERR_INVALID_ARG, scale
     for scale in (2.5e38, 3e38):  # beyond fp32 once it is taken in powers of two
         assert prompt(attn, scale=scale)[0] == ok.ABQ_ERR_INVALID_ARG and tree(attn, scale=scale)[0] == ok.ABQ_ERR_INVALID_ARG, scale
+
+
+def test_launches_stay_within_the_threads_that_hip_counts(attn, tmp_path):
+    """Grid times workgroup of every launch below 2^32, whatever bound of the contexts is given"""
+    sizes = [(64, 1, 32, 32, 1 << 25), (128, 1, 32, 32, 2 ** 31 - 164), (2000, 1, 32, 32, 2 ** 31 - 164), (70000, 1, 32, 8, 2 ** 31 - 164),
+             (1 << 20, 1, 8, 8, 100), (1 << 20, 1, 8, 8, 2 ** 31 - 164), (131071, 1, 64, 64, 100), (131072, 1, 64, 64, 100), (262143, 4, 64, 32, 100),
+             (20000, 64, 32, 8, 2 ** 31 - 164), (300, 64, 32, 8, 2 ** 31 - 164)]
+    calls = [dict(kind="tree", rows=s * n, seqs=s, max_q=n, heads=h, kv_heads=kv, max_k=m) for s, n, h, kv, m in sizes]
+    for c, r in zip(calls, launches(tmp_path, calls)):
+        assert r["status"] == [0, 0, 0] and len(r["launches"]) == (1 if r["parts"] == 1 else 2), (c, r)
+        for made in r["launches"]:
+            assert made["grid"][0] * made["block"][0] < 2 ** 32 and made["grid"][1:] == made["block"][1:] == [1, 1], (c, made)
+        rows = c["max_q"] * c["heads"] // c["kv_heads"]  # every row block of every part has its workgroup
+        blocks = (rows + r["block_rows"] - 1) // r["block_rows"]
+        assert r["launches"][0]["grid"][0] >= c["seqs"] * c["kv_heads"] * r["parts"] * blocks, (c, r)
+    for c, r in zip(calls, launches(tmp_path, [dict(c, workspace=0) for c in calls])):
+        assert r["status"] == [0, 0, 0] and r["parts"] == 1 and r["launches"][0]["grid"][0] * r["launches"][0]["block"][0] < 2 ** 32, (c, r)
