@@ -538,7 +538,7 @@ void plan_attn_prompt(abq_attn_state *st, int most_parts)
     //   1024 alone, 8 heads of 128               15    17    18                     (1)
     //   333 behind 7000, 8 heads of 64           62    38    24    20    22    25   (10)
     const int64_t groups = ((int64_t)st->max_q + st->block_rows - 1) / st->block_rows * each;
-    const double steps = (st->max_k + kTokens - 1) / kTokens, step_us = st->head_dim == 64 ? 0.5 : 0.6;
+    const double steps = ((int64_t)st->max_k + kTokens - 1) / kTokens, step_us = st->head_dim == 64 ? 0.5 : 0.6;
     const double result_us = (double)st->q.rows * st->heads * st->head_dim * 8 / 4e6;
     int64_t most = (st->head_dim == 64 ? 512 : 256) / groups, parts = 1;
     most = most < steps / 4 ? most : (int64_t)(steps / 4);

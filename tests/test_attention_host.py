@@ -202,3 +202,10 @@ def test_launches_stay_within_the_threads_that_hip_counts(attn, tmp_path):
         assert r["launches"][0]["grid"][0] >= c["seqs"] * c["kv_heads"] * r["parts"] * blocks, (c, r)
     for c, r in zip(calls, launches(tmp_path, [dict(c, workspace=0) for c in calls])):
         assert r["status"] == [0, 0, 0] and r["parts"] == 1 and r["launches"][0]["grid"][0] * r["launches"][0]["block"][0] < 2 ** 32, (c, r)
+
+
+def test_a_bound_of_the_keys_as_large_as_its_type_splits_them_as_any_large_one(attn, tmp_path):
+    base = dict(kind="prompt", rows=64, heads=4, kv_heads=4, seqs=1, max_q=64)
+    large = [dict(base, max_k=m) for m in (1 << 30, 2 ** 31 - 64, 2 ** 31 - 63, 2 ** 31 - 1)]
+    made = launches(tmp_path, large)
+    assert all(r["status"] == [0, 0, 0] and r == made[0] and r["parts"] == 64 for r in made), made
