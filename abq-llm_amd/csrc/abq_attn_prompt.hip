@@ -30,7 +30,7 @@ namespace {
 struct PromptArgs {
     abq_rows q, k, v, out;
     const int32_t *q_starts, *k_starts;
-    int heads, kv_heads, seqs, blocks; // blocks: of queries in the longest sequence
+    int heads, kv_heads, seqs, max_q, blocks; // blocks: of queries in the longest sequence
     float scale_log2;
     AttnParts parts;
 };
@@ -81,18 +81,19 @@ template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void at
     const int kv_head = order % a.kv_heads, head = kv_head * (a.heads / a.kv_heads) + order / a.kv_heads;
 
     const SeqRows qs = seq_rows(a.q_starts, seq, a.q.rows), ks = seq_rows(a.k_starts, seq, a.k.rows);
-    if (block * kBlock >= qs.count)
+    const int n = min(qs.count, a.max_q); // its queries that are computed
+    if (block * kBlock >= n)
         return;
     const int ahead = ks.count - qs.count; // query i sees keys up to ahead + i
     const int first = block * kBlock + wave % (4 / KG) * 32; // the wave's first query
-    const int last_key = ahead + min(block * kBlock + kBlock, qs.count) - 1; // seen by the block
+    const int last_key = ahead + min(block * kBlock + kBlock, n) - 1; // seen by the block
     const int tiles = last_key < 0 ? 0 : last_key / kTokens + 1;
     const int whole = min(max(ahead + block * kBlock + 1, 0) / kTokens, last_key / kTokens); // tiles in front of the last that every query sees in full
     const int tile0 = (int)((int64_t)tiles * part / a.parts.parts), tile1 = (int)((int64_t)tiles * (part + 1) / a.parts.parts);
 
     uint4 q[D / 16];
     {
-        const int64_t row = qs.first + min(first + ql, qs.count - 1);
+        const int64_t row = qs.first + min(first + ql, n - 1);
         const uint16_t *src = (const uint16_t *)a.q.data + row * a.q.row_stride + (int64_t)head * a.q.head_stride + 8 * half;
 #pragma unroll
         for (int s = 0; s < D / 16; ++s)
@@ -488,7 +489,7 @@ template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void at
     const float total = sum_across_halves(l);
     const int i = first + ql;
     if (a.parts.parts > 1) {
-        if (i < qs.count) {
+        if (i < n) {
             const int64_t at = ((int64_t)(qs.first + i) * a.heads + head) * a.parts.parts + part;
 #pragma unroll
             for (int d = 0; d < D / 32; ++d)
@@ -515,7 +516,7 @@ template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void at
                     x[y][e] = pack16<DTYPE>(out[d][8 * j + 4 * y + 2 * e] * f, out[d][8 * j + 4 * y + 2 * e + 1] * f);
             const auto r0 = __builtin_amdgcn_permlane32_swap(x[0][0], x[1][0], false, false);
             const auto r1 = __builtin_amdgcn_permlane32_swap(x[0][1], x[1][1], false, false);
-            if (i < qs.count)
+            if (i < n)
                 *(uint4 *)(to + 32 * d + 16 * j + 8 * upper) = uint4{r0[0], r1[0], r0[1], r1[1]};
         }
 }
@@ -580,6 +581,7 @@ hipError_t launch_attn_prompt(const abq_attn_state &st, hipStream_t stream)
     a.heads = st.heads;
     a.kv_heads = st.kv_heads;
     a.seqs = st.seqs;
+    a.max_q = st.max_q;
     a.blocks = (st.max_q + st.block_rows - 1) / st.block_rows;
     a.scale_log2 = st.scale * kLog2e;
     a.parts = attn_parts(st);

@@ -36,7 +36,7 @@ struct TreeArgs {
     abq_rows q, out;
     const int32_t *page_table, *context, *q_starts;
     const uint64_t *mask;
-    int heads, group, seqs, max_pages, row_blocks, dtype;
+    int heads, group, seqs, max_q, max_pages, row_blocks, dtype;
     int page_shift;
     float scale_log2;
     AttnParts parts;
@@ -207,8 +207,8 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(64 * 
     const int part = unit % a.parts.parts, head = unit / a.parts.parts % a.c.kv_heads, seq = unit / a.parts.parts / a.c.kv_heads;
 
     const SeqRows own = seq_rows(a.q_starts, seq, a.q.rows);
-    const int n = min(own.count, 64);
-    const int rows = n * a.group, row0 = row_block * 16 * RT;
+    const int n = min(own.count, 64); // drafts that can be seen, of which max_q are computed
+    const int rows = min(n, a.max_q) * a.group, row0 = row_block * 16 * RT;
     if (row0 >= rows)
         return;
     const int64_t places = (int64_t)a.max_pages << a.page_shift;
@@ -643,6 +643,7 @@ hipError_t launch_attn_tree(const abq_attn_state &st, hipStream_t stream)
     a.heads = st.heads;
     a.group = st.heads / st.kv_heads;
     a.seqs = st.seqs;
+    a.max_q = st.max_q;
     a.max_pages = st.max_pages;
     a.row_blocks = (st.max_q * a.group + st.block_rows - 1) / st.block_rows;
     a.dtype = st.dtype;

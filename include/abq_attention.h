@@ -108,22 +108,22 @@ typedef struct abq_attn_state {
 
 /* Causal attention of packed prompts.  Sequence s owns rows q_starts[s] .. q_starts[s + 1] - 1 of q and out and rows
  * k_starts[s] .. k_starts[s + 1] - 1 of k and v (k_starts NULL: the same as q_starts); rows of k and v are at most 2^25
- * elements apart; starts are device arrays of seqs + 1
- * ascending offsets.  The queries are the last of the sequence's tokens: query i of n sees keys 0 .. m - n + i of m, so with
- * fewer keys than queries the first n - m queries see nothing.  max_q, max_k: bounds of a sequence's queries and keys
- * on the host; queries beyond max_q are not computed, max_k only guides how the work is split.  0 < scale <= 2e38.
- * out must not overlap q, k or v.  A sequence may be empty. */
+ * elements apart; starts are device arrays of seqs + 1 ascending offsets.  The queries are the last of the sequence's tokens:
+ * query i of n sees keys 0 .. m - n + i of m, so with fewer keys than queries the first n - m queries see nothing.  max_q,
+ * max_k: bounds of a sequence's queries and keys on the host; queries beyond max_q are not computed and their rows of out stay
+ * as they are, max_k only guides how the work is split.  0 < scale <= 2e38.  out must not overlap q, k or v.  A sequence may
+ * be empty. */
 abq_status abq_attn_prompt_init(const abq_rows *q, const abq_rows *k, const abq_rows *v, const abq_rows *out, int dtype, int heads,
                                 int kv_heads, int head_dim, const int32_t *q_starts, const int32_t *k_starts, int seqs, int max_q,
                                 int max_k, float scale, abq_attn_state *state);
 
 /* Attention of drafted tokens over the quantised cache.  Sequence s holds context[s] tokens in the cache and behind them its
- * drafts, rows q_starts[s] .. q_starts[s + 1] - 1 of q and out (at most max_q <= 64), whose keys and values have been
- * appended at the places that follow the context.  Place t of sequence s is offset t % page_size of page
- * page_table[s * max_pages + t / page_size]; places on pages outside the cache, or beyond max_pages, are not seen.
- * Draft i sees the context and the drafts j whose bit j is set in mask[q_starts[s] + i] (itself only if its own bit is);
- * mask NULL: drafts 0 .. i, a chain.  One draft per sequence and no mask is ordinary decoding.  max_context only guides how
- * the work is split.  0 < scale <= 2e30. */
+ * drafts, rows q_starts[s] .. q_starts[s + 1] - 1 of q and out (at most 64), whose keys and values have been appended at the
+ * places that follow the context.  Drafts beyond max_q <= 64 are not computed, and their rows of out stay as they are, but
+ * they can be seen.  Place t of sequence s is offset t % page_size of page page_table[s * max_pages + t / page_size]; places on
+ * pages outside the cache, or beyond max_pages, are not seen.  Draft i sees the context and the drafts j whose bit j is set in
+ * mask[q_starts[s] + i] (itself only if its own bit is); mask NULL: drafts 0 .. i, a chain.  One draft per sequence and no
+ * mask is ordinary decoding.  max_context only guides how the work is split.  0 < scale <= 2e30. */
 abq_status abq_attn_tree_init(const abq_kv_cache *cache, const abq_rows *q, const abq_rows *out, int dtype, int heads,
                               const int32_t *page_table, int max_pages, const int32_t *context, const int32_t *q_starts,
                               const uint64_t *mask, int seqs, int max_q, int max_context, float scale, abq_attn_state *state);
