@@ -104,6 +104,33 @@ def _index(t, dtype, numel, what):
     return t.data_ptr()
 
 
+def _stream_of(stream):
+    """The torch stream that a call's argument stands for"""
+    if stream is None:
+        return torch.cuda.current_stream()
+    return torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream
+
+
+class _Memory:
+    """Tensors that an object of this module allocated.  They belong to the stream that was current then.  A call on another stream first
+    has that one wait for what still goes on with them here (once), and keeps them from being handed out again before it is done."""
+
+    def __init__(self, tensors):
+        self.tensors, self.home = tensors, torch.cuda.current_stream()
+        self.known = {self.home.cuda_stream or None}  # (as ctypes has a null pointer)
+
+    def use(self, stream):
+        other = _stream_of(stream)
+        with torch.cuda.stream(other):
+            captured = torch.cuda.is_current_stream_capturing()
+        for t in self.tensors:
+            t.record_stream(other)
+        if self.tensors and not captured:
+            other.wait_stream(self.home)
+        if not captured:  # (a capture may not wait for what is outside of it, and is replayed behind it)
+            self.known.add(other.cuda_stream or None)
+
+
 class KvCache:
     """A paged cache of keys and values in codes of 8 or 4 bits with a scale (and a zero point) per token and head.
 
@@ -120,13 +147,17 @@ class KvCache:
         self.desc = d
         self._ref, self._row = ctypes.byref(d), (kv_heads, head_dim)
         self._append, self._read = lib().abq_kv_append, lib().abq_kv_read
+        self._memory = _Memory((self.k_codes, self.v_codes, self.k_scales, self.v_scales))
+        self._known = self._memory.known
 
     def _call(self, call, name, k, v, slots, stream):
         shape = k.shape
         if shape != v.shape or k.dtype is not v.dtype or shape[1:] != self._row:
             raise ValueError("keys and values [tokens, %d, %d] of one type are wanted" % self._row)
-        at = _index(slots, torch.int32, shape[0], "slots")
-        status = call(self._ref, ctypes.byref(_rows(k)), ctypes.byref(_rows(v)), _dtype(k), at, abq_gemm._stream_ptr(stream))
+        at, on = _index(slots, torch.int32, shape[0], "slots"), abq_gemm._stream_ptr(stream)
+        if on.value not in self._known:
+            self._memory.use(stream)
+        status = call(self._ref, ctypes.byref(_rows(k)), ctypes.byref(_rows(v)), _dtype(k), at, on)
         if status:
             raise AbqError(status, name)
 
@@ -138,18 +169,22 @@ class KvCache:
         """(k, v) [tokens, kv heads, head dim] of the tokens at these slots, in fp16 (or dtype), or into out = (k, v)."""
         if out is None:
             shape = (slots.numel(),) + self._row
-            out = tuple(torch.empty(shape, dtype=dtype or torch.float16, device=slots.device) for _ in range(2))
+            with torch.cuda.stream(None if stream is None else _stream_of(stream)):  # (tensors of the stream that they are written on)
+                out = tuple(torch.empty(shape, dtype=dtype or torch.float16, device=slots.device) for _ in range(2))
         self._call(self._read, "abq_kv_read", out[0], out[1], slots, stream)
         return out
 
 
 class _Attention:
-    def _finish(self, out, workspace):
+    def _finish(self, out, workspace, *made):
         self.out = out
         need = self.workspace_bytes
         if workspace is None and need:
             workspace = torch.empty(need, dtype=torch.uint8, device=out.device)
+            made += (workspace,)
         self.workspace = workspace
+        self._memory = _Memory(made)
+        self._known = self._memory.known
         if workspace is not None and workspace.numel():
             _check(lib().abq_attn_set_workspace(ctypes.byref(self.state), workspace.data_ptr(), workspace.numel() * workspace.element_size()),
                    "abq_attn_set_workspace")
@@ -160,8 +195,11 @@ class _Attention:
         return lib().abq_attn_workspace_bytes(ctypes.byref(self.state))
 
     def run(self, stream=None):
-        """One pass over what the tensors hold now; returns out."""
-        status = self._exec(self._state, abq_gemm._stream_ptr(stream))
+        """One pass over what the tensors hold now; returns out.  A graph that captures it needs the object for as long as it is replayed."""
+        on = abq_gemm._stream_ptr(stream)
+        if on.value not in self._known:
+            self._memory.use(stream)
+        status = self._exec(self._state, on)
         if status:
             raise AbqError(status, "abq_attn_exec")
         return self.out
@@ -176,8 +214,10 @@ class PromptAttention(_Attention):
     def __init__(self, q, k, v, q_starts, k_starts=None, max_q=None, max_k=None, scale=None, out=None, workspace=None):
         if k.shape != v.shape or k.shape[2] != q.shape[2] or not (q.dtype == k.dtype == v.dtype):
             raise ValueError("q [tokens, heads, head dim], k and v [tokens, kv heads, head dim] of one type are wanted")
+        made = ()
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            made = (out,)
         if out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError("out has to be of q's shape and type")
         seqs = q_starts.numel() - 1
@@ -188,7 +228,7 @@ class PromptAttention(_Attention):
         self.state = AttnState()
         _check(lib().abq_attn_prompt_init(*[ctypes.byref(r) for r in rows], _dtype(q), q.shape[1], k.shape[1], q.shape[2], at[0], at[1],
                                           seqs, max_q, max_k, q.shape[2] ** -0.5 if scale is None else scale, ctypes.byref(self.state)), "abq_attn_prompt_init")
-        self._finish(out, workspace)
+        self._finish(out, workspace, *made)
 
 
 class TreeAttention(_Attention):
@@ -201,8 +241,10 @@ class TreeAttention(_Attention):
         d = cache.desc
         if q.dim() != 3 or q.shape[2] != d.head_dim:
             raise ValueError("q [drafts, heads, %d] is wanted" % d.head_dim)
+        made = ()
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            made = (out,)
         if out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError("out has to be of q's shape and type")
         seqs = context.numel()
@@ -214,4 +256,4 @@ class TreeAttention(_Attention):
                                         _index(context, torch.int32, seqs, "context"), _index(q_starts, torch.int32, seqs + 1, "q_starts"),
                                         None if mask is None else _index(mask, torch.int64, q.shape[0], "mask"), seqs, max_q, max_context,
                                         q.shape[2] ** -0.5 if scale is None else scale, ctypes.byref(self.state)), "abq_attn_tree_init")
-        self._finish(out, workspace)
+        self._finish(out, workspace, *made, *cache._memory.tensors)

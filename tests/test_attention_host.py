@@ -209,3 +209,109 @@ def test_a_bound_of_the_keys_as_large_as_its_type_splits_them_as_any_large_one(a
     large = [dict(base, max_k=m) for m in (1 << 30, 2 ** 31 - 64, 2 ** 31 - 63, 2 ** 31 - 1)]
     made = launches(tmp_path, large)
     assert all(r["status"] == [0, 0, 0] and r == made[0] and r["parts"] == 64 for r in made), made
+
+
+class StreamsOfHand:
+    """torch.cuda's streams, written down instead of made: what the binding asks of them, in order"""
+
+    class Stream:
+        def __init__(self, streams, at):
+            self.cuda_stream, self.streams = at, streams
+
+        def wait_stream(self, other):
+            self.streams.log.append(("wait", self.cuda_stream, other.cuda_stream))
+
+    def __init__(self, torch, monkeypatch):
+        self.log, self.captured, self.current = [], False, None
+        self.current = self.home = self.Stream(self, 0x10)
+
+        class Inside:
+            def __init__(self, stream):
+                self.stream = stream
+
+            def __enter__(inside):
+                inside.before, self.current = self.current, inside.stream or self.current
+
+            def __exit__(inside, *_):
+                self.current = inside.before
+
+        empty = torch.empty
+
+        def make(*shape, **kw):
+            t = empty(*shape, **kw)
+            self.log.append(("made", self.current.cuda_stream))
+            return t
+        monkeypatch.setattr(torch, "empty", make)
+        monkeypatch.setattr(torch.cuda, "current_stream", lambda *_: self.current)
+        monkeypatch.setattr(torch.cuda, "ExternalStream", lambda at, *_: self.Stream(self, at))
+        monkeypatch.setattr(torch.cuda, "stream", Inside)
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: self.captured)
+        monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: self.log.append(("keep", t.data_ptr(), s.cuda_stream)))
+
+    def taken(self):
+        log, self.log = self.log, []
+        return log
+
+
+def test_memory_that_the_binding_makes_is_safe_on_other_streams(attn, monkeypatch):
+    """The workspace and the result belong to the stream that was current: another one waits for it once before the first launch, and
+    keeps the memory from being handed out"""
+    torch = attn.torch
+
+    class Fake(torch.Tensor):  # a CPU tensor that says it is on the device: no launch is made
+        is_cuda = True
+    on_device = lambda t: t.as_subclass(Fake)  # noqa: E731
+    streams = StreamsOfHand(torch, monkeypatch)
+    monkeypatch.setattr(attn, "_rows", lambda t: attn.Rows(t.data_ptr(), t.shape[0], t.stride(0), t.stride(1)))
+    q, k = on_device(torch.zeros(40, 2, 128).half()), on_device(torch.zeros(1500, 2, 128).half())
+    starts = [on_device(torch.tensor([0, n], dtype=torch.int32)) for n in (40, 1500)]
+    call = attn.PromptAttention(q, k, k, *starts, 40, 1500)
+    assert call.state.parts > 1 and streams.taken() == [("made", 0x10)] * 2
+    call._exec = lambda state, on: streams.log.append(("run", on.value)) or 0
+    memory = {call.workspace.data_ptr(), call.out.data_ptr()}
+    other = streams.Stream(streams, 0x20)
+
+    def kept(log, at):
+        assert {e[1] for e in log if e[0] == "keep"} == memory and all(e[2] == at for e in log if e[0] == "keep"), log
+        return [e for e in log if e[0] != "keep"]
+
+    call.run(stream=streams.home)
+    assert streams.taken() == [("run", 0x10)]
+    call.run(stream=other)
+    assert kept(streams.taken(), 0x20) == [("wait", 0x20, 0x10), ("run", 0x20)]
+    call.run(stream=other)
+    call.run(stream=0x20)
+    assert streams.taken() == [("run", 0x20)] * 2
+    streams.captured = True  # a capture does not wait for what is outside of it
+    call.run(stream=0x30)
+    assert kept(streams.taken(), 0x30) == [("run", 0x30)]
+    streams.captured = False
+    call.run(stream=0x30)
+    assert kept(streams.taken(), 0x30) == [("wait", 0x30, 0x10), ("run", 0x30)]
+
+    # what the caller brings is the caller's
+    mine = attn.PromptAttention(q, k, k, *starts, 40, 1500, out=on_device(torch.zeros(40, 2, 128).half()), workspace=torch.zeros(call.workspace.numel(), dtype=torch.uint8))
+    mine._exec = call._exec
+    streams.taken()
+    mine.run(stream=other)
+    assert streams.taken() == [("run", 0x20)]
+
+    # the cache's arrays, and rows that are read back
+    cache = attn.KvCache(4, 64, 2, 128, device="cpu")
+    cache._append = cache._read = lambda *a: streams.log.append(("run", a[-1].value)) or 0
+    memory = {t.data_ptr() for t in (cache.k_codes, cache.v_codes, cache.k_scales, cache.v_scales)}
+    slots = on_device(torch.zeros(40, dtype=torch.int32))
+    streams.taken()
+    cache.append(q, q, slots, stream=other)
+    assert kept(streams.taken(), 0x20) == [("wait", 0x20, 0x10), ("run", 0x20)]
+    cache.read(slots, stream=other)
+    assert streams.taken() == [("made", 0x20)] * 2 + [("run", 0x20)]
+    cache.read(slots, stream=streams.home)
+    assert streams.taken() == [("made", 0x10)] * 2 + [("run", 0x10)]
+    table, context = on_device(torch.zeros(1, 4, dtype=torch.int32)), on_device(torch.zeros(1, dtype=torch.int32))
+    tree = attn.TreeAttention(q[:1], cache, table, context, starts[0], 1, 200)
+    tree._exec = call._exec
+    memory |= {tree.out.data_ptr()}
+    streams.taken()
+    tree.run(stream=other)
+    assert kept(streams.taken(), 0x20) == [("wait", 0x20, 0x10), ("run", 0x20)]
