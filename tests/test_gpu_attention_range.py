@@ -4,7 +4,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from attention_reference import cache_contents, check, load_abq_attention  # noqa: E402
+from attention_reference import attend, cache_contents, check, load_abq_attention  # noqa: E402
 from test_gpu_attention import prompt_reference, starts  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -138,3 +138,36 @@ def test_bf16_queries_near_the_types_end_on_the_cache(attn, symmetric, size):
     got = attn.TreeAttention(q.cuda(), cache, table, torch.tensor([tokens - 1], dtype=torch.int32).cuda(), starts([1]), 1, tokens - 1).run()
     want = held[at].expand(1, 2, dim)
     check(got.cpu(), want, want.abs() * 2.0 ** -8 * 1.1 + held.abs().max() * 2.0 ** -18, size)
+
+
+@pytest.mark.parametrize("bits,symmetric", [(8, True), (8, False), (4, True), (4, False)])
+@pytest.mark.parametrize("heads", [3, 20])
+def test_value_scales_far_apart_in_one_sequence(attn, bits, symmetric, heads):
+    """A token's values lie anywhere between 1e-4 and 300, some are 0, and for one query a token of small values takes nearly all.  Weights
+    times value scales are held to 11 bits or to 2^-35 of the largest, whichever is more."""
+    gen = torch.Generator().manual_seed(26)
+    dim, tokens = 128, 700
+    level = torch.exp(torch.rand(tokens, 1, 1, generator=gen) * 14.9 - 9.2)
+    v = (torch.randn(tokens, 1, dim, generator=gen) * level).half()
+    v[::13] = 0
+    k = torch.randn(tokens, 1, dim, generator=gen).half()
+    small = int(level[1:].flatten().argmin()) + 1
+    v[small] = (torch.randn(1, dim, generator=gen) * 1e-3).half()
+    q = torch.randn(1, heads, dim, generator=gen).half()
+    q[0, 0] = k[small, 0] * 1.5  # (about 17 ahead of the others' scores)
+    cache, table, held = tree_of(attn, v, k, bits, symmetric, torch.float16)
+    got = attn.TreeAttention(q.cuda(), cache, table, torch.tensor([tokens - 1], dtype=torch.int32).cuda(), starts([1]), 1, tokens - 1).run().cpu()
+    kc, vc, (ks, kz), (vs, vz) = cache_contents(cache)
+    half = 2 ** (bits - 1)
+    codes = lambda c, z: torch.from_numpy(abs(c[:tokens, 0] - half) * 1.0 + abs(z[:tokens, 0, None] - half) * 1.0)  # noqa: E731
+    keys = torch.from_numpy((kc[:tokens, 0] - kz[:tokens, 0, None]) * ks[:tokens, 0, None].astype("float64"))
+    scale, seen = dim ** -0.5, torch.ones(1, tokens, dtype=torch.bool)
+    step = torch.from_numpy(vs[:tokens, 0].astype("float64"))
+    spread = codes(vc, vz) * 2.0 ** -8 * step[:, None] + held.abs()
+    for h in range(heads):
+        out, allowed = attend(q[0, h][None], keys, held, seen, scale, torch.float16, spread, 0.0)
+        p = torch.softmax(q[0, h].double() @ keys.T * scale, 0)
+        more = q[0, h].double().abs() @ (codes(kc, kz) * torch.from_numpy(ks[:tokens, 0, None].astype("float64"))).T * scale
+        allowed = allowed + 2.0 ** -35 * (p * step).max() * codes(vc, vz).sum(0) + float(more.max()) * (dim + 8) * 2.0 ** -23 * (p @ spread)
+        check(got[0, h][None], out, allowed, h)
+        assert (allowed < out.abs().max() * 0.05).all()  # (the bound says something)
