@@ -134,7 +134,8 @@ class _Memory:
 class KvCache:
     """A paged cache of keys and values in codes of 8 or 4 bits with a scale (and a zero point) per token and head.
 
-    A token's place is its slot, page * page_size + offset."""
+    A token's place is its slot, page * page_size + offset.  With zero points (symmetric=False) a row that lies more than 39 of its spreads
+    from zero (8 bits; 667 with 4) is not held as what it is: zero points end at 1e4, scales begin at 1e-5."""
 
     def __init__(self, num_pages, page_size, kv_heads, head_dim, bits=8, symmetric=True, device="cuda"):
         d = KvCacheDesc(bits, int(bool(symmetric)), kv_heads, head_dim, page_size, num_pages)
@@ -208,8 +209,8 @@ class _Attention:
 class PromptAttention(_Attention):
     """Causal attention of packed prompts: q [tokens, heads, head dim], k and v [tokens, kv heads, head dim], sequence s in rows
     starts[s] .. starts[s + 1] - 1 (int32 on the device).  With k_starts, the queries are the last tokens of each sequence's keys.
-    max_q, max_k: bounds of a sequence's queries and keys.  workspace: a device tensor of at least workspace_bytes; by default one
-    is made, an empty tensor means none."""
+    max_q, max_k: bounds of a sequence's queries (those beyond are not computed) and keys.  workspace: a device tensor of at least
+    workspace_bytes; by default one is made, an empty tensor means none."""
 
     def __init__(self, q, k, v, q_starts, k_starts=None, max_q=None, max_k=None, scale=None, out=None, workspace=None):
         if k.shape != v.shape or k.shape[2] != q.shape[2] or not (q.dtype == k.dtype == v.dtype):
@@ -235,7 +236,7 @@ class TreeAttention(_Attention):
     """Attention of drafted tokens (ordinary decoding: one per sequence) over a KvCache: q [drafts, heads, head dim], sequence s in rows
     q_starts[s] .. q_starts[s + 1] - 1; page_table int32 [sequences, pages], context int32 [sequences]: tokens in front of the
     drafts, which stand behind them in the cache.  mask: int64 [drafts], bit j: sees draft j of its sequence; without one a draft sees
-    those before it and itself.  max_q, max_context: bounds of a sequence's drafts (at most 64) and context."""
+    those before it and itself.  max_q, max_context: bounds of a sequence's drafts (at most 64; those beyond are seen, not computed) and context."""
 
     def __init__(self, q, cache, page_table, context, q_starts, max_q, max_context, mask=None, scale=None, out=None, workspace=None):
         d = cache.desc

@@ -12,10 +12,10 @@
 // (32 rows of one column of pieces lie in different banks), values by the row modulo 4 (so do four rows of four pieces).
 //
 // P is rounded to the type of the inputs for the second product, which wants both of its operands of one type; its sum is taken
-// in fp32 before that.
+// in fp32 before that (a sum of the rounded weights takes 1 % longer).
 //
 // Long prompts are bound by the matrix cores, at the clock that the power left to the chip allows: 16384 tokens, 32 heads of 128
-// on 8 key heads, bf16, 2.2 TFLOP of what queries see, take 1.92 - 2.09 ms (1.05 - 1.15 PFLOP/s; a large matrix product reaches
+// on 8 key heads, bf16, 2.2 TFLOP of what queries see, take 1.97 - 2.02 ms (1.09 - 1.12 PFLOP/s; a large matrix product reaches
 // 1.38) with the matrix cores busy in 67 % of clocks, of which there are 1.6 - 1.9 GHz.  Short ones are bound by the chain of
 // steps: a tile's 64 tokens take 0.6 us whatever the grid, so 1024 tokens of 32 heads, 16 tiles, 18 - 20 us.
 #include "abq_attn.h"
@@ -106,7 +106,7 @@ template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void at
     // Weights are 2^(score - base + lift): base follows the running maximum only when that has left it 2^kSlack behind, which
     // spares nearly every rescaling.  In fp16 the lift leaves weights their normal range down to 2^-20 of the largest one.  bf16 has
     // the exponents of the sums, and its values may stand at their end: there the lift keeps the sum of all weights below 1/2, so
-    // that a sum of weights times values stays below the largest of the values.  (At the other end, values below 2^-100 lose digits.)
+    // that a sum of weights times values stays below the largest of the values.  (At the other end, values below 2^-90 lose digits.)
     constexpr float kSlack = 8;
     const float lift = DTYPE == ABQ_BF16 ? -kSlack - 1 - (float)(32 - __builtin_clz((unsigned)ks.count | 1)) : 6.f;
     const float slack = fminf(kSlack / a.scale_log2, 3e38f); // (finite, so that any score is more than that above none)

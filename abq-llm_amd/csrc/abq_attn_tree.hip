@@ -8,8 +8,9 @@
 // so codes enter the matrix cores as the whole numbers they are, exact in fp16, and are never scaled one by one: a code costs
 // one half of a byte permute (or mask) and one half of a packed add.  Folding s_v into the exponent keeps the largest weight at
 // 1 whatever the scales are, so that weights rounded to fp16 (11 bits; the one rounding of the sum, as large as that of the
-// result) do not run into its subnormals.  Queries in bf16 become fp16 after a division of each row by a power of two, which
-// loses nothing that a 32-bit sum would keep.
+// result) do not run into its subnormals.  Queries in bf16 become fp16 after a division of each row by a power of two: elements
+// down to 2^-31 of the row's largest keep all their bits, those below 2^-39 of it become 0, which a 32-bit sum beside the largest
+// one's term would lose as well.  Sums of weights are taken before they are rounded, those of weights times zero points behind it.
 //
 // Both products are taken transposed, scores^T = K q^T and out^T = V^T w^T (16 x 16 x 32 MFMA), because the result of the
 // first then lies in the registers as the second wants it: lane (r, g) gets the scores of row r for tokens 4 g .. 4 g + 3, and
@@ -24,7 +25,7 @@
 // 4.8 TB/s of the 5.1 that a copy reaches; four waves per SIMD cover each other's loads, so none keeps a second buffer.  With more
 // rows a step's vector work (400 operations beside 32 MFMA: codes to fp16, factors, exponentials) and the loads share the time:
 // two waves per SIMD, each with a step under way while it works at another.  20 rows on 48 ragged contexts, 630 MB: 148 us,
-// 4.3 TB/s; 108 rows on 3 x 5500 tokens of 4 bits, 25 us, bound by that work and, at 9 steps a wave, by its start and end.
+// 4.3 TB/s; 108 rows on 3 x 5500 tokens of 4 bits, 28 us, bound by that work and, at 9 steps a wave, by its start and end.
 #include "abq_attn.h"
 
 namespace abq {
