@@ -29,11 +29,12 @@ int64_t product(int64_t a, int64_t b, int64_t c)
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
-abq_status check_rows(const abq_rows *r, int64_t rows, int heads, int head_dim)
+// written: rows of a result, which may not lie on one another
+abq_status check_rows(const abq_rows *r, int64_t rows, int heads, int head_dim, bool written = false)
 {
     if (!r || r->rows != rows || (rows && !r->data) || !aligned16(r->data) || r->row_stride % 8 || r->head_stride % 8)
         return ABQ_ERR_INVALID_ARG;
-    if (r->row_stride < 0 || r->head_stride < 0 || (heads > 1 && r->head_stride < head_dim))
+    if (r->row_stride < 0 || r->head_stride < 0 || (heads > 1 && r->head_stride < head_dim) || (written && rows > 1 && r->row_stride < head_dim))
         return ABQ_ERR_INVALID_ARG;
     return ABQ_OK;
 }
@@ -57,14 +58,15 @@ abq_status check_cache(const abq_kv_cache *c)
     return ABQ_OK;
 }
 
-abq_status check_cache_call(const abq_kv_cache *c, const abq_rows *k, const abq_rows *v, int dtype, const int32_t *slots)
+abq_status check_cache_call(const abq_kv_cache *c, const abq_rows *k, const abq_rows *v, int dtype, const int32_t *slots, bool written)
 {
     abq_status s = check_cache(c);
     if (s != ABQ_OK)
         return s;
     if (!k || !v || (dtype != ABQ_F16 && dtype != ABQ_BF16) || k->rows < 0 || (k->rows && !slots))
         return ABQ_ERR_INVALID_ARG;
-    if ((s = check_rows(k, k->rows, c->kv_heads, c->head_dim)) != ABQ_OK || (s = check_rows(v, k->rows, c->kv_heads, c->head_dim)) != ABQ_OK)
+    if ((s = check_rows(k, k->rows, c->kv_heads, c->head_dim, written)) != ABQ_OK ||
+        (s = check_rows(v, k->rows, c->kv_heads, c->head_dim, written)) != ABQ_OK)
         return s;
     if (k->rows > 0x7ffffff0 || (k->rows + 3) / 4 * 2 * c->kv_heads > 4 * kMostBlocks - 4)
         return ABQ_ERR_TOO_LARGE;
@@ -83,7 +85,7 @@ abq_status init_common(int kind, const abq_rows *q, const abq_rows *out, int dty
     if (heads % kv_heads)
         return ABQ_ERR_INVALID_ARG;
     abq_status s;
-    if ((s = check_rows(q, q->rows, heads, head_dim)) != ABQ_OK || (s = check_rows(out, q->rows, heads, head_dim)) != ABQ_OK)
+    if ((s = check_rows(q, q->rows, heads, head_dim)) != ABQ_OK || (s = check_rows(out, q->rows, heads, head_dim, true)) != ABQ_OK)
         return s;
     if (q->rows > 0x7ffffff0 || product(q->rows, heads, 1) > 1ll << 42) // (so that bytes of a workspace fit 64 bits)
         return ABQ_ERR_TOO_LARGE;
@@ -131,13 +133,13 @@ size_t abq_kv_scales_bytes(const abq_kv_cache *c)
 
 abq_status abq_kv_append(const abq_kv_cache *c, const abq_rows *k, const abq_rows *v, int dtype, const int32_t *slots, void *stream)
 {
-    const abq_status s = check_cache_call(c, k, v, dtype, slots);
+    const abq_status s = check_cache_call(c, k, v, dtype, slots, false);
     return s != ABQ_OK ? s : hip_status(launch_kv_append(*c, *k, *v, dtype, slots, (hipStream_t)stream));
 }
 
 abq_status abq_kv_read(const abq_kv_cache *c, const abq_rows *k, const abq_rows *v, int dtype, const int32_t *slots, void *stream)
 {
-    const abq_status s = check_cache_call(c, k, v, dtype, slots);
+    const abq_status s = check_cache_call(c, k, v, dtype, slots, true);
     return s != ABQ_OK ? s : hip_status(launch_kv_read(*c, *k, *v, dtype, slots, (hipStream_t)stream));
 }
 

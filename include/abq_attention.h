@@ -25,7 +25,9 @@ typedef enum abq_dtype {
 
 /* A device matrix of rows (tokens) of heads: element d of head h of row r stands at data[r * row_stride + h * head_stride
  * + d], strides in elements.  Rows of heads are read and written 16 bytes at a time: data must be 16-byte aligned and both
- * strides multiples of 8 (a slice of a fused QKV result is one).  Nothing outside rows 0 .. rows - 1 is touched. */
+ * strides multiples of 8 (a slice of a fused QKV result is one), head_stride at least head_dim where there are several heads, and
+ * in results row_stride as well where there are several rows (rows that are read may repeat).  Nothing outside rows
+ * 0 .. rows - 1 is touched. */
 typedef struct abq_rows {
     void *data;
     int64_t rows;

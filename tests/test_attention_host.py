@@ -315,3 +315,19 @@ def test_memory_that_the_binding_makes_is_safe_on_other_streams(attn, monkeypatc
     streams.taken()
     tree.run(stream=other)
     assert kept(streams.taken(), 0x20) == [("wait", 0x20, 0x10), ("run", 0x20)]
+
+
+def test_results_whose_rows_lie_on_one_another_are_refused(attn):
+    """Rows that are read may repeat (a stride of 0); rows that are written would race"""
+    L, ok = attn.lib(), attn.abq_gemm
+    for stride in (0, 8, 120):
+        flat = {"row_stride": stride}
+        assert prompt(attn, q=flat, k=flat, v=flat)[0] == ok.ABQ_OK and tree(attn, q=flat)[0] == ok.ABQ_OK, stride
+        assert prompt(attn, out=flat)[0] == ok.ABQ_ERR_INVALID_ARG and tree(attn, out=flat)[0] == ok.ABQ_ERR_INVALID_ARG, stride
+        for k, v in ((flat, {}), ({}, flat)):
+            args = [ctypes.byref(cache_desc(attn)), ctypes.byref(rows(attn, **k)), ctypes.byref(rows(attn, **v)), 0, 5 * A, None]
+            assert L.abq_kv_read(*args) == ok.ABQ_ERR_INVALID_ARG, stride
+        # heads outermost, and a single row whose stride says nothing
+        assert prompt(attn, out={"row_stride": 128, "head_stride": 12 * 128})[0] == ok.ABQ_OK
+        one = {"rows": 1, "row_stride": stride}
+        assert prompt(attn, q=one, k=one, v=one, out=one)[0] == ok.ABQ_OK, stride
