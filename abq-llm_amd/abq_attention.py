@@ -138,6 +138,8 @@ class KvCache:
     from zero (8 bits; 667 with 4) is not held as what it is: zero points end at 1e4, scales begin at 1e-5."""
 
     def __init__(self, num_pages, page_size, kv_heads, head_dim, bits=8, symmetric=True, device="cuda"):
+        if torch.device(device).type != "cuda":
+            raise ValueError("the cache has to be on the device, not on %s" % device)
         d = KvCacheDesc(bits, int(bool(symmetric)), kv_heads, head_dim, page_size, num_pages)
         codes, scales = lib().abq_kv_codes_bytes(ctypes.byref(d)), lib().abq_kv_scales_bytes(ctypes.byref(d))
         if not codes:
@@ -180,6 +182,8 @@ class _Attention:
     def _finish(self, out, workspace, *made):
         self.out = out
         need = self.workspace_bytes
+        if workspace is not None and workspace.numel() and not (workspace.is_cuda and workspace.is_contiguous()):
+            raise ValueError("a contiguous device tensor is wanted as the workspace")
         if workspace is None and need:
             workspace = torch.empty(need, dtype=torch.uint8, device=out.device)
             made += (workspace,)

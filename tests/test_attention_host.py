@@ -290,14 +290,17 @@ def test_memory_that_the_binding_makes_is_safe_on_other_streams(attn, monkeypatc
     assert kept(streams.taken(), 0x30) == [("wait", 0x30, 0x10), ("run", 0x30)]
 
     # what the caller brings is the caller's
-    mine = attn.PromptAttention(q, k, k, *starts, 40, 1500, out=on_device(torch.zeros(40, 2, 128).half()), workspace=torch.zeros(call.workspace.numel(), dtype=torch.uint8))
+    mine = attn.PromptAttention(q, k, k, *starts, 40, 1500, out=on_device(torch.zeros(40, 2, 128).half()),
+                                workspace=on_device(torch.zeros(call.workspace.numel(), dtype=torch.uint8)))
     mine._exec = call._exec
     streams.taken()
     mine.run(stream=other)
     assert streams.taken() == [("run", 0x20)]
 
     # the cache's arrays, and rows that are read back
-    cache = attn.KvCache(4, 64, 2, 128, device="cpu")
+    for name in ("zeros", "ones"):
+        monkeypatch.setattr(torch, name, lambda *a, make=getattr(torch, name), device=None, **kw: make(*a, **kw))
+    cache = attn.KvCache(4, 64, 2, 128)
     cache._append = cache._read = lambda *a: streams.log.append(("run", a[-1].value)) or 0
     memory = {t.data_ptr() for t in (cache.k_codes, cache.v_codes, cache.k_scales, cache.v_scales)}
     slots = on_device(torch.zeros(40, dtype=torch.int32))
@@ -331,3 +334,19 @@ def test_results_whose_rows_lie_on_one_another_are_refused(attn):
         assert prompt(attn, out={"row_stride": 128, "head_stride": 12 * 128})[0] == ok.ABQ_OK
         one = {"rows": 1, "row_stride": stride}
         assert prompt(attn, q=one, k=one, v=one, out=one)[0] == ok.ABQ_OK, stride
+
+
+def test_memory_of_the_host_is_refused(attn):
+    """The binding hands out addresses that the kernels read and write: what is not on the device, or not in one piece, never gets there"""
+    torch = attn.torch
+
+    class Fake(torch.Tensor):  # a CPU tensor that says it is on the device: no launch is made
+        is_cuda = True
+    on_device = lambda t: t.as_subclass(Fake)  # noqa: E731
+    with pytest.raises(ValueError):
+        attn.KvCache(4, 64, 2, 128, device="cpu")
+    q, k = on_device(torch.zeros(40, 2, 128).half()), on_device(torch.zeros(1500, 2, 128).half())
+    starts = [on_device(torch.tensor([0, n], dtype=torch.int32)) for n in (40, 1500)]
+    for workspace in (torch.zeros(1 << 20, dtype=torch.uint8), on_device(torch.zeros(1 << 14, 64, dtype=torch.uint8))[:, :32]):
+        with pytest.raises(ValueError):
+            attn.PromptAttention(q, k, k, *starts, 40, 1500, out=torch.empty_like(q), workspace=workspace)
