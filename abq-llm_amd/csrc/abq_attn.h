@@ -65,6 +65,15 @@ template <int DTYPE> __device__ __forceinline__ uint32_t pack16(float a, float b
         return __builtin_bit_cast(uint32_t, half2v{(_Float16)a, (_Float16)b});
 }
 
+// A result that is finite, but beyond the type's largest, becomes that one: weights that were rounded on one side of a quotient alone
+// take a mean of values at the end of the type past it
+template <int DTYPE> __device__ __forceinline__ float largest16() { return DTYPE == ABQ_BF16 ? 0x1.fep127f : 65504.f; }
+template <int DTYPE> __device__ __forceinline__ float saturated16(float x)
+{
+    return fabsf(x) < INFINITY ? __builtin_amdgcn_fmed3f(x, -largest16<DTYPE>(), largest16<DTYPE>()) : x;
+}
+template <int DTYPE> __device__ __forceinline__ uint32_t pack16_saturated(float a, float b) { return pack16<DTYPE>(saturated16<DTYPE>(a), saturated16<DTYPE>(b)); }
+
 // Reductions over lanes l, l ^ 16, l ^ 32, l ^ 48 (over l, l ^ 32 alone: across_halves), the result in all of them.  A swap of a
 // register with its own copy leaves one half's (or row's) values in the one and the other's in the other.
 struct TwoWords {

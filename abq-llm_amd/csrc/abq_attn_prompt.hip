@@ -501,7 +501,27 @@ template <int DTYPE, int D, int KG> __global__ __launch_bounds__(256, 2) void at
         }
         return;
     }
-    const float f = total > 0 ? 1.f / total : total; // (a sum that is not a number stays one)
+    float f = total > 0 ? 1.f / total : total; // (a sum that is not a number stays one)
+    // (a finite result becomes the type's largest at most: saturated16; fp16 has a bit of the wave's mode for it, which lets infinities be)
+    if constexpr (DTYPE == ABQ_F16) {
+        __builtin_amdgcn_s_setreg(1 | 23 << 6, 1); // MODE.FP16_OVFL
+        asm volatile("" : "+v"(f));                // (the conversions come behind it)
+    } else {
+        float far = 0;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                far = fmaxf(far, fabsf(out[d][j]));
+        if (__any(far * f > largest16<DTYPE>())) {
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    out[d][j] = saturated16<DTYPE>(out[d][j] * f);
+            f = 1.f;
+        }
+    }
     uint16_t *to = (uint16_t *)a.out.data + (int64_t)(qs.first + i) * a.out.row_stride + (int64_t)head * a.out.head_stride;
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)

@@ -505,7 +505,8 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(64 * 
             uint32_t x[kEach / 2];
 #pragma unroll
             for (int e = 0; e < kEach / 2; ++e)
-                x[e] = a.dtype == ABQ_BF16 ? pack16<ABQ_BF16>(acc[2 * e] * f, acc[2 * e + 1] * f) : pack16<ABQ_F16>(acc[2 * e] * f, acc[2 * e + 1] * f);
+                x[e] = a.dtype == ABQ_BF16 ? pack16_saturated<ABQ_BF16>(acc[2 * e] * f, acc[2 * e + 1] * f)
+                                           : pack16_saturated<ABQ_F16>(acc[2 * e] * f, acc[2 * e + 1] * f);
             if constexpr (kEach == 8)
                 *(uint4 *)to = uint4{x[0], x[1], x[2], x[3]};
             else
@@ -560,8 +561,8 @@ template <int D> __global__ __launch_bounds__(256) void attn_join_kernel(JoinArg
     const float f = total > 0 ? 1.f / total : total;
     uint16_t *to = (uint16_t *)a.out.data + row * a.out.row_stride + (int64_t)head * a.out.head_stride + e0;
     if (lane < kLanes)
-        *(uint2 *)to = a.dtype == ABQ_BF16 ? uint2{pack16<ABQ_BF16>(acc[0] * f, acc[1] * f), pack16<ABQ_BF16>(acc[2] * f, acc[3] * f)}
-                                           : uint2{pack16<ABQ_F16>(acc[0] * f, acc[1] * f), pack16<ABQ_F16>(acc[2] * f, acc[3] * f)};
+        *(uint2 *)to = a.dtype == ABQ_BF16 ? uint2{pack16_saturated<ABQ_BF16>(acc[0] * f, acc[1] * f), pack16_saturated<ABQ_BF16>(acc[2] * f, acc[3] * f)}
+                                           : uint2{pack16_saturated<ABQ_F16>(acc[0] * f, acc[1] * f), pack16_saturated<ABQ_F16>(acc[2] * f, acc[3] * f)};
 }
 
 } // namespace

@@ -84,7 +84,7 @@ abq_status abq_kv_read(const abq_kv_cache *cache, const abq_rows *k, const abq_r
  *
  * out[i][h] = sum_t p[t] v[t][h / group] over the tokens t that query i sees, p = softmax(scale * q[i][h] . k[t][h / group]),
  * group = heads / kv_heads.  Scores, statistics and sums are fp32; a query that sees nothing gets zeros; what a query does
- * not see never reaches its result, infinities and NaN included.
+ * not see never reaches its result, infinities and NaN included.  A finite result beyond dtype's largest becomes that one.
  *
  * As with a GEMM, a caller-owned state is filled once (init) and run any number of times (exec).
  * ------------------------------------------------------------------------------------- */

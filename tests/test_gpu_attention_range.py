@@ -171,3 +171,59 @@ def test_value_scales_far_apart_in_one_sequence(attn, bits, symmetric, heads):
         allowed = allowed + 2.0 ** -35 * (p * step).max() * codes(vc, vz).sum(0) + float(more.max()) * (dim + 8) * 2.0 ** -23 * (p @ spread)
         check(got[0, h][None], out, allowed, h)
         assert (allowed < out.abs().max() * 0.05).all()  # (the bound says something)
+
+
+def held_mean(got, value, u, tokens, what):
+    """Every token holds the value: so does every result, but for weights rounded on one side of the quotient (u), the sums' fp32 and
+    one rounding"""
+    assert torch.isfinite(got).all(), ("not finite", what)
+    assert ((got.double() - value).abs() <= abs(value) * (2.02 * u + tokens * 2.0 ** -23)).all(), what
+
+
+@pytest.mark.parametrize("dtype,u", [(torch.float16, 2.0 ** -11), (torch.bfloat16, 2.0 ** -8)])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,lens,k_lens,split", [(4, [200, 64], [200, 64], False), (256, [200], [200], False), (4, [200], [1500], True)])
+def test_means_of_the_types_largest_value_in_prompts(attn, dtype, u, dim, heads, lens, k_lens, split):
+    gen = torch.Generator().manual_seed(27)
+    largest = torch.finfo(dtype).max
+    for spread in (1, 3, 5):  # (a few tokens of about the same weight, many, and one)
+        q = (spread * torch.randn(sum(lens), heads, dim, generator=gen)).to(dtype).cuda()
+        k = torch.randn(sum(k_lens), 2, dim, generator=gen).to(dtype).cuda()
+        v = torch.full((sum(k_lens), 2, dim), largest, dtype=dtype)
+        v[:, :, 1::2] *= -1
+        v[:, :, 2::4] = 1
+        call = attn.PromptAttention(q, k, v.cuda(), starts(lens), starts(k_lens), max(lens), max(k_lens))
+        assert (call.state.parts > 1) == split
+        got = call.run().cpu()
+        for at, value in ((slice(0, None, 4), largest), (slice(1, None, 2), -largest), (slice(2, None, 4), 1.0)):
+            held_mean(got[:, :, at], value, u, max(k_lens), (spread, value))
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("context,group,drafts,split", [(30, 8, 64, False), (6000, 8, 64, False), (6000, 8, 64, True), (6000, 16, 1, False)])
+def test_means_of_the_types_largest_value_in_drafts(attn, bits, symmetric, context, group, drafts, split):
+    gen = torch.Generator().manual_seed(28)
+    dim, seqs = 128, 2 if drafts > 1 else 40
+    size = (context + drafts + 63) // 64
+    cache = attn.KvCache(seqs * size, 64, 1, dim, bits=bits, symmetric=symmetric)
+    tokens = seqs * size * 64
+    k = torch.randn(tokens, 1, dim, generator=gen).half().cuda()
+    v = torch.full((tokens, 1, dim), 65504.0).half()
+    if symmetric:
+        v[:, :, 1::2] *= -1
+    else:
+        v[:, :, 1::2] = 0  # (a zero point of 0: with one of its own the smallest code would stand for less than the type holds)
+    cache.append(k, v.cuda(), torch.arange(tokens, dtype=torch.int32).cuda())
+    table = torch.arange(seqs * size, dtype=torch.int32).cuda().view(seqs, size)
+    for spread in (1, 4, 6, 8):
+        q = (spread * torch.randn(seqs * drafts, group, dim, generator=gen)).half().cuda()
+        call = attn.TreeAttention(q, cache, table, torch.full((seqs,), context, dtype=torch.int32).cuda(), starts([drafts] * seqs), drafts, context,
+                                  workspace=None if split else torch.empty(0, device="cuda"))
+        assert (call.state.parts > 1) == split
+        got = call.run().cpu()
+        held_mean(got[:, :, 0::2], 65504.0, 2.0 ** -11, context + drafts, spread)
+        if symmetric:
+            held_mean(got[:, :, 1::2], -65504.0, 2.0 ** -11, context + drafts, -spread)
+        else:
+            assert (got[:, :, 1::2].abs() <= 65504 * 0.01).all()
