@@ -15,7 +15,7 @@
 // in fp32 before that (a sum of the rounded weights takes 1 % longer).
 //
 // Long prompts are bound by the matrix cores, at the clock that the power left to the chip allows: 16384 tokens, 32 heads of 128
-// on 8 key heads, bf16, 2.2 TFLOP of what queries see, take 1.97 - 2.02 ms (1.09 - 1.12 PFLOP/s; a large matrix product reaches
+// on 8 key heads, bf16, 2.2 TFLOP of what queries see, take 1.97 - 2.11 ms (1.04 - 1.12 PFLOP/s; a large matrix product reaches
 // 1.38) with the matrix cores busy in 67 % of clocks, of which there are 1.6 - 1.9 GHz.  Short ones are bound by the chain of
 // steps: a tile's 64 tokens take 0.6 us whatever the grid, so 1024 tokens of 32 heads, 16 tiles, 18 - 20 us.
 #include "abq_attn.h"
