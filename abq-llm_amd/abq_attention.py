@@ -3,8 +3,10 @@
 Works as abq_gemm.py does and on top of it: device buffers are torch tensors, there is no CPU fallback, and a call that the
 library refuses raises AbqError.  Import torch before this module.
 """
+import collections
 import ctypes
 import importlib.util
+import math
 import os
 import sys
 
@@ -23,6 +25,10 @@ F16, BF16 = 0, 1
 EXPORTED = [
     "abq_kv_codes_bytes", "abq_kv_scales_bytes", "abq_kv_append", "abq_kv_read",
     "abq_attn_prompt_init", "abq_attn_tree_init", "abq_attn_workspace_bytes", "abq_attn_set_workspace", "abq_attn_exec",
+    "abq_rotary_apply", "abq_kv_append_rotary",
+    "abq_kv_pages_fork", "abq_kv_pages_extend", "abq_kv_pages_compact", "abq_kv_copy_pages",
+    "abq_kv_bound_codes_bytes", "abq_kv_bound_scales_bytes", "abq_kv_bound", "abq_attn_choose",
+    "abq_attn_sparse_init", "abq_attn_sparse_workspace_bytes", "abq_attn_sparse_set_workspace", "abq_attn_sparse_exec",
 ]
 
 
@@ -50,6 +56,22 @@ class AttnState(ctypes.Structure):
     ]
 
 
+class RotaryDesc(ctypes.Structure):
+    _fields_ = [("rotary_dim", ctypes.c_int), ("axes", ctypes.c_int), ("interleaved", ctypes.c_int), ("turns", ctypes.c_void_p), ("axis", ctypes.c_void_p)]
+
+
+class KvPagesDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("seqs", "max_pages", "page_size", "num_pages")] + [(n, ctypes.c_void_p) for n in ("table", "lengths", "refs")]
+
+
+class KvBoundsDesc(ctypes.Structure):
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p)]
+
+
+class SparseState(ctypes.Structure):
+    _fields_ = [("attn", AttnState), ("blocks", ctypes.c_void_p), ("count", ctypes.c_int)]
+
+
 _lib = None
 
 
@@ -70,6 +92,23 @@ def lib():
         L.abq_attn_workspace_bytes.restype = ctypes.c_size_t
         L.abq_attn_set_workspace.argtypes = [P(AttnState), vp, ctypes.c_size_t]
         L.abq_attn_exec.argtypes = [P(AttnState), vp]
+        i64 = ctypes.c_int64
+        L.abq_rotary_apply.argtypes = [P(RotaryDesc), P(Rows), P(Rows), ci, P(Rows), P(Rows), ci, ci, ci, vp, i64, vp]
+        L.abq_kv_append_rotary.argtypes = [P(KvCacheDesc), P(RotaryDesc), P(Rows), P(Rows), ci, P(Rows), P(Rows), P(Rows), ci, vp, i64, vp, vp]
+        L.abq_kv_pages_fork.argtypes = [P(KvPagesDesc), vp, vp]
+        L.abq_kv_pages_extend.argtypes = [P(KvPagesDesc), vp, vp, i64, vp, vp, vp, vp]
+        L.abq_kv_pages_compact.argtypes = [P(KvPagesDesc), vp, vp]
+        L.abq_kv_copy_pages.argtypes = [P(KvCacheDesc), P(KvBoundsDesc), vp, i64, vp]
+        for name in ("abq_kv_bound_codes_bytes", "abq_kv_bound_scales_bytes"):
+            getattr(L, name).argtypes = [P(KvCacheDesc)]
+            getattr(L, name).restype = ctypes.c_size_t
+        L.abq_kv_bound.argtypes = [P(KvCacheDesc), P(KvBoundsDesc), vp, i64, vp]
+        L.abq_attn_choose.argtypes = [P(KvCacheDesc), P(KvBoundsDesc), P(Rows), ci, ci, vp, ci, vp, vp, ci, ci, ci, ci, ci, vp, vp]
+        L.abq_attn_sparse_init.argtypes = [P(KvCacheDesc), P(Rows), P(Rows), ci, ci, vp, ci, vp, vp, vp, vp, ci, ci, ci, ci, ctypes.c_float, P(SparseState)]
+        L.abq_attn_sparse_workspace_bytes.argtypes = [P(SparseState)]
+        L.abq_attn_sparse_workspace_bytes.restype = ctypes.c_size_t
+        L.abq_attn_sparse_set_workspace.argtypes = [P(SparseState), vp, ctypes.c_size_t]
+        L.abq_attn_sparse_exec.argtypes = [P(SparseState), vp]
         _lib = L
     return _lib
 
@@ -131,13 +170,133 @@ class _Memory:
             self.known.add(other.cuda_stream or None)
 
 
-class KvCache:
+class _OnStream:
+    """Objects whose calls take a stream and whose memory (self._memory) is safe on any"""
+
+    def _on(self, stream):
+        on = abq_gemm._stream_ptr(stream)
+        if on.value not in self._memory.known:
+            self._memory.use(stream)
+        return on
+
+
+class Rotary(_OnStream):
+    """Rotary positions of a head's first 2 * len(turns) elements: pair i turns by turns[i] revolutions per position (float64), of the
+    axis axis[i] (default: one axis).  Pairs are element i and i + len(turns), or neighbours if interleaved.  Both are copied to the device."""
+
+    def __init__(self, turns, axis=None, axes=None, interleaved=False, device="cuda"):
+        if torch.device(device).type != "cuda":
+            raise ValueError("the angles have to be on the device, not on %s" % device)
+        turns = torch.as_tensor(turns, dtype=torch.float64)
+        if turns.dim() != 1 or not turns.numel() or turns.numel() % 8:
+            raise ValueError("one number of revolutions for each of a multiple of 8 pairs is wanted")
+        if axis is not None:
+            axis = torch.as_tensor(axis, dtype=torch.int32)
+            if axis.shape != turns.shape or int(axis.min()) < 0:
+                raise ValueError("an axis, from 0, for each pair is wanted")
+            axes = axes or int(axis.max()) + 1
+            if int(axis.max()) >= axes:
+                raise ValueError("there are %d axes" % axes)
+        self.turns, self.axes = turns.to(device).contiguous(), axes or 1
+        self.axis = None if axis is None else axis.to(device).contiguous()
+        self.desc = RotaryDesc(2 * turns.numel(), self.axes, int(bool(interleaved)), self.turns.data_ptr(), None if axis is None else self.axis.data_ptr())
+        self._ref = ctypes.byref(self.desc)
+        self._memory = _Memory(tuple(t for t in (self.turns, self.axis) if t is not None))
+
+    @classmethod
+    def of_base(cls, dim, base=10000.0, sections=None, interleaved=False, device="cuda"):
+        """The usual angles, base^(-2 i / dim) per position; sections: how many pairs each axis has, in order, if there are several."""
+        pairs = dim // 2
+        turns = torch.tensor([base ** (-i / pairs) / (2 * math.pi) for i in range(pairs)], dtype=torch.float64)
+        axis = None
+        if sections is not None:
+            if sum(sections) != pairs:
+                raise ValueError("sections of %d pairs in all are wanted" % pairs)
+            axis = torch.repeat_interleave(torch.arange(len(sections)), torch.tensor(sections))
+        return cls(turns, axis, None if sections is None else len(sections), interleaved, device)
+
+    def _positions(self, positions, tokens):
+        """(address, stride) of positions int32 [tokens], or [axes, tokens] with the tokens beside each other"""
+        if positions.dim() == 1:
+            positions = positions[None]
+        if not positions.is_cuda or positions.dtype != torch.int32 or positions.shape != (self.axes, tokens) or (tokens > 1 and positions.stride(1) != 1):
+            raise ValueError("positions: a device tensor [%d, %d] of torch.int32 is wanted" % (self.axes, tokens))
+        return positions.data_ptr(), positions.stride(0) if self.axes > 1 else tokens
+
+    def apply(self, q, k, positions, out=None, stream=None):
+        """(q, k) turned, [tokens, heads, dim] each, into out = (q, k), which may be q and k themselves; k may be None."""
+        on = self._on(stream)
+        if k is not None and (k.dtype is not q.dtype or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]):
+            raise ValueError("q [tokens, heads, dim] and k [tokens, kv heads, dim] of one type are wanted")
+        if out is None:
+            with torch.cuda.stream(None if stream is None else _stream_of(stream)):  # (tensors of the stream that they are written on)
+                out = (torch.empty(q.shape, dtype=q.dtype, device=q.device), None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device))
+        for x, y in zip((q, k), out):
+            if (x is None) != (y is None) or (x is not None and (x.shape != y.shape or x.dtype is not y.dtype)):
+                raise ValueError("out has to be of the inputs' shapes and type")
+        at, step = self._positions(positions, q.shape[0])
+        rows = [None if t is None else ctypes.byref(_rows(t)) for t in (q, out[0], k, out[1])]
+        _check(lib().abq_rotary_apply(self._ref, rows[0], rows[1], q.shape[1], rows[2], rows[3], 0 if k is None else k.shape[1], q.shape[2], _dtype(q), at,
+                                      step, on), "abq_rotary_apply")
+        return out
+
+
+Extension = collections.namedtuple("Extension", "slots starts granted copies")
+
+
+class PageTable(_OnStream):
+    """Which pages hold which sequence's tokens: table int32 [sequences, max_pages] (-1: none), lengths [sequences] and refs [num_pages], how
+    many entries name each page, on the device.  Every sequence is empty at first."""
+
+    def __init__(self, num_pages, page_size, sequences, max_pages, device="cuda"):
+        if torch.device(device).type != "cuda":
+            raise ValueError("the table has to be on the device, not on %s" % device)
+        if min(num_pages, page_size, sequences, max_pages) < 1:
+            raise ValueError("no such table: %d sequences of %d pages, of %d of %d tokens" % (sequences, max_pages, num_pages, page_size))
+        self.table = torch.full((sequences, max_pages), -1, dtype=torch.int32, device=device)
+        self.lengths, self.refs = (torch.zeros(n, dtype=torch.int32, device=device) for n in (sequences, num_pages))
+        self.desc = KvPagesDesc(sequences, max_pages, page_size, num_pages, *(t.data_ptr() for t in (self.table, self.lengths, self.refs)))
+        self._ref = ctypes.byref(self.desc)
+        self._memory = _Memory((self.table, self.lengths, self.refs))
+
+    def _made(self, shapes, stream):
+        with torch.cuda.stream(None if stream is None else _stream_of(stream)):
+            return [torch.empty(s, dtype=torch.int32, device=self.table.device) for s in shapes]
+
+    def fork(self, parents, stream=None):
+        """Sequence s takes over the tokens of sequence parents[s] (int32 [sequences]; -1: none) as they were before, on the same pages."""
+        at, on = _index(parents, torch.int32, self.desc.seqs, "parents"), self._on(stream)
+        _check(lib().abq_kv_pages_fork(self._ref, at, on), "abq_kv_pages_fork")
+
+    def extend(self, counts, rows, out=None, stream=None):
+        """Room for counts[s] more tokens in sequence s (int32 [sequences]), or counts[s] < 0 taken away.  Returns, or fills out with, an
+        Extension: slots [rows] of the new tokens, one sequence behind the other, starts [sequences + 1], granted [sequences] and copies
+        [sequences, 2], the pages that KvCache.copy_pages has to copy in every layer before anything is written."""
+        n = self.desc.seqs
+        at, on = _index(counts, torch.int32, n, "counts"), self._on(stream)
+        out = out or Extension(*self._made([(rows,), (n + 1,), (n,), (n, 2)], stream))
+        to = [_index(t, torch.int32, m, name) for t, m, name in zip(out, (rows, n + 1, n, 2 * n), Extension._fields)]
+        _check(lib().abq_kv_pages_extend(self._ref, at, to[0], rows, *to[1:], on), "abq_kv_pages_extend")
+        return out
+
+    def compact(self, out=None, stream=None):
+        """Moves the live pages to the front; returns (or fills out with) moves [num_pages // 2, 2] for KvCache.copy_pages of every layer."""
+        on, half = self._on(stream), self.desc.num_pages // 2
+        out = self._made([(half, 2)], stream)[0] if out is None else out
+        _check(lib().abq_kv_pages_compact(self._ref, _index(out, torch.int32, 2 * half, "moves"), on), "abq_kv_pages_compact")
+        return out
+
+
+class KvCache(_OnStream):
     """A paged cache of keys and values in codes of 8 or 4 bits with a scale (and a zero point) per token and head.
 
     A token's place is its slot, page * page_size + offset.  With zero points (symmetric=False) a row that lies more than 39 of its spreads
-    from zero (8 bits; 667 with 4) is not held as what it is: zero points end at 1e4, scales begin at 1e-5."""
+    from zero (8 bits; 667 with 4) is not held as what it is: zero points end at 1e4, scales begin at 1e-5.
 
-    def __init__(self, num_pages, page_size, kv_heads, head_dim, bits=8, symmetric=True, device="cuda"):
+    With bounds=True it has room for bounds of every page's keys (bound_codes int8 [pages, kv heads, 2, head dim], bound_scales [pages,
+    kv heads]), which bound() writes and SparseAttention chooses pages by."""
+
+    def __init__(self, num_pages, page_size, kv_heads, head_dim, bits=8, symmetric=True, device="cuda", bounds=False):
         if torch.device(device).type != "cuda":
             raise ValueError("the cache has to be on the device, not on %s" % device)
         d = KvCacheDesc(bits, int(bool(symmetric)), kv_heads, head_dim, page_size, num_pages)
@@ -150,7 +309,15 @@ class KvCache:
         self.desc = d
         self._ref, self._row = ctypes.byref(d), (kv_heads, head_dim)
         self._append, self._read = lib().abq_kv_append, lib().abq_kv_read
-        self._memory = _Memory((self.k_codes, self.v_codes, self.k_scales, self.v_scales))
+        held = (self.k_codes, self.v_codes, self.k_scales, self.v_scales)
+        self.bounds = self._bounds = None
+        if bounds:
+            self.bound_codes = torch.zeros((num_pages, kv_heads, 2, head_dim), dtype=torch.int8, device=device)
+            self.bound_scales = torch.zeros((num_pages, kv_heads), dtype=torch.float32, device=device)
+            self.bounds = KvBoundsDesc(self.bound_codes.data_ptr(), self.bound_scales.data_ptr())
+            self._bounds = ctypes.byref(self.bounds)
+            held += (self.bound_codes, self.bound_scales)
+        self._memory = _Memory(held)
         self._known = self._memory.known
 
     def _call(self, call, name, k, v, slots, stream):
@@ -178,7 +345,45 @@ class KvCache:
         return out
 
 
+    def append_rotated(self, rotary, q, k, v, positions, slots, q_out=None, k_out=None, stream=None):
+        """Turns q and k by their positions and appends the turned k and v, in one launch.  Returns (q_out, k_out): the turned q, in a new
+        tensor by default (None without q), and the turned k if k_out is given (the same tensors as q and k turn them in place)."""
+        if k.shape != v.shape or k.dtype is not v.dtype or k.shape[1:] != self._row:
+            raise ValueError("keys and values [tokens, %d, %d] of one type are wanted" % self._row)
+        if q is not None and (q.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or q.dtype is not k.dtype):
+            raise ValueError("q [%d, heads, %d] of the keys' type is wanted" % (k.shape[0], k.shape[2]))
+        if q is not None and q_out is None:
+            with torch.cuda.stream(None if stream is None else _stream_of(stream)):
+                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        for x, y in ((q, q_out), (k, k_out)):
+            if y is not None and (x is None or x.shape != y.shape or x.dtype is not y.dtype):
+                raise ValueError("q_out and k_out have to be of the inputs' shapes and type")
+        at, on = _index(slots, torch.int32, k.shape[0], "slots"), self._on(stream)
+        rotary._on(stream)
+        turns, step = rotary._positions(positions, k.shape[0])
+        rows = [None if t is None else ctypes.byref(_rows(t)) for t in (q, q_out, k, k_out, v)]
+        _check(lib().abq_kv_append_rotary(self._ref, rotary._ref, rows[0], rows[1], 0 if q is None else q.shape[1], rows[2], rows[3], rows[4], _dtype(k),
+                                          turns, step, at, on), "abq_kv_append_rotary")
+        return q_out, k_out
+
+    def copy_pages(self, pairs, stream=None):
+        """Copies page pairs[i, 0] to page pairs[i, 1] (int32 [n, 2]; -1: nothing), bounds included."""
+        if pairs.dim() != 2 or pairs.shape[1] != 2:
+            raise ValueError("pairs of pages [n, 2] are wanted")
+        at, on = _index(pairs, torch.int32, pairs.numel(), "pairs"), self._on(stream)
+        _check(lib().abq_kv_copy_pages(self._ref, self._bounds, at, pairs.shape[0], on), "abq_kv_copy_pages")
+
+    def bound(self, slots, stream=None):
+        """Writes the bounds of the pages that these slots complete: behind an append, with its slots."""
+        if self.bounds is None:
+            raise ValueError("this cache has no bounds")
+        at, on = _index(slots, torch.int32, slots.numel(), "slots"), self._on(stream)
+        _check(lib().abq_kv_bound(self._ref, self._bounds, at, slots.numel(), on), "abq_kv_bound")
+
+
 class _Attention:
+    _calls = ("abq_attn_workspace_bytes", "abq_attn_set_workspace", "abq_attn_exec")
+
     def _finish(self, out, workspace, *made):
         self.out = out
         need = self.workspace_bytes
@@ -191,13 +396,13 @@ class _Attention:
         self._memory = _Memory(made)
         self._known = self._memory.known
         if workspace is not None and workspace.numel():
-            _check(lib().abq_attn_set_workspace(ctypes.byref(self.state), workspace.data_ptr(), workspace.numel() * workspace.element_size()),
-                   "abq_attn_set_workspace")
-        self._exec, self._state = lib().abq_attn_exec, ctypes.byref(self.state)
+            _check(getattr(lib(), self._calls[1])(ctypes.byref(self.state), workspace.data_ptr(), workspace.numel() * workspace.element_size()),
+                   self._calls[1])
+        self._exec, self._state = getattr(lib(), self._calls[2]), ctypes.byref(self.state)
 
     @property
     def workspace_bytes(self):
-        return lib().abq_attn_workspace_bytes(ctypes.byref(self.state))
+        return getattr(lib(), self._calls[0])(ctypes.byref(self.state))
 
     def run(self, stream=None):
         """One pass over what the tensors hold now; returns out.  A graph that captures it needs the object for as long as it is replayed."""
@@ -206,7 +411,7 @@ class _Attention:
             self._memory.use(stream)
         status = self._exec(self._state, on)
         if status:
-            raise AbqError(status, "abq_attn_exec")
+            raise AbqError(status, self._calls[2])
         return self.out
 
 
@@ -262,3 +467,55 @@ class TreeAttention(_Attention):
                                         None if mask is None else _index(mask, torch.int64, q.shape[0], "mask"), seqs, max_q, max_context,
                                         q.shape[2] ** -0.5 if scale is None else scale, ctypes.byref(self.state)), "abq_attn_tree_init")
         self._finish(out, workspace, *made, *cache._memory.tensors)
+
+
+class SparseAttention(_Attention):
+    """Attention of drafted tokens as TreeAttention's, but every draft and key head sees only `count` of the context's complete pages, and what
+    stands behind them: the first `first`, the last `last`, and those whose bounds promise the largest scores for its queries.  Each pass
+    chooses them anew into blocks, int32 [drafts, kv heads, count]; with blocks given, those are seen and nothing is chosen."""
+
+    _calls = ("abq_attn_sparse_workspace_bytes", "abq_attn_sparse_set_workspace", "abq_attn_sparse_exec")
+
+    def __init__(self, q, cache, page_table, context, q_starts, max_q, max_context, count, first=1, last=1, mask=None, scale=None, out=None, workspace=None,
+                 blocks=None):
+        d = cache.desc
+        if q.dim() != 3 or q.shape[2] != d.head_dim:
+            raise ValueError("q [drafts, heads, %d] is wanted" % d.head_dim)
+        if blocks is None and cache.bounds is None:
+            raise ValueError("this cache has no bounds to choose pages by")
+        if count < 1 or min(first, last) < 0 or first + last > count:
+            raise ValueError("count >= first + last pages, one at least, are wanted")
+        made = ()
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            made = (out,)
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError("out has to be of q's shape and type")
+        self._choose = blocks is None
+        if blocks is None:
+            blocks = torch.full((q.shape[0], d.kv_heads, count), -1, dtype=torch.int32, device=q.device)
+            made += (blocks,)
+        self.blocks, seqs = blocks, context.numel()
+        rows = [_rows(t) for t in (q, out)]
+        table = _index(page_table, torch.int32, seqs * page_table.shape[-1], "page_table")
+        at = [_index(blocks, torch.int32, q.shape[0] * d.kv_heads * count, "blocks"), _index(context, torch.int32, seqs, "context"),
+              _index(q_starts, torch.int32, seqs + 1, "q_starts")]
+        self.held = (q, cache, page_table, context, q_starts, mask, blocks)
+        self.state = SparseState()
+        _check(lib().abq_attn_sparse_init(ctypes.byref(d), ctypes.byref(rows[0]), ctypes.byref(rows[1]), _dtype(q), q.shape[1], table, page_table.shape[-1],
+                                          at[1], at[2], None if mask is None else _index(mask, torch.int64, q.shape[0], "mask"), at[0], count, seqs, max_q,
+                                          max_context, q.shape[2] ** -0.5 if scale is None else scale, ctypes.byref(self.state)), "abq_attn_sparse_init")
+        self._chosen = (ctypes.byref(d), cache._bounds, ctypes.byref(rows[0]), _dtype(q), q.shape[1], table, page_table.shape[-1], at[1], at[2], seqs, max_q,
+                        first, last, count, at[0])
+        if self._choose and page_table.shape[-1] > 32768:
+            raise AbqError(abq_gemm.ABQ_ERR_TOO_LARGE, "abq_attn_choose")
+        self._finish(out, workspace, *made, *cache._memory.tensors)
+
+    def run(self, stream=None):
+        """One pass over what the tensors hold now; returns out.  A graph that captures it needs the object for as long as it is replayed."""
+        if self._choose:
+            on = abq_gemm._stream_ptr(stream)
+            if on.value not in self._known:
+                self._memory.use(stream)
+            _check(lib().abq_attn_choose(*self._chosen, on), "abq_attn_choose")
+        return super().run(stream)

@@ -6,7 +6,7 @@
 #include <math.h>
 #include <string.h>
 
-#include "abq_attn.h"
+#include "abq_attn_checks.h"
 
 namespace abq {
 
@@ -19,44 +19,6 @@ constexpr int64_t kMostTileStride = 1 << 25;
 
 // Scales that fp32 holds times log2(e), and for drafts times a token's scale and zero point, of up to 1e4 each, as well
 constexpr float kMostPromptScale = 2e38f, kMostTreeScale = 2e30f;
-
-// a * b * c, none of them negative, or more than any limit here where that does not fit
-int64_t product(int64_t a, int64_t b, int64_t c)
-{
-    int64_t x;
-    return __builtin_mul_overflow(a, b, &x) || __builtin_mul_overflow(x, c, &x) ? INT64_MAX : x;
-}
-
-bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
-
-// written: rows of a result, which may not lie on one another
-abq_status check_rows(const abq_rows *r, int64_t rows, int heads, int head_dim, bool written = false)
-{
-    if (!r || r->rows != rows || (rows && !r->data) || !aligned16(r->data) || r->row_stride % 8 || r->head_stride % 8)
-        return ABQ_ERR_INVALID_ARG;
-    if (r->row_stride < 0 || r->head_stride < 0 || (heads > 1 && r->head_stride < head_dim) || (written && rows > 1 && r->row_stride < head_dim))
-        return ABQ_ERR_INVALID_ARG;
-    return ABQ_OK;
-}
-
-bool cache_sizes_valid(const abq_kv_cache *c)
-{
-    return c && (c->bits == 8 || c->bits == 4) && (c->head_dim == 64 || c->head_dim == 128) && c->kv_heads > 0 && c->num_pages > 0 &&
-           c->page_size >= 16 && c->page_size <= 4096 && (c->page_size & (c->page_size - 1)) == 0 &&
-           (int64_t)c->num_pages * c->page_size <= 0x7fffffff && c->kv_heads <= 65536;
-}
-
-abq_status check_cache(const abq_kv_cache *c)
-{
-    if (!c)
-        return ABQ_ERR_INVALID_ARG;
-    if ((c->bits != 8 && c->bits != 4) || (c->head_dim != 64 && c->head_dim != 128))
-        return ABQ_ERR_UNSUPPORTED;
-    if (!cache_sizes_valid(c) || !c->k_codes || !c->v_codes || !c->k_scales || !c->v_scales || !aligned16(c->k_codes) ||
-        !aligned16(c->v_codes) || !aligned16(c->k_scales) || !aligned16(c->v_scales))
-        return ABQ_ERR_INVALID_ARG;
-    return ABQ_OK;
-}
 
 abq_status check_cache_call(const abq_kv_cache *c, const abq_rows *k, const abq_rows *v, int dtype, const int32_t *slots, bool written)
 {
@@ -103,6 +65,9 @@ abq_status init_common(int kind, const abq_rows *q, const abq_rows *out, int dty
     return ABQ_OK;
 }
 
+// (the state inside that of attention to chosen pages runs with its lists alone)
+bool ready(const abq_attn_state &st) { return st.init_success && (st.kind == kPromptKind || st.kind == kTreeKind); }
+
 void plan(abq_attn_state *st, int most_parts)
 {
     if (st->kind == kTreeKind)
@@ -110,8 +75,6 @@ void plan(abq_attn_state *st, int most_parts)
     else
         plan_attn_prompt(st, most_parts);
 }
-
-constexpr int kMostParts = 4096;
 
 } // namespace
 
@@ -203,7 +166,7 @@ abq_status abq_attn_tree_init(const abq_kv_cache *cache, const abq_rows *q, cons
 
 size_t abq_attn_workspace_bytes(const abq_attn_state *state)
 {
-    if (!state || !state->init_success)
+    if (!state || !ready(*state))
         return 0;
     abq_attn_state best = *state;
     plan(&best, kMostParts);
@@ -214,7 +177,7 @@ abq_status abq_attn_set_workspace(abq_attn_state *state, void *workspace, size_t
 {
     if (!state)
         return ABQ_ERR_INVALID_ARG;
-    if (!state->init_success)
+    if (!ready(*state))
         return ABQ_ERR_NOT_INITIALIZED;
     if ((bytes && !workspace) || !aligned16(workspace))
         return ABQ_ERR_INVALID_ARG;
@@ -231,7 +194,7 @@ abq_status abq_attn_exec(const abq_attn_state *state, void *stream)
 {
     if (!state)
         return ABQ_ERR_INVALID_ARG;
-    if (!state->init_success)
+    if (!ready(*state))
         return ABQ_ERR_NOT_INITIALIZED;
     if (state->q.rows == 0)
         return ABQ_OK;

@@ -22,6 +22,8 @@ void plan_attn_tree(abq_attn_state *st, int most_parts);
 // HIP counts the threads of a launch in 32 bits; workgroups have 256, where nothing else is said
 constexpr int64_t kMostThreads = 0xffffffffll, kMostBlocks = kMostThreads / 256;
 
+constexpr int kMostParts = 4096;
+
 // Bytes of the parts' results: per query row and head, `parts` sums of head_dim floats and as many pairs (maximum, sum)
 inline size_t attn_parts_bytes(const abq_attn_state &st, int parts)
 {

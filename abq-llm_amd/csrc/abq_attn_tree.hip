@@ -26,7 +26,7 @@
 // rows a step's vector work (400 operations beside 32 MFMA: codes to fp16, factors, exponentials) and the loads share the time:
 // two waves per SIMD, each with a step under way while it works at another.  20 rows on 48 ragged contexts, 630 MB: 148 us,
 // 4.3 TB/s; 108 rows on 3 x 5500 tokens of 4 bits, 28 us, bound by that work and, at 9 steps a wave, by its start and end.
-#include "abq_attn.h"
+#include "abq_decoding.h"
 
 namespace abq {
 
@@ -41,6 +41,9 @@ struct TreeArgs {
     int page_shift;
     float scale_log2;
     AttnParts parts;
+    // pages of the context that each row and key head sees ([row][key head][listed]), where it does not see all of it
+    const int32_t *blocks;
+    int listed;
 };
 
 constexpr int kStep = 32; // tokens of a wave's step
@@ -78,9 +81,9 @@ template <int K> __device__ __forceinline__ float of_lane(float x)
     return __builtin_bit_cast(float, of_lane<K>(__builtin_bit_cast(uint32_t, x)));
 }
 
-// `seen`: bit h is cleared if half h lies on a page outside the cache
+// at0, at1: the places of the halves' first tokens.  `seen`: bit h is cleared if half h lies on a page outside the cache
 template <int BITS, bool ASYM, int D>
-__device__ __forceinline__ void load_step(Step<BITS, ASYM, D> &s, const TreeArgs &a, const int32_t *pages, int last_page, int head, int at, int lane,
+__device__ __forceinline__ void load_step(Step<BITS, ASYM, D> &s, const TreeArgs &a, const int32_t *pages, int last_page, int head, int at0, int at1, int lane,
                                           uint32_t *seen)
 {
     using S = Step<BITS, ASYM, D>;
@@ -90,7 +93,7 @@ __device__ __forceinline__ void load_step(Step<BITS, ASYM, D> &s, const TreeArgs
     *seen = 3;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const int pos = at + 16 * h;
+        const int pos = h ? at1 : at0;
         int page = pages[min(pos >> a.page_shift, last_page)];
         if ((uint32_t)page >= (uint32_t)a.c.num_pages) {
             page = 0;
@@ -188,7 +191,9 @@ template <int BITS, int D> __device__ __forceinline__ int query_offset(int ks, i
     return (ks / kPieces) * (32 * kPieces) + g * 8 * kPieces + (ks % kPieces) * 8;
 }
 
-template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(64 * tree_waves(RT), RT == 1 ? 4 : 2) void attn_tree_kernel(TreeArgs a)
+// LISTED: a workgroup has one draft's rows, whose steps go over the pages of its list, and then from the end of the last complete page on.
+template <int BITS, bool ASYM, int D, int RT, bool LISTED>
+__global__ __launch_bounds__(64 * tree_waves(RT), RT == 1 ? 4 : 2) void attn_tree_kernel(TreeArgs a)
 {
     using S = Step<BITS, ASYM, D>;
     constexpr int kWaves = tree_waves(RT);
@@ -203,13 +208,14 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(64 * 
     const uint32_t round = 8 * a.row_blocks, in_round = blockIdx.x % round;
     const uint32_t unit = blockIdx.x / round * 8 + in_round % 8;
     const int row_block = in_round / 8;
-    if (unit >= (uint32_t)a.seqs * a.c.kv_heads * a.parts.parts)
+    if (unit >= (uint32_t)a.seqs * a.c.kv_heads * a.parts.parts * (LISTED ? a.max_q : 1))
         return;
-    const int part = unit % a.parts.parts, head = unit / a.parts.parts % a.c.kv_heads, seq = unit / a.parts.parts / a.c.kv_heads;
+    const int part = unit % a.parts.parts, head = unit / a.parts.parts % a.c.kv_heads;
+    const int seq = unit / a.parts.parts / a.c.kv_heads / (LISTED ? a.max_q : 1), draft0 = LISTED ? unit / a.parts.parts / a.c.kv_heads % a.max_q : 0;
 
     const SeqRows own = seq_rows(a.q_starts, seq, a.q.rows);
     const int n = min(own.count, 64); // drafts that can be seen, of which max_q are computed
-    const int rows = min(n, a.max_q) * a.group, row0 = row_block * 16 * RT;
+    const int rows = LISTED ? (draft0 < n ? a.group : 0) : min(n, a.max_q) * a.group, row0 = row_block * 16 * RT;
     if (row0 >= rows)
         return;
     const int64_t places = (int64_t)a.max_pages << a.page_shift;
@@ -217,6 +223,28 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(64 * 
     const int len = (int)min((int64_t)context + n, places);
     const int32_t *pages = a.page_table + (int64_t)seq * a.max_pages;
     const int last_page = (len - 1) >> a.page_shift; // (len is 0 only without steps)
+    // tokens that are gone over: all, or those of the list up to the last page that it names, and what stands behind the complete pages
+    const int complete = min(context >> a.page_shift, a.max_pages), behind = complete << a.page_shift;
+    const int32_t *list = LISTED ? a.blocks + ((int64_t)(own.first + draft0) * a.c.kv_heads + head) * a.listed : nullptr;
+    int named = 0;
+    if constexpr (LISTED) {
+        for (int i0 = (a.listed - 1) & ~63; i0 >= 0 && named == 0; i0 -= 64) {
+            const uint64_t some = __ballot(i0 + lane < a.listed && (uint32_t)list[min(i0 + lane, a.listed - 1)] < (uint32_t)complete);
+            named = some ? i0 + 64 - __builtin_clzll(some) : 0;
+        }
+    }
+    const int64_t inside = (int64_t)named << a.page_shift, over = LISTED ? inside + len - behind : len;
+    // the place of a step's half, or -1 if it has none
+    auto place_of = [&](int step, int h) {
+        const int64_t x = (int64_t)step * kStep + 16 * h;
+        if constexpr (LISTED) {
+            if (x >= inside)
+                return behind + (int)(x - inside);
+            const int32_t block = list[x >> a.page_shift];
+            return (uint32_t)block < (uint32_t)complete ? (block << a.page_shift) + (int)(x & (a.c.page_size - 1)) : -1;
+        }
+        return (int)x;
+    };
 
     // the queries as the products take them, the power of two that they were divided by, and their sums
     half8v q[RT][D / 32];
@@ -224,7 +252,7 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(64 * 
     uint64_t sees[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const int row = min(row0 + 16 * rt + t, rows - 1), draft = row / a.group;
+        const int row = min(row0 + 16 * rt + t, rows - 1), draft = LISTED ? draft0 : row / a.group;
         const uint16_t *src = (const uint16_t *)a.q.data + (int64_t)(own.first + draft) * a.q.row_stride + (int64_t)(head * a.group + row % a.group) * a.q.head_stride;
         sees[rt] = a.mask ? a.mask[own.first + draft] : ~0ull >> (63 - draft);
         factor[rt] = 1.f;
@@ -283,10 +311,11 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(64 * 
             out[rt][i] = float4v{0, 0, 0, 0};
     }
 
-    const int steps = (len + kStep - 1) / kStep;
+    const int steps = (int)((over + kStep - 1) / kStep);
     const int step0 = (int)((int64_t)steps * part / a.parts.parts) + wave, step1 = (int)((int64_t)steps * (part + 1) / a.parts.parts);
     const Magic mg = magic();
-    auto weigh_step = [&](S &s, int step, uint32_t seen) {
+    auto weigh_step = [&](S &s, int step, int at0, int at1, uint32_t seen) {
+        const int at[2] = {LISTED ? at0 : step * kStep, LISTED ? at1 : step * kStep + 16};
         // scores
         float score[RT][2][4];
 #pragma unroll
@@ -316,11 +345,10 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(64 * 
         }
         // The lane's one token: factor and offset of the scores, logarithm and reciprocal of the value scale.  (Codes are less half
         // their range here, and so are zero points.)  What no row sees holds anything, and is replaced.
-        const int at = step * kStep;
-        const bool some = at + kStep > context || seen != 3; // (some row does not see some token of the step)
+        const bool some = (LISTED && at[0] + 16 > context) || at[1] + 16 > context || seen != 3; // (some row does not see some token of the step)
         if (some) {
             const int h = t >> 2 & 1;
-            const bool there = at + 16 * h + 4 * g + (t & 3) < len && (seen >> h & 1);
+            const bool there = (h ? at[1] : at[0]) + 4 * g + (t & 3) < len && (seen >> h & 1);
             s.ks = there ? s.ks : 0.f;
             s.vs = there ? s.vs : 1.f;
             if (ASYM) {
@@ -348,7 +376,7 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(64 * 
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int pos = at + 16 * h + 4 * g + i;
+                    const int pos = at[h] + 4 * g + i;
                     const bool there = pos < len && (seen >> h & 1);
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt)
@@ -423,27 +451,35 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(64 * 
     // One row tile leaves registers for four waves per SIMD, which cover each other's loads; with more, a wave loads a step ahead.
     // Eight waves in a workgroup keep them there where there are few workgroups (of four and of eight: 32768 tokens, 8 heads 25 and 20
     // us, 20 x 700 tokens 11.3 and 10.2, 16 x 1024 of 32 heads 29 either way; sixteen 20, 10.6, 34).
+    auto load = [&](S &s, int step, int &at0, int &at1, uint32_t &seen) {
+        at0 = place_of(step, 0);
+        at1 = place_of(step, 1);
+        load_step<BITS, ASYM, D>(s, a, pages, last_page, head, LISTED ? max(at0, 0) : at0, LISTED ? max(at1, 0) : at1, lane, &seen);
+        if (LISTED)
+            seen &= (at0 < 0 ? ~1u : ~0u) & (at1 < 0 ? ~2u : ~0u);
+    };
+    int at00, at01, at10, at11; // (places of the halves of the two steps in flight)
     if constexpr (RT == 1) {
         for (int step = step0; step < step1; step += kWaves) {
             S s;
             uint32_t seen;
-            load_step<BITS, ASYM, D>(s, a, pages, last_page, head, step * kStep, lane, &seen);
-            weigh_step(s, step, seen);
+            load(s, step, at00, at01, seen);
+            weigh_step(s, step, at00, at01, seen);
         }
     } else {
         S s[2];
         uint32_t seen[2];
         if (step0 < step1)
-            load_step<BITS, ASYM, D>(s[0], a, pages, last_page, head, step0 * kStep, lane, &seen[0]);
+            load(s[0], step0, at00, at01, seen[0]);
         for (int step = step0; step < step1; step += 2 * kWaves) {
             if (step + kWaves < step1)
-                load_step<BITS, ASYM, D>(s[1], a, pages, last_page, head, (step + kWaves) * kStep, lane, &seen[1]);
-            weigh_step(s[0], step, seen[0]);
+                load(s[1], step + kWaves, at10, at11, seen[1]);
+            weigh_step(s[0], step, at00, at01, seen[0]);
             if (step + kWaves >= step1)
                 break;
             if (step + 2 * kWaves < step1)
-                load_step<BITS, ASYM, D>(s[0], a, pages, last_page, head, (step + 2 * kWaves) * kStep, lane, &seen[0]);
-            weigh_step(s[1], step + kWaves, seen[1]);
+                load(s[0], step + 2 * kWaves, at00, at01, seen[0]);
+            weigh_step(s[1], step + kWaves, at10, at11, seen[1]);
         }
     }
 
@@ -489,7 +525,7 @@ template <int BITS, bool ASYM, int D, int RT> __global__ __launch_bounds__(64 * 
             for (int e = 0; e < kEach; ++e)
                 acc[e] += f * (sums[w][r][d0 + e] - (ASYM ? stat_z[w][16 * rt + r] : 0.f));
         }
-        const int64_t q_row = own.first + row / a.group;
+        const int64_t q_row = own.first + (LISTED ? draft0 : row / a.group);
         const int q_head = head * a.group + row % a.group;
         if (a.parts.parts > 1) {
             const int64_t at = (q_row * a.heads + q_head) * a.parts.parts + part;
@@ -578,17 +614,16 @@ hipError_t launch_attn_join(const abq_attn_state &st, hipStream_t stream)
     return hipGetLastError();
 }
 
-void plan_attn_tree(abq_attn_state *st, int most_parts)
+// `rows` of queries for each of key_heads sequences' heads (or drafts', where each has pages of its own), over at most `tokens`
+static void plan_rows(abq_attn_state *st, int rows, int64_t key_heads, int64_t tokens, int most_parts)
 {
-    const int rows = st->max_q * (st->heads / st->kv_heads);
     // Blocks of 32 rows read a code once for two products, where there are two: 27 drafts of 4 heads per key head on 3 x 5500 tokens of
     // 4 bits 30.5 us, in blocks of 16 rows 32; 48 ragged contexts, 20 rows, 147.5 and 173.  (64 drafts on 4000 tokens, or 16 of 4 heads
     // on 4 x 2000, take the same in either: 20.8, 15.)  Up to 16 rows the second half would be empty, but the workgroups have half as many
     // threads, and twice as many of them fit a launch.
-    const int64_t key_heads = (int64_t)st->seqs * st->kv_heads;
     st->block_rows = rows <= 16 && key_heads + 8 <= kMostThreads / (64 * tree_waves(1)) ? 16 : 32;
     const int64_t units = key_heads * ((rows + st->block_rows - 1) / st->block_rows);
-    const int64_t steps = ((int64_t)st->max_k + kStep - 1) / kStep;
+    const int64_t steps = (tokens + kStep - 1) / kStep;
     // Eight waves of 16 rows, or two times four of 32, per compute unit, the more of a part's waves with a step or two the better: with
     // the cache's bytes from memory, and up to 16 rows, one sequence takes
     //   us in parts                        1     2     4     8    16    32
@@ -616,7 +651,25 @@ void plan_attn_tree(abq_attn_state *st, int most_parts)
     st->parts = parts < 1 ? 1 : (int)parts;
 }
 
-#define ABQ_TREE(B, A, D_, RT_) hipLaunchKernelGGL((attn_tree_kernel<B, A, D_, RT_>), grid, dim3(64 * tree_waves(RT_)), 0, stream, a)
+void plan_attn_tree(abq_attn_state *st, int most_parts)
+{
+    plan_rows(st, st->max_q * (st->heads / st->kv_heads), (int64_t)st->seqs * st->kv_heads, st->max_k, most_parts);
+}
+
+void plan_attn_sparse(abq_sparse_state *sparse, int most_parts)
+{
+    abq_attn_state *st = &sparse->attn;
+    const int64_t listed = (int64_t)sparse->count * st->cache.page_size + st->cache.page_size - 1 + st->max_q;
+    plan_rows(st, st->heads / st->kv_heads, (int64_t)st->seqs * st->max_q * st->kv_heads, listed < st->max_k ? listed : st->max_k, most_parts);
+}
+
+#define ABQ_TREE(B, A, D_, RT_)                                                                                               \
+    do {                                                                                                                      \
+        if (a.blocks)                                                                                                         \
+            hipLaunchKernelGGL((attn_tree_kernel<B, A, D_, RT_, true>), grid, dim3(64 * tree_waves(RT_)), 0, stream, a);      \
+        else                                                                                                                  \
+            hipLaunchKernelGGL((attn_tree_kernel<B, A, D_, RT_, false>), grid, dim3(64 * tree_waves(RT_)), 0, stream, a);     \
+    } while (0)
 #define ABQ_TREE_ROWS(B, A, D_)           \
     do {                                  \
         if (st.block_rows == 16)          \
@@ -632,7 +685,7 @@ void plan_attn_tree(abq_attn_state *st, int most_parts)
             ABQ_TREE_ROWS(B, A, 128);     \
     } while (0)
 
-hipError_t launch_attn_tree(const abq_attn_state &st, hipStream_t stream)
+static hipError_t launch_tree(const abq_attn_state &st, const int32_t *blocks, int listed, hipStream_t stream)
 {
     TreeArgs a;
     a.c = st.cache;
@@ -647,12 +700,14 @@ hipError_t launch_attn_tree(const abq_attn_state &st, hipStream_t stream)
     a.seqs = st.seqs;
     a.max_q = st.max_q;
     a.max_pages = st.max_pages;
-    a.row_blocks = (st.max_q * a.group + st.block_rows - 1) / st.block_rows;
+    a.blocks = blocks;
+    a.listed = listed;
+    a.row_blocks = ((blocks ? 1 : st.max_q) * a.group + st.block_rows - 1) / st.block_rows;
     a.dtype = st.dtype;
     a.page_shift = __builtin_ctz((unsigned)st.cache.page_size);
     a.scale_log2 = st.scale * kLog2e;
     a.parts = attn_parts(st);
-    const int64_t units = (int64_t)st.seqs * st.kv_heads * st.parts;
+    const int64_t units = (int64_t)st.seqs * (blocks ? st.max_q : 1) * st.kv_heads * st.parts;
     const dim3 grid((unsigned)((units + 7) / 8 * 8 * a.row_blocks));
     if (st.cache.bits == 8) {
         if (st.cache.symmetric)
@@ -666,5 +721,9 @@ hipError_t launch_attn_tree(const abq_attn_state &st, hipStream_t stream)
     const hipError_t e = hipGetLastError();
     return e != hipSuccess || st.parts < 2 ? e : launch_attn_join(st, stream);
 }
+
+hipError_t launch_attn_tree(const abq_attn_state &st, hipStream_t stream) { return launch_tree(st, nullptr, 0, stream); }
+
+hipError_t launch_attn_sparse(const abq_sparse_state &st, hipStream_t stream) { return launch_tree(st.attn, st.blocks, st.count, stream); }
 
 } // namespace abq

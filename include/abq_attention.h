@@ -80,6 +80,82 @@ abq_status abq_kv_append(const abq_kv_cache *cache, const abq_rows *k, const abq
 abq_status abq_kv_read(const abq_kv_cache *cache, const abq_rows *k, const abq_rows *v, int dtype, const int32_t *slots, void *stream);
 
 /* ---------------------------------------------------------------------------------------
+ * Rotary positions
+ *
+ * Of every head's first rotary_dim elements, pair i (of rotary_dim / 2) is turned by its token's position:
+ *   t = positions[axis[i]][token] * turns[i],  c = cos(2 pi t),  s = sin(2 pi t),  (a, b) -> (a c - b s, b c + a s)
+ * The pair's elements are i and i + rotary_dim / 2, or 2 i and 2 i + 1 if interleaved.  t is a product in fp64, cosine, sine and
+ * the turned elements are fp64 and are rounded to fp32 and then to the type: a row comes out the same wherever it stands, and
+ * positions of any size keep their angle to 2^-52 of the position's number of turns.  The other elements are copied.
+ * ------------------------------------------------------------------------------------- */
+typedef struct abq_rotary {
+    int rotary_dim;      /* a multiple of 16, at most head_dim */
+    int axes;            /* 1 .. 8: rows of positions, such as time, height and width */
+    int interleaved;
+    const double *turns; /* device, [rotary_dim / 2]: revolutions per position, base^(-2 i / rotary_dim) / (2 pi) and whatever scaling a model has */
+    const int32_t *axis; /* device, [rotary_dim / 2], each 0 .. axes - 1 (others count as the nearest of these); NULL: all 0 */
+} abq_rotary;
+
+/* Turns rows of q into q_out and of k into k_out: the same rows, in place, or others that do not overlap.  k (and k_out) may be
+ * NULL.  positions: device int32, axis a of token i at positions[a * position_stride + i]; position_stride >= the number of rows where there
+ * are several axes.  head_dim: a multiple of 16, at most 256. */
+abq_status abq_rotary_apply(const abq_rotary *rotary, const abq_rows *q, const abq_rows *q_out, int heads, const abq_rows *k, const abq_rows *k_out,
+                            int kv_heads, int head_dim, int dtype, const int32_t *positions, int64_t position_stride, void *stream);
+
+/* abq_rotary_apply and abq_kv_append in one launch: q is turned into q_out (both may be NULL), k into k_out if that is not NULL, and the
+ * turned rows of k, as they are rounded to dtype, and those of v are quantised into the cache as abq_kv_append does.  v must not overlap
+ * q_out or k_out. */
+abq_status abq_kv_append_rotary(const abq_kv_cache *cache, const abq_rotary *rotary, const abq_rows *q, const abq_rows *q_out, int heads,
+                                const abq_rows *k, const abq_rows *k_out, const abq_rows *v, int dtype, const int32_t *positions,
+                                int64_t position_stride, const int32_t *slots, void *stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Pages of sequences
+ *
+ * Which pages of the cache hold which sequence's tokens, kept on the device, so that steps of beam search, of drafts or of ordinary
+ * decoding can be captured whole.  One such table serves the caches of all layers, which have num_pages pages of page_size tokens each.
+ * Between calls: table[s * max_pages + j] is the page of tokens j * page_size .. of sequence s for j below
+ * ceil(lengths[s] / page_size), and -1 behind; refs[p] is the number of entries that name page p, 0 for a free one.  Initially every
+ * entry is -1, lengths and refs are 0.  Sequences may share pages.  The calls keep to the arrays whatever these hold.
+ * ------------------------------------------------------------------------------------- */
+typedef struct abq_kv_pages {
+    int seqs;      /* at most 8192 */
+    int max_pages; /* of a sequence; max_pages * page_size < 2^31 - 64 */
+    int page_size; /* as in abq_kv_cache */
+    int num_pages;
+    int32_t *table, *lengths, *refs; /* device: [seqs][max_pages], [seqs], [num_pages] */
+} abq_kv_pages;
+
+/* Sequence s becomes what sequence parents[s] was before the call (device, [seqs]): it has its length and shares its pages.  A parent
+ * outside 0 .. seqs - 1, such as -1, leaves the sequence empty.  Pages that nobody names any more are free. */
+abq_status abq_kv_pages_fork(const abq_kv_pages *pages, const int32_t *parents, void *stream);
+
+/* Gives sequence s room for counts[s] more tokens (device, [seqs]), or takes -counts[s] of its last tokens away.  Tokens to be written in a
+ * page that other entries name as well go to a copy of it.  Pages that were free before the call are handed out lowest first, in the order of the
+ * sequences, a copy's page before the further ones.  A sequence that would need more than max_pages is left as it is; so are the first
+ * one for which the free pages do not suffice and those behind it that need any.  Device arrays, written whole:
+ *   starts  [seqs + 1]  where the sequences' new tokens begin, one behind the other: sums of the positive counts (as q_starts), at most 2^31 - 1
+ *   granted [seqs]      counts[s], 0 for a sequence that was left as it was, -(tokens taken away)
+ *   copies  [seqs][2]   pages (from, to) to be copied in every layer's cache before anything is written to it, or -1, -1
+ *   slots   [rows]      the new tokens' places, for abq_kv_append; -1 for tokens that were not granted and behind the last one */
+abq_status abq_kv_pages_extend(const abq_kv_pages *pages, const int32_t *counts, int32_t *slots, int64_t rows, int32_t *starts, int32_t *granted,
+                               int32_t *copies, void *stream);
+
+/* Moves pages so that the live ones are the first: of n live pages, those behind page n - 1, in order, take the places of the free ones before it,
+ * in order.  moves (device, [num_pages / 2][2]): pages (from, to) to be copied in every layer's cache, -1, -1 behind the last. */
+abq_status abq_kv_pages_compact(const abq_kv_pages *pages, int32_t *moves, void *stream);
+
+/* Bounds of the keys of every page: see abq_kv_bound */
+typedef struct abq_kv_bounds {
+    int8_t *codes; /* [page][head][2][head_dim]: of the largest, of the smallest; abq_kv_bound_codes_bytes, 16-byte aligned */
+    float *scales; /* [page][head]; abq_kv_bound_scales_bytes */
+} abq_kv_bounds;
+
+/* Copies page pairs[i][0] to page pairs[i][1], i = 0 .. count - 1 (device; -1, or anything outside the cache: nothing is copied), with its bounds
+ * if there are any (bounds may be NULL).  No page may be written twice in one call, or written and read, unless it is copied to itself. */
+abq_status abq_kv_copy_pages(const abq_kv_cache *cache, const abq_kv_bounds *bounds, const int32_t *pairs, int64_t count, void *stream);
+
+/* ---------------------------------------------------------------------------------------
  * Attention
  *
  * out[i][h] = sum_t p[t] v[t][h / group] over the tokens t that query i sees, p = softmax(scale * q[i][h] . k[t][h / group]),
@@ -140,6 +216,49 @@ size_t abq_attn_workspace_bytes(const abq_attn_state *state);
 abq_status abq_attn_set_workspace(abq_attn_state *state, void *workspace, size_t bytes);
 
 abq_status abq_attn_exec(const abq_attn_state *state, void *stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Attention to chosen pages
+ *
+ * Every query looks at a few pages of its context, chosen by a bound of the scores that it can have there, and at the newest
+ * tokens.  The bound of a page and key head holds the largest and the smallest of each channel of its keys, as the cache
+ * holds them in fp32, 2 head_dim numbers that are quantised as one symmetric row of 8 bits: signed codes hi, lo, and a scale.
+ * ------------------------------------------------------------------------------------- */
+size_t abq_kv_bound_codes_bytes(const abq_kv_cache *cache);
+size_t abq_kv_bound_scales_bytes(const abq_kv_cache *cache);
+
+/* Writes the bounds of the pages whose last slot is among slots[0 .. count - 1] (device; slots outside the cache are passed over): called
+ * with the slots of each abq_kv_append behind it, it leaves bounds of all pages that are complete. */
+abq_status abq_kv_bound(const abq_kv_cache *cache, const abq_kv_bounds *bounds, const int32_t *slots, int64_t count, void *stream);
+
+/* Chooses pages.  Sequence s has context[s] tokens in the cache and rows q_starts[s] .. q_starts[s + 1] - 1 of q, of which the first max_q
+ * are dealt with.  Of its n = context[s] / page_size complete pages (at most max_pages), each row and key head gets `count`: all if there are
+ * no more, else the first `first`, the last `last` and those with the largest scores, lower pages before higher ones where scores are equal;
+ * first + last <= count.  With q quantised per row and head as a symmetric row of 8 bits, codes c and scale d,
+ *   score = max over the heads of the group (fp32(sum max(c, 0) hi + min(c, 0) lo) * d) * (the bound's scale),   in fp32,
+ * at least the largest q . k of the page but for the roundings to 8 bits.  A page that is not in the cache has the lowest score.
+ * blocks (device, int32 [rows of q][kv_heads][count]): the pages' numbers in the sequence, ascending, -1 behind the last.  Rows that are not
+ * dealt with keep what they hold.  max_pages <= 32768. */
+abq_status abq_attn_choose(const abq_kv_cache *cache, const abq_kv_bounds *bounds, const abq_rows *q, int dtype, int heads, const int32_t *page_table,
+                           int max_pages, const int32_t *context, const int32_t *q_starts, int seqs, int max_q, int first, int last, int count,
+                           int32_t *blocks, void *stream);
+
+/* Attention of drafted tokens as in abq_attn_tree_init, but of the context, row i and key head h see only the tokens of pages
+ * blocks[i][h][0 .. count - 1] (numbers that are not those of complete pages of the context name none; a page that is named
+ * twice counts twice) and those behind the last complete page.  count <= 32768. */
+typedef struct abq_sparse_state {
+    abq_attn_state attn;
+    const int32_t *blocks;
+    int count;
+} abq_sparse_state;
+abq_status abq_attn_sparse_init(const abq_kv_cache *cache, const abq_rows *q, const abq_rows *out, int dtype, int heads, const int32_t *page_table,
+                                int max_pages, const int32_t *context, const int32_t *q_starts, const uint64_t *mask, const int32_t *blocks, int count,
+                                int seqs, int max_q, int max_context, float scale, abq_sparse_state *state);
+
+/* As abq_attn_workspace_bytes, abq_attn_set_workspace and abq_attn_exec */
+size_t abq_attn_sparse_workspace_bytes(const abq_sparse_state *state);
+abq_status abq_attn_sparse_set_workspace(abq_sparse_state *state, void *workspace, size_t bytes);
+abq_status abq_attn_sparse_exec(const abq_sparse_state *state, void *stream);
 
 #ifdef __cplusplus
 }
