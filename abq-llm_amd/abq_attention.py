@@ -8,6 +8,7 @@ import ctypes
 import importlib.util
 import math
 import os
+import struct
 import sys
 
 if "abq_gemm" not in sys.modules:
@@ -27,7 +28,7 @@ EXPORTED = [
     "abq_attn_prompt_init", "abq_attn_tree_init", "abq_attn_workspace_bytes", "abq_attn_set_workspace", "abq_attn_exec",
     "abq_rotary_apply", "abq_kv_append_rotary",
     "abq_kv_pages_fork", "abq_kv_pages_extend", "abq_kv_pages_compact", "abq_kv_copy_pages",
-    "abq_kv_bound_codes_bytes", "abq_kv_bound_scales_bytes", "abq_kv_bound", "abq_attn_choose",
+    "abq_kv_bound_codes_bytes", "abq_kv_bound_scales_bytes", "abq_kv_bound", "abq_attn_choose_workspace_bytes", "abq_attn_choose",
     "abq_attn_sparse_init", "abq_attn_sparse_workspace_bytes", "abq_attn_sparse_set_workspace", "abq_attn_sparse_exec",
 ]
 
@@ -93,8 +94,9 @@ def lib():
         L.abq_attn_set_workspace.argtypes = [P(AttnState), vp, ctypes.c_size_t]
         L.abq_attn_exec.argtypes = [P(AttnState), vp]
         i64 = ctypes.c_int64
-        L.abq_rotary_apply.argtypes = [P(RotaryDesc), P(Rows), P(Rows), ci, P(Rows), P(Rows), ci, ci, ci, vp, i64, vp]
-        L.abq_kv_append_rotary.argtypes = [P(KvCacheDesc), P(RotaryDesc), P(Rows), P(Rows), ci, P(Rows), P(Rows), P(Rows), ci, vp, i64, vp, vp]
+        # (rows as structures or as their bytes)
+        L.abq_rotary_apply.argtypes = [P(RotaryDesc), vp, vp, ci, vp, vp, ci, ci, ci, vp, i64, vp]
+        L.abq_kv_append_rotary.argtypes = [P(KvCacheDesc), P(RotaryDesc), vp, vp, ci, vp, vp, vp, ci, vp, i64, vp, vp]
         L.abq_kv_pages_fork.argtypes = [P(KvPagesDesc), vp, vp]
         L.abq_kv_pages_extend.argtypes = [P(KvPagesDesc), vp, vp, i64, vp, vp, vp, vp]
         L.abq_kv_pages_compact.argtypes = [P(KvPagesDesc), vp, vp]
@@ -103,7 +105,9 @@ def lib():
             getattr(L, name).argtypes = [P(KvCacheDesc)]
             getattr(L, name).restype = ctypes.c_size_t
         L.abq_kv_bound.argtypes = [P(KvCacheDesc), P(KvBoundsDesc), vp, i64, vp]
-        L.abq_attn_choose.argtypes = [P(KvCacheDesc), P(KvBoundsDesc), P(Rows), ci, ci, vp, ci, vp, vp, ci, ci, ci, ci, ci, vp, vp]
+        L.abq_attn_choose_workspace_bytes.argtypes = [P(KvCacheDesc), ci, ci, ci, ci]
+        L.abq_attn_choose_workspace_bytes.restype = ctypes.c_size_t
+        L.abq_attn_choose.argtypes = [P(KvCacheDesc), P(KvBoundsDesc), P(Rows), ci, ci, vp, ci, vp, vp, ci, ci, ci, ci, ci, ci, vp, vp, ctypes.c_size_t, vp]
         L.abq_attn_sparse_init.argtypes = [P(KvCacheDesc), P(Rows), P(Rows), ci, ci, vp, ci, vp, vp, vp, vp, ci, ci, ci, ci, ctypes.c_float, P(SparseState)]
         L.abq_attn_sparse_workspace_bytes.argtypes = [P(SparseState)]
         L.abq_attn_sparse_workspace_bytes.restype = ctypes.c_size_t
@@ -135,6 +139,21 @@ def _rows(t):
     if strides[2] != 1:
         raise ValueError("the elements of a head have to lie beside each other")
     return Rows(t.data_ptr(), t.shape[0], strides[0], strides[1])
+
+
+_ROWS = struct.Struct("Pqqq").pack
+
+
+def _row_bytes(t):
+    """The same as the bytes of the structure, which take less time to make"""
+    if t is None:
+        return None
+    strides = t.stride()
+    if len(strides) != 3 or not t.is_cuda:
+        raise ValueError("a device tensor [rows, heads, head dim] is wanted")
+    if strides[2] != 1:
+        raise ValueError("the elements of a head have to lie beside each other")
+    return _ROWS(t.data_ptr(), t.shape[0], strides[0], strides[1])
 
 
 def _index(t, dtype, numel, what):
@@ -217,11 +236,11 @@ class Rotary(_OnStream):
 
     def _positions(self, positions, tokens):
         """(address, stride) of positions int32 [tokens], or [axes, tokens] with the tokens beside each other"""
-        if positions.dim() == 1:
-            positions = positions[None]
-        if not positions.is_cuda or positions.dtype != torch.int32 or positions.shape != (self.axes, tokens) or (tokens > 1 and positions.stride(1) != 1):
+        shape, strides = tuple(positions.shape), positions.stride()
+        if shape != (self.axes, tokens) and (shape != (tokens,) or self.axes > 1) or not positions.is_cuda or positions.dtype != torch.int32 or (
+                tokens > 1 and strides[-1] != 1):
             raise ValueError("positions: a device tensor [%d, %d] of torch.int32 is wanted" % (self.axes, tokens))
-        return positions.data_ptr(), positions.stride(0) if self.axes > 1 else tokens
+        return positions.data_ptr(), strides[0] if self.axes > 1 else tokens
 
     def apply(self, q, k, positions, out=None, stream=None):
         """(q, k) turned, [tokens, heads, dim] each, into out = (q, k), which may be q and k themselves; k may be None."""
@@ -235,9 +254,8 @@ class Rotary(_OnStream):
             if (x is None) != (y is None) or (x is not None and (x.shape != y.shape or x.dtype is not y.dtype)):
                 raise ValueError("out has to be of the inputs' shapes and type")
         at, step = self._positions(positions, q.shape[0])
-        rows = [None if t is None else ctypes.byref(_rows(t)) for t in (q, out[0], k, out[1])]
-        _check(lib().abq_rotary_apply(self._ref, rows[0], rows[1], q.shape[1], rows[2], rows[3], 0 if k is None else k.shape[1], q.shape[2], _dtype(q), at,
-                                      step, on), "abq_rotary_apply")
+        _check(lib().abq_rotary_apply(self._ref, _row_bytes(q), _row_bytes(out[0]), q.shape[1], _row_bytes(k), _row_bytes(out[1]),
+                                      0 if k is None else k.shape[1], q.shape[2], _dtype(q), at, step, on), "abq_rotary_apply")
         return out
 
 
@@ -257,16 +275,19 @@ class PageTable(_OnStream):
         self.lengths, self.refs = (torch.zeros(n, dtype=torch.int32, device=device) for n in (sequences, num_pages))
         self.desc = KvPagesDesc(sequences, max_pages, page_size, num_pages, *(t.data_ptr() for t in (self.table, self.lengths, self.refs)))
         self._ref = ctypes.byref(self.desc)
+        self._extend, self._fork = lib().abq_kv_pages_extend, lib().abq_kv_pages_fork
         self._memory = _Memory((self.table, self.lengths, self.refs))
 
-    def _made(self, shapes, stream):
-        with torch.cuda.stream(None if stream is None else _stream_of(stream)):
-            return [torch.empty(s, dtype=torch.int32, device=self.table.device) for s in shapes]
+    def _made(self, numbers, stream):
+        if stream is None:
+            return torch.empty(numbers, dtype=torch.int32, device=self.table.device)
+        with torch.cuda.stream(_stream_of(stream)):  # (a tensor of the stream that it is written on)
+            return torch.empty(numbers, dtype=torch.int32, device=self.table.device)
 
     def fork(self, parents, stream=None):
         """Sequence s takes over the tokens of sequence parents[s] (int32 [sequences]; -1: none) as they were before, on the same pages."""
         at, on = _index(parents, torch.int32, self.desc.seqs, "parents"), self._on(stream)
-        _check(lib().abq_kv_pages_fork(self._ref, at, on), "abq_kv_pages_fork")
+        _check(self._fork(self._ref, at, on), "abq_kv_pages_fork")
 
     def extend(self, counts, rows, out=None, stream=None):
         """Room for counts[s] more tokens in sequence s (int32 [sequences]), or counts[s] < 0 taken away.  Returns, or fills out with, an
@@ -274,15 +295,20 @@ class PageTable(_OnStream):
         [sequences, 2], the pages that KvCache.copy_pages has to copy in every layer before anything is written."""
         n = self.desc.seqs
         at, on = _index(counts, torch.int32, n, "counts"), self._on(stream)
-        out = out or Extension(*self._made([(rows,), (n + 1,), (n,), (n, 2)], stream))
-        to = [_index(t, torch.int32, m, name) for t, m, name in zip(out, (rows, n + 1, n, 2 * n), Extension._fields)]
-        _check(lib().abq_kv_pages_extend(self._ref, at, to[0], rows, *to[1:], on), "abq_kv_pages_extend")
+        if out is None:  # (one piece of memory: four of their own take longer than the call)
+            whole = self._made(rows + 4 * n + 1, stream)
+            slots, starts, granted, copies = whole.split((rows, n + 1, n, 2 * n))
+            out, first = Extension(slots, starts, granted, copies.view(n, 2)), whole.data_ptr()
+            to = (first, first + 4 * rows, first + 4 * (rows + n + 1), first + 4 * (rows + 2 * n + 1))
+        else:
+            to = [_index(t, torch.int32, m, name) for t, m, name in zip(out, (rows, n + 1, n, 2 * n), Extension._fields)]
+        _check(self._extend(self._ref, at, to[0], rows, to[1], to[2], to[3], on), "abq_kv_pages_extend")
         return out
 
     def compact(self, out=None, stream=None):
         """Moves the live pages to the front; returns (or fills out with) moves [num_pages // 2, 2] for KvCache.copy_pages of every layer."""
         on, half = self._on(stream), self.desc.num_pages // 2
-        out = self._made([(half, 2)], stream)[0] if out is None else out
+        out = self._made(2 * half, stream).view(half, 2) if out is None else out
         _check(lib().abq_kv_pages_compact(self._ref, _index(out, torch.int32, 2 * half, "moves"), on), "abq_kv_pages_compact")
         return out
 
@@ -308,7 +334,7 @@ class KvCache(_OnStream):
         d.k_codes, d.v_codes, d.k_scales, d.v_scales = (t.data_ptr() for t in (self.k_codes, self.v_codes, self.k_scales, self.v_scales))
         self.desc = d
         self._ref, self._row = ctypes.byref(d), (kv_heads, head_dim)
-        self._append, self._read = lib().abq_kv_append, lib().abq_kv_read
+        self._append, self._read, self._append_rotary = lib().abq_kv_append, lib().abq_kv_read, lib().abq_kv_append_rotary
         held = (self.k_codes, self.v_codes, self.k_scales, self.v_scales)
         self.bounds = self._bounds = None
         if bounds:
@@ -348,22 +374,28 @@ class KvCache(_OnStream):
     def append_rotated(self, rotary, q, k, v, positions, slots, q_out=None, k_out=None, stream=None):
         """Turns q and k by their positions and appends the turned k and v, in one launch.  Returns (q_out, k_out): the turned q, in a new
         tensor by default (None without q), and the turned k if k_out is given (the same tensors as q and k turn them in place)."""
-        if k.shape != v.shape or k.dtype is not v.dtype or k.shape[1:] != self._row:
+        shape, dtype = k.shape, k.dtype
+        if shape != v.shape or dtype is not v.dtype or shape[1:] != self._row:
             raise ValueError("keys and values [tokens, %d, %d] of one type are wanted" % self._row)
-        if q is not None and (q.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or q.dtype is not k.dtype):
-            raise ValueError("q [%d, heads, %d] of the keys' type is wanted" % (k.shape[0], k.shape[2]))
-        if q is not None and q_out is None:
-            with torch.cuda.stream(None if stream is None else _stream_of(stream)):
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        heads = 0
+        if q is not None:
+            if q.dim() != 3 or q.dtype is not dtype or q.shape[::2] != shape[::2]:
+                raise ValueError("q [%d, heads, %d] of the keys' type is wanted" % shape[::2])
+            heads = q.shape[1]
+            if q_out is None:
+                with torch.cuda.stream(None if stream is None else _stream_of(stream)):
+                    q_out = torch.empty(q.shape, dtype=dtype, device=q.device)
         for x, y in ((q, q_out), (k, k_out)):
-            if y is not None and (x is None or x.shape != y.shape or x.dtype is not y.dtype):
+            if y is not None and (x is None or x.shape != y.shape or y.dtype is not dtype):
                 raise ValueError("q_out and k_out have to be of the inputs' shapes and type")
-        at, on = _index(slots, torch.int32, k.shape[0], "slots"), self._on(stream)
-        rotary._on(stream)
-        turns, step = rotary._positions(positions, k.shape[0])
-        rows = [None if t is None else ctypes.byref(_rows(t)) for t in (q, q_out, k, k_out, v)]
-        _check(lib().abq_kv_append_rotary(self._ref, rotary._ref, rows[0], rows[1], 0 if q is None else q.shape[1], rows[2], rows[3], rows[4], _dtype(k),
-                                          turns, step, at, on), "abq_kv_append_rotary")
+        at, on = _index(slots, torch.int32, shape[0], "slots"), self._on(stream)
+        if on.value not in rotary._memory.known:
+            rotary._memory.use(stream)
+        turns, step = rotary._positions(positions, shape[0])
+        status = self._append_rotary(self._ref, rotary._ref, _row_bytes(q), _row_bytes(q_out), heads, _row_bytes(k), _row_bytes(k_out), _row_bytes(v), _dtype(k),
+                                     turns, step, at, on)
+        if status:
+            raise AbqError(status, "abq_kv_append_rotary")
         return q_out, k_out
 
     def copy_pages(self, pairs, stream=None):
@@ -505,10 +537,14 @@ class SparseAttention(_Attention):
         _check(lib().abq_attn_sparse_init(ctypes.byref(d), ctypes.byref(rows[0]), ctypes.byref(rows[1]), _dtype(q), q.shape[1], table, page_table.shape[-1],
                                           at[1], at[2], None if mask is None else _index(mask, torch.int64, q.shape[0], "mask"), at[0], count, seqs, max_q,
                                           max_context, q.shape[2] ** -0.5 if scale is None else scale, ctypes.byref(self.state)), "abq_attn_sparse_init")
-        self._chosen = (ctypes.byref(d), cache._bounds, ctypes.byref(rows[0]), _dtype(q), q.shape[1], table, page_table.shape[-1], at[1], at[2], seqs, max_q,
-                        first, last, count, at[0])
-        if self._choose and page_table.shape[-1] > 32768:
-            raise AbqError(abq_gemm.ABQ_ERR_TOO_LARGE, "abq_attn_choose")
+        if self._choose:
+            if page_table.shape[-1] > 32768:
+                raise AbqError(abq_gemm.ABQ_ERR_TOO_LARGE, "abq_attn_choose")
+            need = lib().abq_attn_choose_workspace_bytes(ctypes.byref(d), page_table.shape[-1], seqs, max_q, max_context)
+            scores = torch.empty(need // 4, dtype=torch.int32, device=q.device) if need else None
+            made += (scores,) if need else ()
+            self._chosen = (ctypes.byref(d), cache._bounds, ctypes.byref(rows[0]), _dtype(q), q.shape[1], table, page_table.shape[-1], at[1], at[2], seqs, max_q,
+                            max_context, first, last, count, at[0], scores.data_ptr() if need else None, need)
         self._finish(out, workspace, *made, *cache._memory.tensors)
 
     def run(self, stream=None):

@@ -61,6 +61,8 @@ abq_status check_bounds(const abq_kv_bounds *b)
     return b && b->codes && b->scales && aligned16(b->codes) && aligned(b->scales, 4) ? ABQ_OK : ABQ_ERR_INVALID_ARG;
 }
 
+int likely_pages(const abq_kv_cache *c, int max_pages, int max_context) { return max_context / c->page_size < max_pages ? max_context / c->page_size : max_pages; }
+
 bool sparse_ready(const abq_sparse_state &st) { return st.attn.init_success && st.attn.kind == kSparseKind; }
 
 } // namespace
@@ -205,27 +207,36 @@ abq_status abq_kv_bound(const abq_kv_cache *cache, const abq_kv_bounds *bounds, 
         return s;
     if (count < 0 || (count && !slots))
         return ABQ_ERR_INVALID_ARG;
-    if (product((count + 15) / 16, (cache->kv_heads + 3) / 4, 1) > kMostBlocks)
+    if (product(count / 8 + 1, (cache->kv_heads + 3) / 4, 1) > kMostBlocks)
         return ABQ_ERR_TOO_LARGE;
     return hip_status(launch_kv_bound(*cache, *bounds, slots, count, (hipStream_t)stream));
 }
 
+size_t abq_attn_choose_workspace_bytes(const abq_kv_cache *cache, int max_pages, int seqs, int max_q, int max_context)
+{
+    if (!cache_sizes_valid(cache) || max_pages <= 0 || max_pages > kMostChosen || seqs <= 0 || max_q <= 0 || max_context < 0)
+        return 0;
+    return choose_workspace_bytes(product(seqs, max_q, cache->kv_heads), max_pages, likely_pages(cache, max_pages, max_context));
+}
+
 abq_status abq_attn_choose(const abq_kv_cache *cache, const abq_kv_bounds *bounds, const abq_rows *q, int dtype, int heads, const int32_t *page_table,
-                           int max_pages, const int32_t *context, const int32_t *q_starts, int seqs, int max_q, int first, int last, int count,
-                           int32_t *blocks, void *stream)
+                           int max_pages, const int32_t *context, const int32_t *q_starts, int seqs, int max_q, int max_context, int first, int last, int count,
+                           int32_t *blocks, void *workspace, size_t workspace_bytes, void *stream)
 {
     abq_status s = check_cache(cache);
     if (s != ABQ_OK || (s = check_bounds(bounds)) != ABQ_OK)
         return s;
     if (!q || q->rows < 0 || !dtype_valid(dtype) || heads <= 0 || heads % cache->kv_heads || !page_table || max_pages <= 0 || !context || !q_starts ||
-        seqs <= 0 || max_q <= 0 || first < 0 || last < 0 || count <= 0 || (int64_t)first + last > count || (q->rows && !blocks))
+        seqs <= 0 || max_q <= 0 || max_context < 0 || first < 0 || last < 0 || count <= 0 || (int64_t)first + last > count || (q->rows && !blocks) ||
+        (workspace_bytes && !workspace) || !aligned(workspace, 4))
         return ABQ_ERR_INVALID_ARG;
     if ((s = check_rows(q, q->rows, heads, cache->head_dim)) != ABQ_OK)
         return s;
     if (max_pages > kMostChosen || count > kMostChosen || q->rows > 0x7ffffff0 || (int64_t)max_pages * cache->page_size > 0x7fffffff - 64 ||
-        product(product(seqs, max_q, cache->kv_heads), 512, 1) > kMostThreads)
+        product(product(seqs, max_q, cache->kv_heads), 1024, 1) > kMostThreads)
         return ABQ_ERR_TOO_LARGE;
-    return hip_status(launch_attn_choose({*cache, *bounds, *q, dtype, heads, page_table, context, q_starts, max_pages, seqs, max_q, first, last, count, blocks},
+    return hip_status(launch_attn_choose({*cache, *bounds, *q, dtype, heads, page_table, context, q_starts, max_pages, seqs, max_q, first, last, count,
+                                          likely_pages(cache, max_pages, max_context), blocks, workspace, workspace_bytes},
                                          (hipStream_t)stream));
 }
 

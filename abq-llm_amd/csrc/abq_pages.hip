@@ -127,38 +127,31 @@ __device__ __forceinline__ int owner_of(const int32_t *ends, int seqs, int r)
     return lo;
 }
 
-__device__ __forceinline__ void write_slot(const PagesArgs &a, int32_t *slots, const int32_t *starts, const int32_t *granted, int64_t row)
+// The last sequence that starts at or before the row, of starts[0 .. seqs] with the row in front of the last
+__device__ __forceinline__ int sequence_of(const int32_t *starts, int seqs, int64_t row)
 {
-    // the sequence: the last one that starts at or before the row
-    int slot = -1;
-    if (row < starts[a.seqs]) {
-        int lo = 0, hi = a.seqs - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (starts[mid] <= row)
-                lo = mid;
-            else
-                hi = mid - 1;
-        }
-        if (granted[lo] > 0) {
-            const int place = a.lengths[lo] - granted[lo] + (int)(row - starts[lo]);
-            const int page = a.table[(int64_t)lo * a.max_pages + (place >> a.page_shift)];
-            slot = (page << a.page_shift) + (place & ((1 << a.page_shift) - 1));
-        }
+    int lo = 0, hi = seqs - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (starts[mid] <= row)
+            lo = mid;
+        else
+            hi = mid - 1;
     }
-    slots[row] = slot;
+    return lo;
+}
+__device__ __forceinline__ int slot_of(const PagesArgs &a, int s, int place)
+{
+    return (a.table[(int64_t)s * a.max_pages + (place >> a.page_shift)] << a.page_shift) + (place & ((1 << a.page_shift) - 1));
 }
 
-// Pages behind the length of a sequence that has become shorter, by a wave
-__device__ __forceinline__ void release(const PagesArgs &a, int s, int taken, int lane)
+// Page number j of a sequence that has become shorter
+__device__ __forceinline__ void release(const PagesArgs &a, int s, int j)
 {
-    const int length = a.lengths[s], to = pages_of(a, length + taken);
-    for (int j = pages_of(a, length) + lane; j < to; j += 64) {
-        int32_t *entry = a.table + (int64_t)s * a.max_pages + j;
-        if (is_page(a, *entry))
-            atomicSub(&a.refs[*entry], 1);
-        *entry = -1;
-    }
+    int32_t *entry = a.table + (int64_t)s * a.max_pages + j;
+    if (is_page(a, *entry))
+        atomicSub(&a.refs[*entry], 1);
+    *entry = -1;
 }
 
 struct ExtendArgs {
@@ -168,52 +161,58 @@ struct ExtendArgs {
     int64_t rows;
 };
 
-// Everything that is decided in order.  `all`: also what the second launch would do.
+// Everything that is decided in order, each sequence a thread's.  `all`: also what the second launch would do.
 __global__ __launch_bounds__(kScan) void pages_extend_kernel(ExtendArgs e, int all)
 {
     const PagesArgs &a = e.p;
     __shared__ int32_t ends[kMostSeqs]; // of the pages that sequences 0 .. s need, capped at kCapped
+    __shared__ int32_t starts[kMostSeqs], lengths[kMostSeqs]; // of their new tokens; before the call
     __shared__ uint8_t flags[kMostSeqs];
-    __shared__ int64_t sums[2][kScan / 64];
+    __shared__ int64_t sums[2][2][kScan / 64];
     __shared__ int32_t counted[2][kScan / 64];
     constexpr int32_t kCapped = 0x7fffffff; // (more than there can be pages)
-    constexpr int kCopied = 1, kNeeds = 2, kGrows = 4;
-    const int per = (a.seqs + kScan - 1) / kScan, s0 = threadIdx.x * per, s1 = min(s0 + per, a.seqs);
-    int64_t need = 0, grow = 0;
-    for (int s = s0; s < s1; ++s) {
-        const Wish w = wish_of(a, e.counts, s);
-        need += w.pages;
-        grow += w.grow;
+    constexpr int kCopied = 1, kNeeds = 2, kGrows = 4, kGiven = 8, kShrinks = 16;
+    // (the first pages' counts are asked for ahead of everything that waits for something else)
+    const bool wide = ((uintptr_t)a.refs & 15) == 0;
+    auto counts_of = [&](int p0) {
+        if (wide && p0 + 3 < a.num_pages)
+            return *(const int4 *)(a.refs + p0);
+        return int4{p0 < a.num_pages ? a.refs[p0] : 1, p0 + 1 < a.num_pages ? a.refs[p0 + 1] : 1, p0 + 2 < a.num_pages ? a.refs[p0 + 2] : 1,
+                    p0 + 3 < a.num_pages ? a.refs[p0 + 3] : 1};
+    };
+    int4 refs = counts_of(4 * threadIdx.x);
+    int64_t all_need = 0, all_grow = 0;
+    for (int s0 = 0, round = 0; s0 < a.seqs; s0 += kScan, ++round) {
+        const int s = s0 + threadIdx.x;
+        Wish w = {};
+        if (s < a.seqs)
+            w = wish_of(a, e.counts, s);
+        int64_t here_need, here_grow;
+        const int64_t need = all_need + scan(w.pages, sums[round & 1][0], &here_need), grow = all_grow + scan((int64_t)w.grow, sums[round & 1][1], &here_grow);
+        if (s < a.seqs) {
+            ends[s] = (int32_t)min(need + w.pages, (int64_t)kCapped);
+            starts[s] = e.starts[s] = (int32_t)min(grow, (int64_t)kCapped);
+            lengths[s] = w.length;
+            flags[s] = (w.copied ? kCopied : 0) | (w.pages > 0 ? kNeeds : 0) | (w.grow > 0 && w.fits ? kGrows : 0);
+            if (w.copied)
+                e.copies[2 * s] = w.last;
+        }
+        all_need += here_need;
+        all_grow += here_grow;
     }
-    int64_t all_need, all_grow;
-    int64_t before = scan(need, sums[0], &all_need), start = scan(grow, sums[1], &all_grow);
-    for (int s = s0; s < s1; ++s) {
-        const Wish w = wish_of(a, e.counts, s);
-        e.starts[s] = (int32_t)min(start, (int64_t)kCapped);
-        start += w.grow;
-        before += w.pages;
-        ends[s] = (int32_t)min(before, (int64_t)kCapped);
-        flags[s] = (w.copied ? kCopied : 0) | (w.pages > 0 ? kNeeds : 0) | (w.grow > 0 && w.fits ? kGrows : 0);
-        e.copies[2 * s] = w.copied ? w.last : -1;
-    }
+    const int tokens = (int)min(all_grow, (int64_t)kCapped);
     if (threadIdx.x == 0)
-        e.starts[a.seqs] = (int32_t)min(all_grow, (int64_t)kCapped);
+        e.starts[a.seqs] = tokens;
     __syncthreads();
     // Free pages, in order, as the next ones of the sequences, until there are enough or no more.  One sequence at most gets only a
     // part of its pages, and gives them back below.
     const int64_t wanted = min(all_need, (int64_t)a.num_pages);
-    const bool wide = ((uintptr_t)a.refs & 15) == 0;
     int found = 0;
     for (int base = 0, round = 0; base < a.num_pages && found < wanted; base += 4 * kScan, ++round) {
         const int p0 = base + 4 * threadIdx.x;
-        bool free[4];
-        if (wide && p0 + 3 < a.num_pages) {
-            const int4 r = *(const int4 *)(a.refs + p0);
-            free[0] = r.x == 0, free[1] = r.y == 0, free[2] = r.z == 0, free[3] = r.w == 0;
-        } else
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                free[i] = p0 + i < a.num_pages && a.refs[p0 + i] == 0;
+        if (round > 0)
+            refs = counts_of(p0);
+        const bool free[4] = {refs.x == 0, refs.y == 0, refs.z == 0, refs.w == 0};
         int32_t here;
         int r = found + scan((int32_t)free[0] + free[1] + free[2] + free[3], counted[round & 1], &here);
 #pragma unroll
@@ -221,7 +220,7 @@ __global__ __launch_bounds__(kScan) void pages_extend_kernel(ExtendArgs e, int a
             if (!free[i] || r >= wanted)
                 continue;
             const int s = owner_of(ends, a.seqs, r);
-            const int64_t column = (int64_t)pages_of(a, length_of(a, s)) - (flags[s] & kCopied) + r - (s ? ends[s - 1] : 0);
+            const int64_t column = (int64_t)pages_of(a, lengths[s]) - (flags[s] & kCopied) + r - (s ? ends[s - 1] : 0);
             if (ends[s] < kCapped && column < a.max_pages) {
                 a.table[(int64_t)s * a.max_pages + column] = p0 + i;
                 a.refs[p0 + i] = 1;
@@ -231,8 +230,8 @@ __global__ __launch_bounds__(kScan) void pages_extend_kernel(ExtendArgs e, int a
         found += here;
     }
     __syncthreads();
-    for (int s = s0; s < s1; ++s) {
-        const int length = length_of(a, s), count = e.counts[s], first = s ? ends[s - 1] : 0, f = flags[s];
+    for (int s = threadIdx.x; s < a.seqs; s += kScan) {
+        const int length = lengths[s], count = e.counts[s], first = s ? ends[s - 1] : 0, f = flags[s];
         const int64_t column = (int64_t)pages_of(a, length) - (f & kCopied);
         int32_t *entry = a.table + (int64_t)s * a.max_pages + column;
         const bool given = (f & kGrows) && (!(f & kNeeds) || ends[s] <= found);
@@ -250,29 +249,64 @@ __global__ __launch_bounds__(kScan) void pages_extend_kernel(ExtendArgs e, int a
         const int granted = given ? count : count < 0 ? -(int)min(-(int64_t)count, (int64_t)length) : 0;
         e.granted[s] = granted;
         a.lengths[s] = length + granted;
+        if (all && granted < 0) {
+            const int to = pages_of(a, length), kept = pages_of(a, length + granted);
+            if (to - kept <= 4)
+                for (int j = kept; j < to; ++j)
+                    release(a, s, j);
+            else
+                flags[s] = kShrinks;
+        } else if (all && given)
+            flags[s] = kGiven;
     }
     if (!all)
         return;
     __syncthreads();
-    for (int64_t row = threadIdx.x; row < e.rows; row += kScan)
-        write_slot(a, e.slots, e.starts, e.granted, row);
-    for (int s = threadIdx.x >> 6; s < a.seqs; s += kScan / 64)
-        if (e.granted[s] < 0)
-            release(a, s, -e.granted[s], threadIdx.x & 63);
+    for (int64_t row = threadIdx.x; row < e.rows; row += kScan) {
+        int slot = -1;
+        if (row < tokens) {
+            const int s = sequence_of(starts, a.seqs, row);
+            if (flags[s] == kGiven)
+                slot = slot_of(a, s, lengths[s] + (int)(row - starts[s]));
+        }
+        e.slots[row] = slot;
+    }
+    // sequences that have lost many pages, a wave each
+    const int lane = threadIdx.x & 63;
+    for (int s0 = threadIdx.x & ~63; s0 < a.seqs; s0 += kScan) {
+        const int s1 = s0 + lane;
+        uint64_t many = __ballot(s1 < a.seqs && flags[min(s1, a.seqs - 1)] == kShrinks);
+        for (; many; many &= many - 1) {
+            const int s = s0 + __builtin_ctzll(many), to = pages_of(a, lengths[s]);
+            for (int j = pages_of(a, a.lengths[s]) + lane; j < to; j += 64)
+                release(a, s, j);
+        }
+    }
 }
 
 // What follows from it: slots, and the pages of sequences that have become shorter, a wave each, by the workgroups behind the slots'
 __global__ __launch_bounds__(256) void pages_slots_kernel(ExtendArgs e, uint32_t slot_blocks)
 {
+    const PagesArgs &a = e.p;
     if (blockIdx.x < slot_blocks) {
         const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
-        if (row < e.rows)
-            write_slot(e.p, e.slots, e.starts, e.granted, row);
+        if (row >= e.rows)
+            return;
+        int slot = -1;
+        if (row < e.starts[a.seqs]) {
+            const int s = sequence_of(e.starts, a.seqs, row);
+            if (e.granted[s] > 0)
+                slot = slot_of(a, s, a.lengths[s] - e.granted[s] + (int)(row - e.starts[s]));
+        }
+        e.slots[row] = slot;
         return;
     }
     const int s = (blockIdx.x - slot_blocks) * 4 + (threadIdx.x >> 6);
-    if (s < e.p.seqs && e.granted[s] < 0)
-        release(e.p, s, -e.granted[s], threadIdx.x & 63);
+    if (s < a.seqs && e.granted[s] < 0) {
+        const int to = pages_of(a, a.lengths[s] - e.granted[s]);
+        for (int j = pages_of(a, a.lengths[s]) + (threadIdx.x & 63); j < to; j += 64)
+            release(a, s, j);
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------------- compact
@@ -342,48 +376,44 @@ __global__ __launch_bounds__(256) void pages_rename_kernel(PagesArgs a, const in
 
 // ---------------------------------------------------------------------------------------------------------- copies
 
-// A cache's arrays, each so many 16-byte words a page; bounds' scales, whose pages may be of 4 bytes, by themselves
+// A cache's arrays, each so many 16-byte words a page and so many turns of a workgroup; bounds' scales, whose pages may be of 4 bytes, by
+// themselves, as the last turn's
+constexpr int kArrays = 5;
 struct CopyArgs {
-    uint4 *at[5];
-    int64_t words[5];
+    uint4 *at[kArrays];
+    int64_t words[kArrays];
+    int32_t turns[kArrays]; // up to and with this array
     float *scales;
     int heads, num_pages;
     const int32_t *pairs;
-    int splits;
+    int64_t each; // workgroups of a pair
 };
 
-constexpr int kCopyWords = 1024; // of a workgroup's turn: 16 KB, four words of a lane in flight
-
+// A turn is 4 KB, a word of a lane: with four words of a lane in 16 KB, 315 pages of 132 KB took 24 us instead of 15, three of 530 KB 10
+// instead of 2.5
 __global__ __launch_bounds__(256) void copy_pages_kernel(CopyArgs a)
 {
-    const int64_t pair = blockIdx.x / a.splits;
-    const int split = blockIdx.x % a.splits;
+    const int64_t pair = blockIdx.x / a.each;
     const int from = a.pairs[2 * pair], to = a.pairs[2 * pair + 1];
     if ((uint32_t)from >= (uint32_t)a.num_pages || (uint32_t)to >= (uint32_t)a.num_pages || from == to)
         return;
-    int turn = 0; // of all arrays' turns, those of this workgroup are every splits-th
+    for (int turn = (int)(blockIdx.x % a.each); turn < a.turns[kArrays - 1]; turn += (int)a.each) {
+        uint4 *at = a.at[0];
+        int64_t n = a.words[0], i = turn;
 #pragma unroll
-    for (int k = 0; k < 5; ++k) {
-        const int64_t n = a.words[k];
-        const uint4 *src = a.at[k] + from * n;
-        uint4 *dst = a.at[k] + to * n;
-        for (int64_t base = 0; base < n; base += kCopyWords, ++turn) {
-            if (turn % a.splits != split)
-                continue;
-            uint4 x[kCopyWords / 256];
-#pragma unroll
-            for (int i = 0; i < kCopyWords / 256; ++i)
-                if (base + 256 * i + threadIdx.x < n)
-                    x[i] = src[base + 256 * i + threadIdx.x];
-#pragma unroll
-            for (int i = 0; i < kCopyWords / 256; ++i)
-                if (base + 256 * i + threadIdx.x < n)
-                    dst[base + 256 * i + threadIdx.x] = x[i];
-        }
+        for (int k = 1; k < kArrays; ++k)
+            if (turn >= a.turns[k - 1]) {
+                at = a.at[k];
+                n = a.words[k];
+                i = turn - a.turns[k - 1];
+            }
+        i = i * 256 + threadIdx.x;
+        if (i < n)
+            at[to * n + i] = at[from * n + i];
+        if (a.scales && turn == a.turns[kArrays - 1] - 1)
+            for (int h = threadIdx.x; h < a.heads; h += 256)
+                a.scales[(int64_t)to * a.heads + h] = a.scales[(int64_t)from * a.heads + h];
     }
-    if (split == 0 && a.scales)
-        for (int i = threadIdx.x; i < a.heads; i += 256)
-            a.scales[(int64_t)to * a.heads + i] = a.scales[(int64_t)from * a.heads + i];
 }
 
 PagesArgs pages_args(const abq_kv_pages &p)
@@ -407,7 +437,7 @@ hipError_t launch_pages_extend(const abq_kv_pages &p, const int32_t *counts, int
 {
     const ExtendArgs e = {pages_args(p), counts, slots, starts, granted, copies, rows};
     // one launch where the workgroup that scans has little else to do
-    const int all = rows <= 2 * kScan && p.seqs <= 64;
+    const int all = rows <= 4 * kScan;
     hipLaunchKernelGGL(pages_extend_kernel, dim3(1), dim3(kScan), 0, stream, e, all);
     if (!all) {
         const uint32_t slot_blocks = (uint32_t)((rows + 255) / 256);
@@ -426,35 +456,26 @@ hipError_t launch_pages_compact(const abq_kv_pages &p, int32_t *moves, hipStream
     return hipGetLastError();
 }
 
-// Turns of a page's arrays
-static int copy_turns(const CopyArgs &a)
-{
-    int64_t turns = 0;
-    for (const int64_t n : a.words)
-        turns += (n + kCopyWords - 1) / kCopyWords;
-    return (int)turns;
-}
-
 hipError_t launch_copy_pages(const abq_kv_cache &c, const abq_kv_bounds *bounds, const int32_t *pairs, int64_t count, hipStream_t stream)
 {
     if (count == 0)
         return hipSuccess;
     CopyArgs a = {};
     const int64_t rows = (int64_t)c.page_size * c.kv_heads, codes = rows * c.head_dim * c.bits / 8 / 16, scales = rows * (c.symmetric ? 1 : 2) / 4;
-    void *at[5] = {c.k_codes, c.v_codes, c.k_scales, c.v_scales, bounds ? bounds->codes : nullptr};
-    const int64_t words[5] = {codes, codes, scales, scales, bounds ? (int64_t)c.kv_heads * 2 * c.head_dim / 16 : 0};
-    for (int i = 0; i < 5; ++i) {
+    void *at[kArrays] = {c.k_codes, c.v_codes, c.k_scales, c.v_scales, bounds ? bounds->codes : nullptr};
+    const int64_t words[kArrays] = {codes, codes, scales, scales, bounds ? (int64_t)c.kv_heads * 2 * c.head_dim / 16 : 0};
+    for (int i = 0; i < kArrays; ++i) {
         a.at[i] = (uint4 *)at[i];
         a.words[i] = words[i];
+        a.turns[i] = (i ? a.turns[i - 1] : 0) + (int)((words[i] + 255) / 256);
     }
     a.scales = bounds ? bounds->scales : nullptr;
     a.heads = c.kv_heads;
     a.num_pages = c.num_pages;
     a.pairs = pairs;
-    const int turns = copy_turns(a);
     const int64_t most = kMostBlocks / count;
-    a.splits = (int)(turns < most ? turns : most);
-    hipLaunchKernelGGL(copy_pages_kernel, dim3((unsigned)(count * a.splits)), dim3(256), 0, stream, a);
+    a.each = a.turns[kArrays - 1] < most ? a.turns[kArrays - 1] : most;
+    hipLaunchKernelGGL(copy_pages_kernel, dim3((unsigned)(count * a.each)), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 

@@ -184,32 +184,49 @@ template <int DTYPE, int BITS, int D, bool BESIDE> __global__ __launch_bounds__(
     Place at = {};
     if constexpr (BITS != 0)
         at = place_of(a, a.slots[token]);
-    auto turn = [&](const abq_rows &in, const abq_rows &out, int heads, int step, auto keys) {
+    // steps: rows of queries, then of keys
+    const int steps_q = (r.heads[0] + rows - 1) / rows, steps = steps_q + (r.heads[1] + rows - 1) / rows;
+    auto fetch = [&](int step, uint4 *lo, uint4 *hi) {
+        const bool keys = step >= steps_q;
+        const int head = (keys ? step - steps_q : step) * rows + mine;
+        const uint16_t *src = (const uint16_t *)(keys ? r.k.data : r.q.data) + token * (keys ? r.k.row_stride : r.q.row_stride) +
+                              (mine < rows && head < (keys ? r.heads[1] : r.heads[0]) ? head : 0) * (keys ? r.k.head_stride : r.q.head_stride);
+        *lo = *(const uint4 *)(src + p.e0);
+        *hi = *(const uint4 *)(src + p.e1);
+    };
+    auto turn = [&](uint4 lo0, uint4 hi0, const abq_rows &out, int heads, int step, auto keys) {
         const int head = step * rows + mine;
-        const bool there = mine < rows && head < heads;
-        const uint16_t *src = (const uint16_t *)in.data + token * in.row_stride + (there ? head : 0) * in.head_stride;
-        const uint4 lo0 = *(const uint4 *)(src + p.e0), hi0 = *(const uint4 *)(src + p.e1);
         uint4 lo = lo0, hi = hi0;
         turn16<DTYPE, BESIDE>(lo, hi, c, s);
         if (!p.turn) {
             lo.x = lo0.x, lo.y = lo0.y, lo.z = lo0.z, lo.w = lo0.w;
             hi.x = hi0.x, hi.y = hi0.y, hi.z = hi0.z, hi.w = hi0.w;
         }
-        if (there && out.data) {
+        if (mine >= rows || head >= heads) // (a row's lanes are there together)
+            return;
+        if (out.data) {
             uint16_t *dst = (uint16_t *)out.data + token * out.row_stride + head * out.head_stride;
             *(uint4 *)(dst + p.e0) = lo;
             *(uint4 *)(dst + p.e1) = hi;
         }
         if constexpr (BITS != 0 && decltype(keys)::value)
-            if (there) // (a row's lanes are there together)
-                append_key<DTYPE, BITS, D>(a, lo, hi, p, at, head, chunk == 0);
+            append_key<DTYPE, BITS, D>(a, lo, hi, p, at, head, chunk == 0);
     };
-    const int steps_q = (r.heads[0] + rows - 1) / rows, steps = steps_q + (r.heads[1] + rows - 1) / rows;
     int step = split;
-    for (; step < steps_q; step += r.splits)
-        turn(r.q, r.q_out, r.heads[0], step, std::false_type());
-    for (; step < steps; step += r.splits)
-        turn(r.k, r.k_out, r.heads[1], step - steps_q, std::true_type());
+    if (step >= steps)
+        return;
+    uint4 lo, hi, next_lo, next_hi;
+    fetch(step, &lo, &hi);
+    for (; step < steps; step += r.splits) {
+        if (step + r.splits < steps) // (rows in place are read before any other is written: each is one lane's)
+            fetch(step + r.splits, &next_lo, &next_hi);
+        if (step < steps_q)
+            turn(lo, hi, r.q_out, r.heads[0], step, std::false_type());
+        else
+            turn(lo, hi, r.k_out, r.heads[1], step - steps_q, std::true_type());
+        lo = next_lo;
+        hi = next_hi;
+    }
 }
 
 } // namespace

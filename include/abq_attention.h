@@ -238,10 +238,13 @@ abq_status abq_kv_bound(const abq_kv_cache *cache, const abq_kv_bounds *bounds, 
  *   score = max over the heads of the group (fp32(sum max(c, 0) hi + min(c, 0) lo) * d) * (the bound's scale),   in fp32,
  * at least the largest q . k of the page but for the roundings to 8 bits.  A page that is not in the cache has the lowest score.
  * blocks (device, int32 [rows of q][kv_heads][count]): the pages' numbers in the sequence, ascending, -1 behind the last.  Rows that are not
- * dealt with keep what they hold.  max_pages <= 32768. */
+ * dealt with keep what they hold.  max_pages <= 32768; max_context only guides how the work is split.  workspace: NULL, or a device buffer,
+ * 4-byte aligned, of abq_attn_choose_workspace_bytes (0: none is used), which nothing else may use while the call is under way; a smaller one is
+ * as none.  The choice is the same with and without. */
+size_t abq_attn_choose_workspace_bytes(const abq_kv_cache *cache, int max_pages, int seqs, int max_q, int max_context);
 abq_status abq_attn_choose(const abq_kv_cache *cache, const abq_kv_bounds *bounds, const abq_rows *q, int dtype, int heads, const int32_t *page_table,
-                           int max_pages, const int32_t *context, const int32_t *q_starts, int seqs, int max_q, int first, int last, int count,
-                           int32_t *blocks, void *stream);
+                           int max_pages, const int32_t *context, const int32_t *q_starts, int seqs, int max_q, int max_context, int first, int last, int count,
+                           int32_t *blocks, void *workspace, size_t workspace_bytes, void *stream);
 
 /* Attention of drafted tokens as in abq_attn_tree_init, but of the context, row i and key head h see only the tokens of pages
  * blocks[i][h][0 .. count - 1] (numbers that are not those of complete pages of the context name none; a page that is named

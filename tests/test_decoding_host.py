@@ -137,9 +137,10 @@ def test_bounds_and_the_choice_are_refused(attn):
     def bound(c={}, bounds=good, slots=A, count=3):
         return L.abq_kv_bound(ref(cache_desc(attn, **c)), ref(bounds), slots, count, None)
 
-    def choose(c={}, bounds=good, q={}, dtype=0, heads=2, table=A, max_pages=4, context=A, q_starts=A, seqs=2, max_q=3, first=1, last=1, count=3, blocks=A):
+    def choose(c={}, bounds=good, q={}, dtype=0, heads=2, table=A, max_pages=4, context=A, q_starts=A, seqs=2, max_q=3, max_context=100, first=1, last=1, count=3, blocks=A, workspace=None,
+               bytes=0):
         return L.abq_attn_choose(ref(cache_desc(attn, **c)), ref(bounds), ref(None if q is None else rows(attn, **q)), dtype, heads, table, max_pages, context, q_starts, seqs,
-                                 max_q, first, last, count, blocks, None)
+                                 max_q, max_context, first, last, count, blocks, workspace, bytes, None)
 
     for b in bad_bounds:
         assert bound(bounds=b) == ok.ABQ_ERR_INVALID_ARG and choose(bounds=b) == ok.ABQ_ERR_INVALID_ARG
@@ -148,12 +149,16 @@ def test_bounds_and_the_choice_are_refused(attn):
     assert bound(slots=None) == bound(count=-1) == ok.ABQ_ERR_INVALID_ARG and bound(count=1 << 40) == ok.ABQ_ERR_TOO_LARGE and bound(count=0, slots=None) == ok.ABQ_OK
     for kw in [{"q": b} for b in BAD_ROWS if "rows" not in b] + [{"q": {"rows": -1}}, {"q": None}, {"dtype": 3}, {"heads": 0}, {"heads": 3}, {"table": None}, {"max_pages": 0},
                                                                  {"context": None}, {"q_starts": None}, {"seqs": 0}, {"max_q": 0}, {"first": -1}, {"last": -1}, {"count": 0},
-                                                                 {"first": 2, "last": 2}, {"blocks": None}, {"first": 2 ** 31 - 1, "last": 2 ** 31 - 1}]:
+                                                                 {"first": 2, "last": 2}, {"blocks": None}, {"first": 2 ** 31 - 1, "last": 2 ** 31 - 1}, {"max_context": -1},
+                                                                 {"bytes": 8}, {"workspace": A + 2, "bytes": 8}]:
         assert choose(**kw) == ok.ABQ_ERR_INVALID_ARG, kw
     for kw in ({"max_pages": 32769}, {"count": 32769}, {"seqs": 1 << 22, "max_q": 64}, {"max_pages": 32768, "c": {"page_size": 4096, "num_pages": (1 << 19) - 1}, "seqs": 2 ** 31 - 1,
                                                                                      "max_q": 2 ** 31 - 1}):
         assert choose(**kw) == ok.ABQ_ERR_TOO_LARGE, kw
     assert choose(q={"rows": 0}, blocks=None) == ok.ABQ_OK
+    need = lambda *a, **c: L.abq_attn_choose_workspace_bytes(ref(cache_desc(attn, **c)), *a)  # noqa: E731
+    assert need(2000, 1, 1, 1500 * 64) == 2000 * 2 * 4 and need(2000, 1, 1, 100) == need(100, 1, 1, 10 ** 6) == need(2000, 999, 1, 10 ** 6) == 0
+    assert need(0, 1, 1, 10 ** 6) == need(32769, 1, 1, 10 ** 6) == need(2000, 1, 1, 10 ** 6, bits=3) == need(2000, 2 ** 31 - 1, 2 ** 31 - 1, 10 ** 6) == 0
 
 
 def sparse(attn, cache={}, q={}, out={}, dtype=0, heads=2, page_table=A, max_pages=4, context=A, q_starts=A, mask=A, blocks=A, count=3, seqs=2, max_q=10, max_context=100, scale=0.1):
@@ -243,8 +248,7 @@ def test_memory_of_the_objects_is_safe_on_other_streams(attn, monkeypatch):
         monkeypatch.setattr(torch, name, lambda *a, make=getattr(torch, name), device=None, **kw: make(*a, **kw))
     monkeypatch.setattr(torch.Tensor, "is_cuda", True)
     table = attn.PageTable(8, 16, 2, 3)
-    L = attn.lib()
-    monkeypatch.setattr(L, "abq_kv_pages_fork", lambda p, at, on: streams.log.append(("run", on.value)) or 0)
+    table._fork = table._extend = lambda *a: streams.log.append(("run", a[-1].value)) or 0
     other, parents = streams.Stream(streams, 0x20), torch.zeros(2, dtype=torch.int32)
     streams.taken()
     table.fork(parents, stream=streams.home)
@@ -255,6 +259,6 @@ def test_memory_of_the_objects_is_safe_on_other_streams(attn, monkeypatch):
     assert [e for e in log if e[0] != "keep"] == [("wait", 0x20, 0x10), ("run", 0x20)]
     table.fork(parents, stream=0x20)
     assert streams.taken() == [("run", 0x20)]
-    monkeypatch.setattr(L, "abq_kv_pages_extend", lambda *a: streams.log.append(("run", a[-1].value)) or 0)
-    table.extend(parents, 5, stream=other)
-    assert streams.taken() == [("made", 0x20)] * 4 + [("run", 0x20)]
+    given = table.extend(parents, 5, stream=other)
+    assert streams.taken() == [("made", 0x20), ("run", 0x20)]
+    assert [tuple(t.shape) for t in given] == [(5,), (3,), (2,), (2, 2)]

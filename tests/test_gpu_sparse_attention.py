@@ -1,4 +1,6 @@
 """Bounds of pages, the choice of pages by them, and attention to chosen pages, through the C ABI, against the formulas."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -78,11 +80,12 @@ def test_bounds_of_complete_pages(attn, bits, symmetric, dim, kv, size):
 
 # ---------------------------------------------------------------------------------------------- choice
 
-def chosen(attn, cache, q, table, context, lens, max_q, first, last, count, out):
-    import ctypes
+def chosen(attn, cache, q, table, context, lens, max_q, first, last, count, out, max_context=1 << 20, workspace=True):
+    need = attn.lib().abq_attn_choose_workspace_bytes(ctypes.byref(cache.desc), table.shape[1], context.numel(), max_q, max_context) if workspace else 0
+    scores = torch.full((need // 4 + 1,), -1, dtype=torch.int32, device="cuda")
     attn._check(attn.lib().abq_attn_choose(ctypes.byref(cache.desc), cache._bounds, ctypes.byref(attn._rows(q)), attn._dtype(q), q.shape[1], table.data_ptr(),
-                                           table.shape[1], context.data_ptr(), lens.data_ptr(), context.numel(), max_q, first, last, count, out.data_ptr(),
-                                           attn.abq_gemm._stream_ptr(None)), "abq_attn_choose")
+                                           table.shape[1], context.data_ptr(), lens.data_ptr(), context.numel(), max_q, max_context, first, last, count,
+                                           out.data_ptr(), scores.data_ptr() if need else None, need, attn.abq_gemm._stream_ptr(None)), "abq_attn_choose")
 
 
 def wanted(cache, q, table, context, lens, max_q, first, last, count, out):
@@ -124,8 +127,10 @@ def test_the_choice(attn, dtype, dim, heads, kv, size, columns, context, lens, f
     args = (q.cuda(), table.cuda(), ints(context), starts(lens), max_q, first, last, count)
     out = torch.full((rows, kv, count), 55, dtype=torch.int32, device="cuda")
     want = wanted(cache, q, table, context, lens, max_q, first, last, count, out)
-    chosen(attn, cache, *args, out)
-    assert np.array_equal(out.cpu().numpy(), want)
+    for kw in ({}, {"max_context": 0}, {"workspace": False}):
+        got = out.clone()
+        chosen(attn, cache, *args, got, **kw)
+        assert np.array_equal(got.cpu().numpy(), want), kw
 
 
 def test_the_choice_among_many_pages(attn):
@@ -138,8 +143,11 @@ def test_the_choice_among_many_pages(attn):
         table = torch.randint(0, 500, (1, columns), generator=gen).to(torch.int32)
         q = torch.randn(1, 3, 64, generator=gen).half()
         out = torch.full((1, 1, count), 55, dtype=torch.int32, device="cuda")
-        chosen(attn, cache, q.cuda(), table.cuda(), ints([context]), starts([1]), 1, 0, 1, count, out)
-        assert np.array_equal(out.cpu().numpy(), wanted(cache, q, table, [context], [1], 1, 0, 1, count, out)), columns
+        want = wanted(cache, q, table, [context], [1], 1, 0, 1, count, out)
+        for workspace in (True, False):
+            got = out.clone()
+            chosen(attn, cache, q.cuda(), table.cuda(), ints([context]), starts([1]), 1, 0, 1, count, got, workspace=workspace)
+            assert np.array_equal(got.cpu().numpy(), want), (columns, workspace)
 
 
 def test_the_bounds_promise_at_least_the_scores(attn):
