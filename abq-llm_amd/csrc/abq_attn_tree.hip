@@ -395,11 +395,13 @@ __global__ __launch_bounds__(64 * tree_waves(RT), RT == 1 ? 4 : 2) void attn_tre
             most = max_across_quarters(most);
             if (__any(most - base[rt] > kSlack)) { // (the difference has no rounding)
                 const float to = fmaxf(most, base[rt]);
-                const float down = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(base[rt] - to);
+                // (from 2^24 on the lift is rounded to steps of 2 and more: never to so much more that weights leave fp16.  Below, the sum
+                // of the two is off by the last bits of either, which is nothing.)
+                const float lifted = kLift - to, moved = to == -INFINITY ? 0.f : lifted + to > kLift + 0.5f ? -to : lifted;
+                // what was weighed so far follows the shift that it was weighed with, lifted or not
+                const float down = base[rt] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(moved - shift[rt]);
                 base[rt] = to;
-                // (from 2^24 on the lift is rounded to steps of 2 and more: never to more than it is)
-                const float lifted = kLift - to;
-                shift[rt] = to == -INFINITY ? 0.f : lifted + to > kLift ? -to : lifted;
+                shift[rt] = moved;
                 l[rt] *= down;
                 z[rt] *= down;
 #pragma unroll
