@@ -3,7 +3,6 @@
 Works as abq_gemm.py does and on top of it: device buffers are torch tensors, there is no CPU fallback, and a call that the
 library refuses raises AbqError.  Import torch before this module.
 """
-import collections
 import ctypes
 import importlib.util
 import math
@@ -259,7 +258,24 @@ class Rotary(_OnStream):
         return out
 
 
-Extension = collections.namedtuple("Extension", "slots starts granted copies")
+class Extension:
+    """What PageTable.extend gives: slots [rows] of the new tokens, one sequence behind the other, starts [sequences + 1], granted [sequences]
+    and copies [sequences, 2], the pages that KvCache.copy_pages has to copy in every layer before anything is written; int32."""
+
+    def __init__(self, rows, sequences, whole):
+        self.sizes, self.whole, self._parts = (rows, sequences + 1, sequences, 2 * sequences), whole, None
+        first = whole.data_ptr()
+        self.at = (first, first + 4 * rows, first + 4 * (rows + sequences + 1), first + 4 * (rows + 2 * sequences + 1))
+
+    def _part(self, i):
+        if self._parts is None:  # (views are made where they are looked at: four take as long as a launch)
+            self._parts = self.whole.split(self.sizes)
+        return self._parts[i]
+
+    slots = property(lambda self: self._part(0))
+    starts = property(lambda self: self._part(1))
+    granted = property(lambda self: self._part(2))
+    copies = property(lambda self: self._part(3).view(-1, 2))
 
 
 class PageTable(_OnStream):
@@ -290,19 +306,14 @@ class PageTable(_OnStream):
         _check(self._fork(self._ref, at, on), "abq_kv_pages_fork")
 
     def extend(self, counts, rows, out=None, stream=None):
-        """Room for counts[s] more tokens in sequence s (int32 [sequences]), or counts[s] < 0 taken away.  Returns, or fills out with, an
-        Extension: slots [rows] of the new tokens, one sequence behind the other, starts [sequences + 1], granted [sequences] and copies
-        [sequences, 2], the pages that KvCache.copy_pages has to copy in every layer before anything is written."""
-        n = self.desc.seqs
-        at, on = _index(counts, torch.int32, n, "counts"), self._on(stream)
-        if out is None:  # (one piece of memory: four of their own take longer than the call)
-            whole = self._made(rows + 4 * n + 1, stream)
-            slots, starts, granted, copies = whole.split((rows, n + 1, n, 2 * n))
-            out, first = Extension(slots, starts, granted, copies.view(n, 2)), whole.data_ptr()
-            to = (first, first + 4 * rows, first + 4 * (rows + n + 1), first + 4 * (rows + 2 * n + 1))
-        else:
-            to = [_index(t, torch.int32, m, name) for t, m, name in zip(out, (rows, n + 1, n, 2 * n), Extension._fields)]
-        _check(self._extend(self._ref, at, to[0], rows, to[1], to[2], to[3], on), "abq_kv_pages_extend")
+        """Room for counts[s] more tokens in sequence s (int32 [sequences]), or counts[s] < 0 taken away.  Returns an Extension, a new one or
+        out, which an earlier call with as many rows has given."""
+        at, on = _index(counts, torch.int32, self.desc.seqs, "counts"), self._on(stream)
+        if out is None:
+            out = Extension(rows, self.desc.seqs, self._made(rows + 4 * self.desc.seqs + 1, stream))
+        elif out.sizes != (rows, self.desc.seqs + 1, self.desc.seqs, 2 * self.desc.seqs):
+            raise ValueError("an Extension of %d rows and %d sequences is wanted" % (rows, self.desc.seqs))
+        _check(self._extend(self._ref, at, out.at[0], rows, out.at[1], out.at[2], out.at[3], on), "abq_kv_pages_extend")
         return out
 
     def compact(self, out=None, stream=None):

@@ -135,20 +135,114 @@ template <int CTRL> __device__ __forceinline__ float add_dpp(float x)
 // over the 16 lanes of a row: neighbours, pairs, mirrored halves, the other eight
 __device__ __forceinline__ float sum_of_row(float x) { return add_dpp<0x128>(add_dpp<0x141>(add_dpp<0x4e>(add_dpp<0xb1>(x)))); }
 
-// Floats as unsigned numbers of the same order
+// Floats as unsigned numbers of the same order, none of them 0, and back
 __device__ __forceinline__ uint32_t ordered(float x)
 {
     const uint32_t w = __builtin_bit_cast(uint32_t, x);
     return w & 0x80000000u ? ~w : w | 0x80000000u;
 }
+__device__ __forceinline__ float number_of(uint32_t key) { return __builtin_bit_cast(float, key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 
-// What a wave asks for at once: bounds of four tiles of 16 pages, as columns of the product
-template <int D> struct Tiles {
-    static constexpr int kCount = 4, kChunks = D / 64;
+// What page p of n is chosen by
+__device__ __forceinline__ uint32_t key_of(const ChooseArgs &a, int p, int n, bool in_cache, float score)
+{
+    return p < a.first || p >= n - a.last ? ~0u : in_cache ? ordered(score) : 0;
+}
+
+// What a wave asks for at once: bounds of COUNT tiles of 16 pages, as columns of the product, those of tile i from page p0 + i * step on.
+// Page numbers are asked for before the number of pages is known, their bounds before the query is: three loads one behind the
+// other instead of five.
+template <int D, int COUNT> struct Tiles {
+    static constexpr int kCount = COUNT, kChunks = D / 64;
     int page[kCount];
     int4v bounds[kCount][2][kChunks];
     float scale[kCount];
+
+    __device__ __forceinline__ void ask_pages(const ChooseArgs &a, const int32_t *pages, int p0, int step)
+    {
+#pragma unroll
+        for (int i = 0; i < kCount; ++i)
+            page[i] = pages[min(p0 + step * i + (int)(threadIdx.x & 15), a.max_pages - 1)];
+    }
+    __device__ __forceinline__ void ask_bounds(const ChooseArgs &a, int head, int p0, int step, int n)
+    {
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) {
+            if (p0 + step * i >= n)
+                continue;
+            const int64_t at = (int64_t)(in_cache(a, i) ? page[i] : 0) * a.c.kv_heads + head;
+            const int8_t *bound = a.b.codes + at * 2 * D + 16 * (threadIdx.x >> 4 & 3);
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j) {
+                bounds[i][0][j] = *(const int4v *)(bound + 64 * j);
+                bounds[i][1][j] = *(const int4v *)(bound + D + 64 * j);
+            }
+            scale[i] = a.b.scales[at];
+        }
+    }
+    __device__ __forceinline__ bool in_cache(const ChooseArgs &a, int i) const { return (uint32_t)page[i] < (uint32_t)a.c.num_pages; }
 };
+
+// Sixteen rows of queries as the product takes them, in LDS: what is positive of their codes, what is negative (padded against bank conflicts),
+// and their scales.  A wave quantises a row: what every wave would do for itself otherwise is most of the kernel's time.
+template <int D> struct Rows16 {
+    __align__(16) int8_t codes[2][16][D + 16];
+    float scales[16];
+
+    // rows[i] goes to row i0 + i * step; NULL: it stays as it is
+    template <int N> __device__ __forceinline__ void quantise(const uint16_t *const (&rows)[N], int i0, int step, int dtype)
+    {
+        constexpr int kEach = D / 64;
+        const int lane = threadIdx.x & 63;
+        uint32_t w[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (rows[i])
+                w[i] = kEach == 2 ? ((const uint32_t *)rows[i])[lane] : rows[i][lane];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (!rows[i])
+                continue;
+            float x[2];
+            x[0] = dtype == ABQ_BF16 ? value16<ABQ_BF16>(w[i]) : value16<ABQ_F16>(w[i]);
+            x[1] = kEach == 1 ? 0 : dtype == ABQ_BF16 ? value16<ABQ_BF16>(w[i] >> 16) : value16<ABQ_F16>(w[i] >> 16);
+            const QuantRow q = quant_row_params(max_of_wave(fmaxf(fabsf(x[0]), fabsf(x[1]))), 0.f, 8, 1);
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+                const int c = (int8_t)quant_code_bits(x[e], q);
+                codes[0][i0 + i * step][kEach * lane + e] = (int8_t)max(c, 0);
+                codes[1][i0 + i * step][kEach * lane + e] = (int8_t)min(c, 0);
+            }
+            if (lane == 0)
+                scales[i0 + i * step] = q.scale;
+        }
+    }
+    // lane (t, g): the channels 64 j + 16 g .. + 15 of row t, and the scales of rows 4 g .. 4 g + 3, whose sums it gets
+    __device__ __forceinline__ void read(int4v (&up)[D / 64], int4v (&down)[D / 64], float (&scale)[4]) const
+    {
+        const int t = threadIdx.x & 15, g = threadIdx.x >> 4 & 3;
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) {
+            up[j] = *(const int4v *)&codes[0][t][64 * j + 16 * g];
+            down[j] = *(const int4v *)&codes[1][t][64 * j + 16 * g];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            scale[i] = scales[4 * g + i];
+    }
+};
+
+// Sums of a tile's pages: lane (t, g) has page t's of rows 4 g .. 4 g + 3
+template <int D, int COUNT> __device__ __forceinline__ int4v sums_of(const Tiles<D, COUNT> &tiles, int i, const int4v (&up)[D / 64], const int4v (&down)[D / 64])
+{
+    int4v acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) {
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(up[j], tiles.bounds[i][0][j], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(down[j], tiles.bounds[i][1][j], acc, 0, 0, 0);
+    }
+    return acc;
+}
 
 // A query row of a sequence and a key head
 struct ChooseUnit {
@@ -160,116 +254,55 @@ __device__ __forceinline__ ChooseUnit choose_unit(const ChooseArgs &a, uint32_t 
 }
 __device__ __forceinline__ int complete_pages(const ChooseArgs &a, int seq) { return min(max(a.context[seq], 0) >> a.page_shift, a.max_pages); }
 
-// Scores of the pages from begin on, as many as there are before end, by all waves of a workgroup: keys[p - begin] for page p
-template <int D, int WAVES> __device__ __forceinline__ void score_pages(const ChooseArgs &a, const ChooseUnit &u, int begin, int end, uint32_t *keys)
+// Scores of all pages of a query row into LDS, by a workgroup
+template <int D, int WAVES> __device__ __forceinline__ void score_pages(const ChooseArgs &a, const ChooseUnit &u, uint32_t *keys)
 {
-    __shared__ __align__(16) int8_t rows[2][16][D + 16]; // of queries: what is positive of them, what is negative (padded against bank conflicts)
-    __shared__ float row_scales[16];
-    constexpr int kChunks = D / 64;
-    using T = Tiles<D>;
+    __shared__ Rows16<D> rows;
+    using T = Tiles<D, 4>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = lane & 15, g = lane >> 4;
     const int32_t *pages = a.page_table + (int64_t)u.seq * a.max_pages;
+    constexpr int kStep = 16 * WAVES, kRound = kStep * T::kCount;
     T tiles;
-    // Page numbers are asked for before the number of pages is known, their bounds before the query is: three loads one behind the other
-    // instead of five
-    auto ask_pages = [&](int p0) {
-#pragma unroll
-        for (int i = 0; i < T::kCount; ++i)
-            tiles.page[i] = pages[min(p0 + 16 * WAVES * i + t, a.max_pages - 1)];
-    };
-    auto ask_bounds = [&](int p0, int n) {
-#pragma unroll
-        for (int i = 0; i < T::kCount; ++i) {
-            if (p0 + 16 * WAVES * i >= n)
-                continue;
-            const int64_t at = (int64_t)((uint32_t)tiles.page[i] < (uint32_t)a.c.num_pages ? tiles.page[i] : 0) * a.c.kv_heads + u.head;
-            const int8_t *bound = a.b.codes + at * 2 * D + 16 * g;
-#pragma unroll
-            for (int j = 0; j < kChunks; ++j) {
-                tiles.bounds[i][0][j] = *(const int4v *)(bound + 64 * j);
-                tiles.bounds[i][1][j] = *(const int4v *)(bound + D + 64 * j);
-            }
-            tiles.scale[i] = a.b.scales[at];
-        }
-    };
-    ask_pages(begin + 16 * wave);
+    tiles.ask_pages(a, pages, 16 * wave, kStep);
     const SeqRows own = seq_rows(a.q_starts, u.seq, a.q.rows);
-    const int all = complete_pages(a, u.seq), n = min(all, end);
-    if (u.draft >= own.count || all <= a.count || begin >= n)
+    const int n = complete_pages(a, u.seq);
+    if (u.draft >= own.count || n <= a.count)
         return;
-    ask_bounds(begin + 16 * wave, n);
-    const int64_t q_row = own.first + u.draft;
-
+    tiles.ask_bounds(a, u.head, 16 * wave, kStep, n);
     for (int h0 = 0; h0 < a.group; h0 += 16) {
-        // Heads h0 .. h0 + 15 as rows of the product, a wave quantising each: what every wave would do for itself otherwise is most of the
-        // kernel's time.  (Rows behind the last head are whatever is there: their sums are not looked at.)
         if (h0 > 0)
             __syncthreads();
         for (int h = wave; h < min(a.group - h0, 16); h += WAVES) {
-            constexpr int kEach = D / 64;
-            const uint16_t *src = (const uint16_t *)a.q.data + q_row * a.q.row_stride + (int64_t)(u.head * a.group + h0 + h) * a.q.head_stride + kEach * lane;
-            float x[kEach], most = 0;
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                x[i] = a.dtype == ABQ_BF16 ? value16<ABQ_BF16>(src[i]) : value16<ABQ_F16>(src[i]);
-                most = fmaxf(most, fabsf(x[i]));
-            }
-            const QuantRow row = quant_row_params(max_of_wave(most), 0.f, 8, 1);
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                const int c = (int8_t)quant_code_bits(x[i], row);
-                rows[0][h][kEach * lane + i] = (int8_t)max(c, 0);
-                rows[1][h][kEach * lane + i] = (int8_t)min(c, 0);
-            }
-            if (lane == 0)
-                row_scales[h] = row.scale;
+            const uint16_t *row[1] = {(const uint16_t *)a.q.data + (own.first + u.draft) * a.q.row_stride + (int64_t)(u.head * a.group + h0 + h) * a.q.head_stride};
+            rows.quantise(row, h, 0, a.dtype);
         }
         __syncthreads();
-        // lane (t, g): the channels 64 j + 16 g .. + 15 of head h0 + t, and the scales of heads h0 + 4 g .. + 3, whose sums it gets
-        int4v up[kChunks], down[kChunks];
-#pragma unroll
-        for (int j = 0; j < kChunks; ++j) {
-            up[j] = *(const int4v *)&rows[0][t][64 * j + 16 * g];
-            down[j] = *(const int4v *)&rows[1][t][64 * j + 16 * g];
-        }
+        int4v up[D / 64], down[D / 64];
         float scale[4];
-        bool heads[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            scale[i] = row_scales[4 * g + i];
-            heads[i] = h0 + 4 * g + i < a.group;
-        }
-        constexpr int kRound = 16 * WAVES * T::kCount;
-        for (int p0 = begin + 16 * wave; p0 < n; p0 += kRound) {
-            if (p0 >= begin + kRound || h0 > 0) { // (else they are there)
-                ask_pages(p0);
-                ask_bounds(p0, n);
+        rows.read(up, down, scale);
+        for (int p0 = 16 * wave; p0 < n; p0 += kRound) {
+            if (p0 >= kRound || h0 > 0) { // (else they are there)
+                tiles.ask_pages(a, pages, p0, kStep);
+                tiles.ask_bounds(a, u.head, p0, kStep, n);
             }
 #pragma unroll
             for (int i = 0; i < T::kCount; ++i) {
-                const int p = p0 + 16 * WAVES * i + t;
+                const int p = p0 + kStep * i + t;
                 if (p - t >= n)
                     continue;
-                int4v acc = {0, 0, 0, 0};
-#pragma unroll
-                for (int j = 0; j < kChunks; ++j) {
-                    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(up[j], tiles.bounds[i][0][j], acc, 0, 0, 0);
-                    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(down[j], tiles.bounds[i][1][j], acc, 0, 0, 0);
-                }
-                // (lane (t, g) has page t's sums of heads 4 g .. 4 g + 3)
-                float score = -INFINITY;
+                const int4v acc = sums_of(tiles, i, up, down);
+                float score = -INFINITY; // (rows behind the last head are whatever is there: their sums are not looked at)
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    score = heads[k] ? fmaxf(score, (float)acc[k] * scale[k]) : score;
+                    score = h0 + 4 * g + k < a.group ? fmaxf(score, (float)acc[k] * scale[k]) : score;
                 score = max_across_quarters(score);
                 if (g == 0 && p < n) {
-                    const bool in_cache = (uint32_t)tiles.page[i] < (uint32_t)a.c.num_pages;
                     if (h0 > 0)
-                        score = fmaxf(score, __builtin_bit_cast(float, keys[p - begin]));
+                        score = fmaxf(score, __builtin_bit_cast(float, keys[p]));
                     if (h0 + 16 < a.group)
-                        keys[p - begin] = __builtin_bit_cast(uint32_t, score);
+                        keys[p] = __builtin_bit_cast(uint32_t, score);
                     else
-                        keys[p - begin] = p < a.first || p >= all - a.last ? ~0u : in_cache ? ordered(score * tiles.scale[i]) : 0;
+                        keys[p] = key_of(a, p, n, tiles.in_cache(a, i), score * tiles.scale[i]);
                 }
             }
         }
@@ -364,7 +397,7 @@ template <int D, int WAVES, bool SCORED> __global__ __launch_bounds__(64 * WAVES
     constexpr int kThreads = 64 * WAVES;
     const ChooseUnit u = choose_unit(a, blockIdx.x);
     if constexpr (!SCORED)
-        score_pages<D, WAVES>(a, u, 0, a.max_pages, keys);
+        score_pages<D, WAVES>(a, u, keys);
     const SeqRows own = seq_rows(a.q_starts, u.seq, a.q.rows);
     if (u.draft >= own.count)
         return;
@@ -382,14 +415,85 @@ template <int D, int WAVES, bool SCORED> __global__ __launch_bounds__(64 * WAVES
     write_largest<WAVES>(keys, n, want, out);
 }
 
-// The scores alone, a workgroup for each kScorePages of them
-constexpr int kScoreWaves = 4, kScorePages = 16 * kScoreWaves * 2;
+// The scores alone, a workgroup for kScorePages pages of a sequence and key head and for some of the sequence's drafts, whose rows it goes over
+// with the bounds in registers.  Rows of all its drafts' heads fill the product's sixteen; each goes into its draft's largest.
+constexpr int kScoreWaves = 4, kScoreTiles = 2, kScorePages = 16 * kScoreWaves * kScoreTiles;
+// 32 rows of queries a workgroup: more of them in turn take longer than reading the bounds again
+constexpr int score_drafts(int group) { return group >= 32 ? 1 : 32 / group; }
 
 template <int D> __global__ __launch_bounds__(64 * kScoreWaves) void attn_score_kernel(ChooseArgs a, uint32_t *scored)
 {
-    const uint32_t parts = (a.max_pages + kScorePages - 1) / kScorePages, unit = blockIdx.x / parts;
-    const int begin = (int)(blockIdx.x % parts) * kScorePages;
-    score_pages<D, kScoreWaves>(a, choose_unit(a, unit), begin, begin + kScorePages, scored + (int64_t)unit * a.max_pages + begin);
+    __shared__ Rows16<D> rows;
+    __shared__ uint32_t keys[score_drafts(1)][kScorePages];
+    __shared__ float scales[kScorePages]; // of bounds; negative: the page is not in the cache
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = lane & 15, g = lane >> 4;
+    const int each = score_drafts(a.group);
+    const uint32_t parts = (a.max_pages + kScorePages - 1) / kScorePages, turns = (a.max_q + each - 1) / each, unit = blockIdx.x / parts / turns;
+    const int begin = (int)(blockIdx.x % parts) * kScorePages, d0 = (int)(blockIdx.x / parts % turns) * each, seq = unit / a.c.kv_heads, head = unit % a.c.kv_heads;
+    constexpr int kStep = 16 * kScoreWaves;
+    Tiles<D, kScoreTiles> tiles;
+    tiles.ask_pages(a, a.page_table + (int64_t)seq * a.max_pages, begin + 16 * wave, kStep);
+    const SeqRows own = seq_rows(a.q_starts, seq, a.q.rows);
+    const int all = complete_pages(a, seq), n = min(all - begin, kScorePages), some = min(min(own.count, a.max_q) - d0, each);
+    if (some <= 0 || all <= a.count || n <= 0)
+        return;
+    tiles.ask_bounds(a, head, begin + 16 * wave, kStep, all);
+    uint32_t *out = scored + (((int64_t)seq * a.max_q + d0) * a.c.kv_heads + head) * a.max_pages + begin; // of draft d0
+    const int count = some * a.group;
+    const bool one = some == 1 && count <= 16; // (no other row has a part in a page's score)
+    if (!one)
+        for (int i = threadIdx.x; i < some * kScorePages; i += 64 * kScoreWaves)
+            (&keys[0][0])[i] = 0;
+    for (int r0 = 0; r0 < count; r0 += 16) {
+        if (r0 > 0)
+            __syncthreads();
+        const uint16_t *row[16 / kScoreWaves];
+#pragma unroll
+        for (int i = 0; i < 16 / kScoreWaves; ++i) {
+            const int r = r0 + kScoreWaves * i + wave;
+            row[i] = r < count ? (const uint16_t *)a.q.data + (own.first + d0 + r / a.group) * a.q.row_stride + (int64_t)(head * a.group + r % a.group) * a.q.head_stride : nullptr;
+        }
+        rows.quantise(row, wave, kScoreWaves, a.dtype);
+        __syncthreads();
+        int4v up[D / 64], down[D / 64];
+        float scale[4];
+        rows.read(up, down, scale);
+        int draft[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            draft[k] = r0 + 4 * g + k < count ? (r0 + 4 * g + k) / a.group : -1;
+#pragma unroll
+        for (int i = 0; i < kScoreTiles; ++i) {
+            const int p = kStep * i + 16 * wave + t;
+            if (p - t >= n)
+                continue;
+            const int4v acc = sums_of(tiles, i, up, down);
+            if (one) {
+                float score = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    score = draft[k] == 0 ? fmaxf(score, (float)acc[k] * scale[k]) : score;
+                score = max_across_quarters(score);
+                if (g == 0 && p < n)
+                    out[p] = key_of(a, begin + p, all, tiles.in_cache(a, i), score * tiles.scale[i]);
+                continue;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (draft[k] >= 0)
+                    atomicMax(&keys[draft[k]][p], ordered((float)acc[k] * scale[k]));
+            if (g == 0)
+                scales[p] = tiles.in_cache(a, i) ? tiles.scale[i] : -1.f;
+        }
+    }
+    if (one)
+        return;
+    __syncthreads();
+    for (int i = threadIdx.x; i < some * kScorePages; i += 64 * kScoreWaves) {
+        const int d = i / kScorePages, p = i % kScorePages;
+        if (p < n)
+            out[(int64_t)d * a.c.kv_heads * a.max_pages + p] = key_of(a, begin + p, all, scales[p] >= 0, number_of(keys[d][p]) * scales[p]);
+    }
 }
 
 } // namespace
@@ -430,12 +534,12 @@ template <int D, int WAVES, bool SCORED> static hipError_t choose(const ChooseAr
 template <int D> static hipError_t choose(const ChooseArgs &a, int64_t units, int likely, uint32_t *scored, hipStream_t stream)
 {
     if (scored) {
-        const int parts = (a.max_pages + kScorePages - 1) / kScorePages;
-        hipLaunchKernelGGL(attn_score_kernel<D>, dim3((unsigned)(units * parts)), dim3(64 * kScoreWaves), 0, stream, a, scored);
+        const int64_t parts = (a.max_pages + kScorePages - 1) / kScorePages, turns = (a.max_q + score_drafts(a.group) - 1) / score_drafts(a.group);
+        hipLaunchKernelGGL(attn_score_kernel<D>, dim3((unsigned)(a.seqs * a.c.kv_heads * parts * turns)), dim3(64 * kScoreWaves), 0, stream, a, scored);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess)
             return e;
-        return likely <= 1024 ? choose<D, 8, true>(a, scored, units, stream) : choose<D, 16, true>(a, scored, units, stream);
+        return likely <= 1024 || units > 64 ? choose<D, 8, true>(a, scored, units, stream) : choose<D, 16, true>(a, scored, units, stream);
     }
     // Waves: enough to score all pages in a round of 64 a wave, but no more than leave two (eight waves) or four workgroups to a compute unit
     // where there are more of these than units.  128 channels, us with 4, 8, 16 waves: 32 of 125 pages 7.6, 7.9, 9.3; 128 of 512 13.9, 13.4, 14.3;
@@ -445,11 +549,15 @@ template <int D> static hipError_t choose(const ChooseArgs &a, int64_t units, in
     return likely <= 512 || units > 256 ? choose<D, 8, false>(a, nullptr, units, stream) : choose<D, 16, false>(a, nullptr, units, stream);
 }
 
-// A launch of their own for the scores, where few workgroups would each have many: us in one launch and in two, 8 of 600 pages 12.5 and 10.3,
-// of 1200 18.4 and 11.8, of 8000 84 and 28; 64 of 600 13.1 and 12.3, of 2500 33 and 23; but 8 of 300 9.2 and 9.6, 128 of 1200 20.5 and 20.9
-size_t choose_workspace_bytes(int64_t units, int max_pages, int likely)
+// A launch of their own for the scores: where few workgroups would each have many pages, and where several drafts share a sequence's bounds.
+// us in one launch and in two, one draft: 8 units of 600 pages 12.0 and 10.6, of 1500 20.7 and 12.2, of 8000 82 and 27; 64 of 1500 22 and 16.5;
+// but 8 of 300 9.3 and 10.3, 128 of 1200 20.6 and 21.2, 256 of 1200 23.6 and 28.  Drafts: 7 x 5 of 8 heads, 600 pages 18.8 and 17.8, 1250
+// 29.5 and 23.4; 64 of 32 heads, 600 pages 53 and 33; but 7 x 5 of 300 pages 13.4 and 15.6.
+size_t choose_workspace_bytes(int seqs, int max_q, int kv_heads, int max_pages, int likely)
 {
-    return likely > 512 && units <= 64 ? (size_t)units * max_pages * sizeof(uint32_t) : 0;
+    const double units = (double)seqs * max_q * kv_heads, blocks = units * ((max_pages + kScorePages - 1) / kScorePages);
+    const bool two = likely > 512 && (units <= 64 || max_q > 1) && blocks <= kMostBlocks;
+    return two ? (size_t)seqs * max_q * kv_heads * max_pages * sizeof(uint32_t) : 0;
 }
 
 hipError_t launch_attn_choose(const ChooseCall &call, hipStream_t stream)
@@ -459,7 +567,7 @@ hipError_t launch_attn_choose(const ChooseCall &call, hipStream_t stream)
     const ChooseArgs a = {call.cache, call.bounds, call.q, call.page_table, call.context, call.q_starts, call.blocks, call.dtype, call.heads / call.cache.kv_heads,
                           call.seqs, call.max_q, call.max_pages, call.first, call.last, call.count, __builtin_ctz((unsigned)call.cache.page_size)};
     const int64_t units = (int64_t)call.seqs * call.max_q * call.cache.kv_heads;
-    const size_t need = choose_workspace_bytes(units, call.max_pages, call.likely);
+    const size_t need = choose_workspace_bytes(call.seqs, call.max_q, call.cache.kv_heads, call.max_pages, call.likely);
     uint32_t *scored = need && call.workspace_bytes >= need ? (uint32_t *)call.workspace : nullptr;
     return call.cache.head_dim == 64 ? choose<64>(a, units, call.likely, scored, stream) : choose<128>(a, units, call.likely, scored, stream);
 }

@@ -81,10 +81,9 @@ template <int K> __device__ __forceinline__ float of_lane(float x)
     return __builtin_bit_cast(float, of_lane<K>(__builtin_bit_cast(uint32_t, x)));
 }
 
-// at0, at1: the places of the halves' first tokens.  `seen`: bit h is cleared if half h lies on a page outside the cache
+// The halves' first places, and the pages that these lie on.  `seen`: bit h is cleared if half h lies on a page outside the cache
 template <int BITS, bool ASYM, int D>
-__device__ __forceinline__ void load_step(Step<BITS, ASYM, D> &s, const TreeArgs &a, const int32_t *pages, int last_page, int head, int at0, int at1, int lane,
-                                          uint32_t *seen)
+__device__ __forceinline__ void load_step(Step<BITS, ASYM, D> &s, const TreeArgs &a, int head, int at0, int at1, int page0, int page1, int lane, uint32_t *seen)
 {
     using S = Step<BITS, ASYM, D>;
     constexpr int R = D * BITS / 8;
@@ -94,7 +93,7 @@ __device__ __forceinline__ void load_step(Step<BITS, ASYM, D> &s, const TreeArgs
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int pos = h ? at1 : at0;
-        int page = pages[min(pos >> a.page_shift, last_page)];
+        int page = h ? page1 : page0;
         if ((uint32_t)page >= (uint32_t)a.c.num_pages) {
             page = 0;
             *seen &= ~(1u << h);
@@ -234,16 +233,16 @@ __global__ __launch_bounds__(64 * tree_waves(RT), RT == 1 ? 4 : 2) void attn_tre
         }
     }
     const int64_t inside = (int64_t)named << a.page_shift, over = LISTED ? inside + len - behind : len;
-    // the place of a step's half, or -1 if it has none
-    auto place_of = [&](int step, int h) {
-        const int64_t x = (int64_t)step * kStep + 16 * h;
-        if constexpr (LISTED) {
-            if (x >= inside)
-                return behind + (int)(x - inside);
-            const int32_t block = list[x >> a.page_shift];
-            return (uint32_t)block < (uint32_t)complete ? (block << a.page_shift) + (int)(x & (a.c.page_size - 1)) : -1;
-        }
-        return (int)x;
+    // LISTED: where the halves of the wave's next 32 steps lie, a half in each lane, so that two loads one behind the other are made once
+    // for all of them and not for each step
+    int lane_place = 0, lane_page = 0;
+    auto look_up = [&](int step, int step1) {
+        const int64_t x = (int64_t)(step + (lane >> 1) * kWaves) * kStep + 16 * (lane & 1);
+        const bool mine = step + (lane >> 1) * kWaves < step1;
+        const int32_t block = mine && x < inside ? list[x >> a.page_shift] : 0;
+        const bool named_one = x >= inside || (uint32_t)block < (uint32_t)complete;
+        lane_place = x >= inside ? behind + (int)(x - inside) : ((named_one ? block : 0) << a.page_shift) + (int)(x & (a.c.page_size - 1));
+        lane_page = mine && named_one ? pages[min(lane_place >> a.page_shift, last_page)] : -1;
     };
 
     // the queries as the products take them, the power of two that they were divided by, and their sums
@@ -453,12 +452,20 @@ __global__ __launch_bounds__(64 * tree_waves(RT), RT == 1 ? 4 : 2) void attn_tre
     // One row tile leaves registers for four waves per SIMD, which cover each other's loads; with more, a wave loads a step ahead.
     // Eight waves in a workgroup keep them there where there are few workgroups (of four and of eight: 32768 tokens, 8 heads 25 and 20
     // us, 20 x 700 tokens 11.3 and 10.2, 16 x 1024 of 32 heads 29 either way; sixteen 20, 10.6, 34).
+    int nth = 0; // of the wave's steps, within those that were looked up
     auto load = [&](S &s, int step, int &at0, int &at1, uint32_t &seen) {
-        at0 = place_of(step, 0);
-        at1 = place_of(step, 1);
-        load_step<BITS, ASYM, D>(s, a, pages, last_page, head, LISTED ? max(at0, 0) : at0, LISTED ? max(at1, 0) : at1, lane, &seen);
-        if (LISTED)
-            seen &= (at0 < 0 ? ~1u : ~0u) & (at1 < 0 ? ~2u : ~0u);
+        if constexpr (LISTED) {
+            if (nth % 32 == 0)
+                look_up(step, step1);
+            const int l = 2 * (nth++ % 32);
+            at0 = __builtin_amdgcn_readlane(lane_place, l);
+            at1 = __builtin_amdgcn_readlane(lane_place, l + 1);
+            load_step<BITS, ASYM, D>(s, a, head, at0, at1, __builtin_amdgcn_readlane(lane_page, l), __builtin_amdgcn_readlane(lane_page, l + 1), lane, &seen);
+        } else {
+            at0 = step * kStep;
+            at1 = at0 + 16;
+            load_step<BITS, ASYM, D>(s, a, head, at0, at1, pages[min(at0 >> a.page_shift, last_page)], pages[min(at1 >> a.page_shift, last_page)], lane, &seen);
+        }
     };
     int at00, at01, at10, at11; // (places of the halves of the two steps in flight)
     if constexpr (RT == 1) {

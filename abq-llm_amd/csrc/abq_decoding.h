@@ -38,7 +38,7 @@ struct ChooseCall {
     size_t workspace_bytes;
 };
 // Bytes of all pages' scores where they are worth a launch of their own; 0 otherwise
-size_t choose_workspace_bytes(int64_t units, int max_pages, int likely);
+size_t choose_workspace_bytes(int seqs, int max_q, int kv_heads, int max_pages, int likely);
 hipError_t launch_kv_bound(const abq_kv_cache &c, const abq_kv_bounds &bounds, const int32_t *slots, int64_t count, hipStream_t stream);
 hipError_t launch_attn_choose(const ChooseCall &call, hipStream_t stream);
 

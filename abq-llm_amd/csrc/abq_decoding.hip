@@ -216,7 +216,7 @@ size_t abq_attn_choose_workspace_bytes(const abq_kv_cache *cache, int max_pages,
 {
     if (!cache_sizes_valid(cache) || max_pages <= 0 || max_pages > kMostChosen || seqs <= 0 || max_q <= 0 || max_context < 0)
         return 0;
-    return choose_workspace_bytes(product(seqs, max_q, cache->kv_heads), max_pages, likely_pages(cache, max_pages, max_context));
+    return choose_workspace_bytes(seqs, max_q, cache->kv_heads, max_pages, likely_pages(cache, max_pages, max_context));
 }
 
 abq_status abq_attn_choose(const abq_kv_cache *cache, const abq_kv_bounds *bounds, const abq_rows *q, int dtype, int heads, const int32_t *page_table,

@@ -158,6 +158,7 @@ def test_bounds_and_the_choice_are_refused(attn):
     assert choose(q={"rows": 0}, blocks=None) == ok.ABQ_OK
     need = lambda *a, **c: L.abq_attn_choose_workspace_bytes(ref(cache_desc(attn, **c)), *a)  # noqa: E731
     assert need(2000, 1, 1, 1500 * 64) == 2000 * 2 * 4 and need(2000, 1, 1, 100) == need(100, 1, 1, 10 ** 6) == need(2000, 999, 1, 10 ** 6) == 0
+    assert need(2000, 999, 2, 10 ** 6) == 999 * 2 * 2 * 2000 * 4 and need(32768, 1 << 20, 64, 10 ** 6) == 0
     assert need(0, 1, 1, 10 ** 6) == need(32769, 1, 1, 10 ** 6) == need(2000, 1, 1, 10 ** 6, bits=3) == need(2000, 2 ** 31 - 1, 2 ** 31 - 1, 10 ** 6) == 0
 
 
@@ -261,4 +262,8 @@ def test_memory_of_the_objects_is_safe_on_other_streams(attn, monkeypatch):
     assert streams.taken() == [("run", 0x20)]
     given = table.extend(parents, 5, stream=other)
     assert streams.taken() == [("made", 0x20), ("run", 0x20)]
-    assert [tuple(t.shape) for t in given] == [(5,), (3,), (2,), (2, 2)]
+    assert [tuple(t.shape) for t in (given.slots, given.starts, given.granted, given.copies)] == [(5,), (3,), (2,), (2, 2)]
+    assert [t.data_ptr() for t in (given.slots, given.starts, given.granted, given.copies)] == list(given.at)
+    assert table.extend(parents, 5, out=given, stream=other) is given
+    with pytest.raises(ValueError):
+        table.extend(parents, 6, out=given, stream=other)
