@@ -51,7 +51,8 @@ abq_status check_pages(const abq_kv_pages *p)
     if (!p || p->seqs <= 0 || p->max_pages <= 0 || p->num_pages <= 0 || p->page_size < 16 || p->page_size > 4096 || (p->page_size & (p->page_size - 1)) ||
         (int64_t)p->num_pages * p->page_size > 0x7fffffff || !p->table || !p->lengths || !p->refs)
         return ABQ_ERR_INVALID_ARG;
-    if (p->seqs > kMostSeqs || (int64_t)p->max_pages * p->page_size > 0x7fffffff - 64)
+    // (workgroups of 1024 threads for two columns each, or more, and one)
+    if (p->seqs > kMostSeqs || (int64_t)p->max_pages * p->page_size > 0x7fffffff - 64 || p->max_pages > kMostThreads / 1024 - 2)
         return ABQ_ERR_TOO_LARGE;
     return ABQ_OK;
 }
@@ -151,7 +152,9 @@ abq_status abq_kv_pages_fork(const abq_kv_pages *pages, const int32_t *parents, 
     const abq_status s = check_pages(pages);
     if (s != ABQ_OK)
         return s;
-    return parents ? hip_status(launch_pages_fork(*pages, parents, (hipStream_t)stream)) : ABQ_ERR_INVALID_ARG;
+    if (!parents)
+        return ABQ_ERR_INVALID_ARG;
+    return hip_status(launch_pages_fork(*pages, parents, (hipStream_t)stream));
 }
 
 abq_status abq_kv_pages_extend(const abq_kv_pages *pages, const int32_t *counts, int32_t *slots, int64_t rows, int32_t *starts, int32_t *granted,

@@ -386,15 +386,15 @@ struct CopyArgs {
     float *scales;
     int heads, num_pages;
     const int32_t *pairs;
-    int64_t each; // workgroups of a pair
+    uint32_t each; // workgroups of a pair
 };
 
 // A turn is 4 KB, a word of a lane: with four words of a lane in 16 KB, 315 pages of 132 KB took 24 us instead of 15, three of 530 KB 10
 // instead of 2.5
 __global__ __launch_bounds__(256) void copy_pages_kernel(CopyArgs a)
 {
-    const int64_t pair = blockIdx.x / a.each;
-    const int from = a.pairs[2 * pair], to = a.pairs[2 * pair + 1];
+    const uint32_t pair = blockIdx.x / a.each;
+    const int from = a.pairs[2 * (int64_t)pair], to = a.pairs[2 * (int64_t)pair + 1];
     if ((uint32_t)from >= (uint32_t)a.num_pages || (uint32_t)to >= (uint32_t)a.num_pages || from == to)
         return;
     for (int turn = (int)(blockIdx.x % a.each); turn < a.turns[kArrays - 1]; turn += (int)a.each) {
@@ -474,7 +474,7 @@ hipError_t launch_copy_pages(const abq_kv_cache &c, const abq_kv_bounds *bounds,
     a.num_pages = c.num_pages;
     a.pairs = pairs;
     const int64_t most = kMostBlocks / count;
-    a.each = a.turns[kArrays - 1] < most ? a.turns[kArrays - 1] : most;
+    a.each = (uint32_t)(a.turns[kArrays - 1] < most ? a.turns[kArrays - 1] : most);
     hipLaunchKernelGGL(copy_pages_kernel, dim3((unsigned)(count * a.each)), dim3(256), 0, stream, a);
     return hipGetLastError();
 }

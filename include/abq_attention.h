@@ -96,8 +96,8 @@ typedef struct abq_rotary {
     const int32_t *axis; /* device, [rotary_dim / 2], each 0 .. axes - 1 (others count as the nearest of these); NULL: all 0 */
 } abq_rotary;
 
-/* Turns rows of q into q_out and of k into k_out: the same rows, in place, or others that do not overlap.  k (and k_out) may be
- * NULL.  positions: device int32, axis a of token i at positions[a * position_stride + i]; position_stride >= the number of rows where there
+/* Turns rows of q into q_out and of k into k_out: into the same rows, in place, or others; but for that nothing that is written may
+ * overlap anything else that is read or written.  k (and k_out) may be NULL.  positions: device int32, axis a of token i at positions[a * position_stride + i]; position_stride >= the number of rows where there
  * are several axes.  head_dim: a multiple of 16, at most 256. */
 abq_status abq_rotary_apply(const abq_rotary *rotary, const abq_rows *q, const abq_rows *q_out, int heads, const abq_rows *k, const abq_rows *k_out,
                             int kv_heads, int head_dim, int dtype, const int32_t *positions, int64_t position_stride, void *stream);
@@ -120,7 +120,7 @@ abq_status abq_kv_append_rotary(const abq_kv_cache *cache, const abq_rotary *rot
  * ------------------------------------------------------------------------------------- */
 typedef struct abq_kv_pages {
     int seqs;      /* at most 8192 */
-    int max_pages; /* of a sequence; max_pages * page_size < 2^31 - 64 */
+    int max_pages; /* of a sequence; at most 2^22 - 3, and max_pages * page_size < 2^31 - 64 */
     int page_size; /* as in abq_kv_cache */
     int num_pages;
     int32_t *table, *lengths, *refs; /* device: [seqs][max_pages], [seqs], [num_pages] */

@@ -103,7 +103,7 @@ def test_calls_on_pages_are_refused(attn):
     for kw in ({"seqs": 0}, {"max_pages": 0}, {"num_pages": 0}, {"page_size": 8}, {"page_size": 48}, {"page_size": 8192}, {"num_pages": 1 << 27}, {"table": None},
                {"lengths": None}, {"refs": None}, {"seqs": -1}):
         assert calls(**kw) == {ok.ABQ_ERR_INVALID_ARG}, kw
-    for kw in ({"seqs": 8193}, {"max_pages": 1 << 27}):
+    for kw in ({"seqs": 8193}, {"max_pages": 1 << 27}, {"max_pages": (1 << 22) - 2}):
         assert calls(**kw) == {ok.ABQ_ERR_TOO_LARGE}, kw
     p = ref(pages(attn))
     assert L.abq_kv_pages_fork(None, A, None) == L.abq_kv_pages_fork(p, None, None) == L.abq_kv_pages_compact(p, None, None) == ok.ABQ_ERR_INVALID_ARG
@@ -112,7 +112,7 @@ def test_calls_on_pages_are_refused(attn):
         assert L.abq_kv_pages_extend(p, *[None if j == i else x for j, x in enumerate(good)], None) == ok.ABQ_ERR_INVALID_ARG
     assert L.abq_kv_pages_extend(p, A, A, -1, A, A, A, None) == ok.ABQ_ERR_INVALID_ARG
     assert L.abq_kv_pages_extend(p, A, A, 1 << 31, A, A, A, None) == ok.ABQ_ERR_TOO_LARGE
-    assert L.abq_kv_pages_compact(ref(pages(attn, seqs=8192, max_pages=1 << 20)), A, None) == ok.ABQ_ERR_TOO_LARGE
+    assert L.abq_kv_pages_compact(ref(pages(attn, seqs=8192, max_pages=1 << 21)), A, None) == ok.ABQ_ERR_TOO_LARGE
     assert L.abq_kv_pages_compact(ref(pages(attn, num_pages=1)), None, None) == ok.ABQ_OK  # nothing can move: no launch
 
     def copy(c={}, bounds=None, pairs=A, count=3):
@@ -267,3 +267,20 @@ def test_memory_of_the_objects_is_safe_on_other_streams(attn, monkeypatch):
     assert table.extend(parents, 5, out=given, stream=other) is given
     with pytest.raises(ValueError):
         table.extend(parents, 6, out=given, stream=other)
+
+
+def test_launches_stay_within_the_threads_that_hip_counts(attn, tmp_path):
+    """Grid times workgroup of every launch below 2^32, and within what a launch may hold of LDS, at the largest sizes that are taken"""
+    from decoding_launch_probe import launches
+    calls = [("rotary", 2 ** 31 - 16, 8, 0, 128), ("rotary", 1 << 24, 32, 8, 128), ("rotary", 7, 1 << 20, 4, 64), ("rotary", 1 << 23, 8, 2, 256),
+             ("append", 2 ** 20, 32, 8, 128), ("append", 2 ** 22, 64, 8, 64), ("append", 3, 1 << 14, 512, 128),
+             ("fork", 8192, (1 << 22) - 3), ("fork", 4096, 1000), ("fork", 1, 1), ("extend", 8192, 100, 2 ** 31 - 16), ("extend", 5, 100, 4096), ("compact", 8192, 1 << 20),
+             ("copy", 8, 1 << 20), ("copy", 512, (1 << 24) - 1), ("bound", 8, 2 ** 31), ("bound", 64, 1 << 20),
+             ("choose", 8, 1 << 16, 8, 32768, 1 << 19), ("choose", 8, 1, 1, 32768, 1 << 19), ("choose", 32, 2000, 64, 500, 1 << 14), ("choose", 32, 300, 64, 1000, 16000),
+             ("sparse", 8, 100000, 8, 32768, 1 << 19), ("sparse", 64, 8, 64, 300, 1 << 19), ("sparse", 8, 1, 1, 32768, 1 << 19)]
+    refused = {("rotary", 2 ** 31 - 16, 8, 0, 128), ("compact", 8192, 1 << 20), ("bound", 8, 2 ** 31), ("choose", 8, 1 << 16, 8, 32768, 1 << 19)}
+    for call, r in zip(calls, launches(tmp_path, calls)):
+        assert r["status"] == (attn.abq_gemm.ABQ_ERR_TOO_LARGE if call in refused else 0) and bool(r["launches"]) == (call not in refused), (call, r)
+        for made in r["launches"]:
+            assert made["grid"][0] * made["block"][0] < 2 ** 32 and made["grid"][1:] == made["block"][1:] == [1, 1], (call, made)
+            assert made["lds"] <= 128 << 10, (call, made)
