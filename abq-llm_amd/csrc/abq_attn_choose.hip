@@ -27,10 +27,8 @@ struct BoundArgs {
     abq_kv_bounds b;
     const int32_t *slots;
     int64_t count;
-    int page_shift, head_blocks;
+    int page_shift, head_blocks, each; // each: slots that a workgroup looks through
 };
-
-constexpr int kBoundSlots = 8; // that a workgroup looks through
 
 // The elements of a lane's 16 bytes of codes, in order
 template <int BITS> __device__ __forceinline__ float code_of(const uint32_t (&w)[4], int e)
@@ -40,18 +38,41 @@ template <int BITS> __device__ __forceinline__ float code_of(const uint32_t (&w)
     return (float)(w[e / 8] >> (4 * ((e & 1) * 4 + (e & 7) / 2)) & 15);
 }
 
+// Lanes that differ in bit O change parts: afterwards *keep has, in the lanes without the bit, both lanes' `first` (its own and *other's), in
+// those with it both lanes' `second`
+template <int O> __device__ __forceinline__ void exchange(float first, float second, int lane, float *keep, float *other)
+{
+    if constexpr (O >= 16) { // one operation: the upper halves of the one change places with the lower ones of the other
+        const uint32_t f = __builtin_bit_cast(uint32_t, first), s = __builtin_bit_cast(uint32_t, second);
+        uint32_t x, y;
+        if constexpr (O == 32) {
+            const auto r = __builtin_amdgcn_permlane32_swap(f, s, false, false);
+            x = r[0], y = r[1];
+        } else {
+            const auto r = __builtin_amdgcn_permlane16_swap(f, s, false, false);
+            x = r[0], y = r[1];
+        }
+        *keep = __builtin_bit_cast(float, x);
+        *other = __builtin_bit_cast(float, y);
+    } else {
+        *keep = lane & O ? second : first;
+        *other = __shfl_xor(lane & O ? first : second, O);
+    }
+}
+
 // The largest of hi and the smallest of lo over the lanes that differ in the bits O, O / 2 .. LAST, a part of the N channels, from *c0 on, in each
 template <int N, int O, int LAST> __device__ __forceinline__ void scatter(float *hi, float *lo, int lane, int *c0)
 {
     if constexpr (O >= LAST) {
-        const bool upper = lane & O;
 #pragma unroll
         for (int e = 0; e < N / 2; ++e) {
-            const float h = __shfl_xor(upper ? hi[e] : hi[N / 2 + e], O), l = __shfl_xor(upper ? lo[e] : lo[N / 2 + e], O);
-            hi[e] = fmaxf(upper ? hi[N / 2 + e] : hi[e], h);
-            lo[e] = fminf(upper ? lo[N / 2 + e] : lo[e], l);
+            float keep, other;
+            exchange<O>(hi[e], hi[N / 2 + e], lane, &keep, &other);
+            hi[e] = fmaxf(keep, other);
+            exchange<O>(lo[e], lo[N / 2 + e], lane, &keep, &other);
+            lo[e] = fminf(keep, other);
         }
-        *c0 += upper ? N / 2 : 0;
+        *c0 += lane & O ? N / 2 : 0;
         scatter<N / 2, O / 2, LAST>(hi, lo, lane, c0);
     }
 }
@@ -61,9 +82,12 @@ template <int BITS, int D> __global__ __launch_bounds__(256) void kv_bound_kerne
 {
     constexpr int R = D * BITS / 8, kLanes = R / 16, kRows = 64 / kLanes, kEach = D / kLanes;
     const int lane = threadIdx.x & 63, li = lane % kLanes;
-    const int head = blockIdx.x % a.head_blocks * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t i = (int64_t)(blockIdx.x / a.head_blocks) * kBoundSlots + lane;
-    const int slot = lane < kBoundSlots && i < a.count ? a.slots[i] : -1;
+    // A prompt's pages end at every so many workgroups, which go round the eight XCDs: each eight of them in another order, lest all work be
+    // one XCD's
+    const uint32_t block = blockIdx.x ^ (blockIdx.x >> 3 & 7);
+    const int head = block % a.head_blocks * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t i = (int64_t)(block / a.head_blocks) * a.each + lane;
+    const int slot = lane < a.each && i < a.count ? a.slots[i] : -1;
     const int last = (1 << a.page_shift) - 1;
     uint64_t ends = __ballot(slot >= 0 && (slot & last) == last && (slot >> a.page_shift) < a.c.num_pages);
     if (head >= a.c.kv_heads)
@@ -82,7 +106,7 @@ template <int BITS, int D> __global__ __launch_bounds__(256) void kv_bound_kerne
 #pragma unroll 2
         for (int t0 = 0; t0 <= last; t0 += kRows) {
             const int t = min(t0 + lane / kLanes, last); // (a token twice is a token)
-            const uint4 x = *(const uint4 *)(codes + (int64_t)t * R + 16 * li);
+            const uint4 x = *(const uint4 *)(codes + t * R + 16 * li);
             const uint32_t w[4] = {x.x, x.y, x.z, x.w};
             const float scale = scales[t], zero = a.c.symmetric ? (float)(1 << (BITS - 1)) : scales[last + 1 + t];
 #pragma unroll
@@ -510,8 +534,10 @@ hipError_t launch_kv_bound(const abq_kv_cache &c, const abq_kv_bounds &bounds, c
 {
     if (count == 0)
         return hipSuccess;
-    BoundArgs a = {c, bounds, slots, count, __builtin_ctz((unsigned)c.page_size), (c.kv_heads + 3) / 4};
-    const dim3 grid((unsigned)((count + kBoundSlots - 1) / kBoundSlots * a.head_blocks));
+    // Few slots may be of as many sequences, whose pages may all end at once; many are a prompt's, one of so many ends a page, and workgroups
+    // that find none are not for nothing (16384 slots, 256 pages of 32 heads: 42 us with 8 slots a workgroup, whose least is the launch of 16384)
+    BoundArgs a = {c, bounds, slots, count, __builtin_ctz((unsigned)c.page_size), (c.kv_heads + 3) / 4, count <= 1024 ? 1 : c.page_size < 64 ? c.page_size : 64};
+    const dim3 grid((unsigned)(((count + a.each - 1) / a.each * a.head_blocks + 7) / 8 * 8));
     if (c.bits == 8)
         ABQ_BOUND(8);
     else
