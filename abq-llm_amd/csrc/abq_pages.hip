@@ -3,7 +3,9 @@
 //
 // Tables are small (512 sequences of 40 pages, 80 KB; 6000 counts, 24 KB), so these calls are bound by launches and by the length of
 // their chains of loads: whatever has to be decided in order is decided by one workgroup of 1024 threads that scans, everything
-// else by as many as there is work for.  Copies are bound by memory.
+// else by as many as there is work for.  In a captured graph, 4 (512) sequences: fork 2.5 (4.1) us, growth by a token or taking it back 4.9
+// (7.2); 4000 pages of 60 sequences made compact 9.7, of which the moves 5.8 and the entries' new names 3.9.
+// Copies are bound by memory: 915 pages of 132 KB 49 us, 4.9 TB/s, the rate of any copy.
 #include "abq_decoding.h"
 
 namespace abq {
