@@ -455,7 +455,7 @@ template <int D> __global__ __launch_bounds__(64 * kScoreWaves) void attn_score_
 {
     __shared__ Rows16<D> rows;
     __shared__ uint32_t keys[score_drafts(1)][kScorePages];
-    __shared__ float scales[kScorePages]; // of bounds; negative: the page is not in the cache
+    __shared__ float scales[kScorePages]; // of bounds; -inf: the page is not in the cache
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = lane & 15, g = lane >> 4;
     const int each = score_drafts(a.group);
     const uint32_t parts = (a.max_pages + kScorePages - 1) / kScorePages, turns = (a.max_q + each - 1) / each, unit = blockIdx.x / parts / turns;
@@ -513,7 +513,7 @@ template <int D> __global__ __launch_bounds__(64 * kScoreWaves) void attn_score_
                 if (draft[k] >= 0)
                     atomicMax(&keys[draft[k]][p], ordered((float)acc[k] * scale[k]));
             if (g == 0)
-                scales[p] = tiles.in_cache(a, i) ? tiles.scale[i] : -1.f;
+                scales[p] = tiles.in_cache(a, i) ? tiles.scale[i] : -INFINITY;
         }
     }
     if (one)
@@ -522,7 +522,7 @@ template <int D> __global__ __launch_bounds__(64 * kScoreWaves) void attn_score_
     for (int i = threadIdx.x; i < some * kScorePages; i += 64 * kScoreWaves) {
         const int d = i / kScorePages, p = i % kScorePages;
         if (p < n)
-            out[(int64_t)d * a.c.kv_heads * a.max_pages + p] = key_of(a, begin + p, all, scales[p] >= 0, number_of(keys[d][p]) * scales[p]);
+            out[(int64_t)d * a.c.kv_heads * a.max_pages + p] = key_of(a, begin + p, all, scales[p] != -INFINITY, number_of(keys[d][p]) * scales[p]);
     }
 }
 
@@ -536,13 +536,15 @@ template <int D> __global__ __launch_bounds__(64 * kScoreWaves) void attn_score_
             hipLaunchKernelGGL((kv_bound_kernel<B, 128>), grid, dim3(256), 0, stream, a);                  \
     } while (0)
 
+// Few slots may be of as many sequences, whose pages may all end at once; many are a prompt's, one of so many ends a page, and workgroups
+// that find none are not for nothing (16384 slots, 256 pages of 32 heads: 42 us with 8 slots a workgroup, whose least is the launch of 16384)
+int bound_slots(const abq_kv_cache &c, int64_t count) { return count <= 1024 ? 1 : c.page_size < 64 ? c.page_size : 64; }
+
 hipError_t launch_kv_bound(const abq_kv_cache &c, const abq_kv_bounds &bounds, const int32_t *slots, int64_t count, hipStream_t stream)
 {
     if (count == 0)
         return hipSuccess;
-    // Few slots may be of as many sequences, whose pages may all end at once; many are a prompt's, one of so many ends a page, and workgroups
-    // that find none are not for nothing (16384 slots, 256 pages of 32 heads: 42 us with 8 slots a workgroup, whose least is the launch of 16384)
-    BoundArgs a = {c, bounds, slots, count, __builtin_ctz((unsigned)c.page_size), (c.kv_heads + 3) / 4, count <= 1024 ? 1 : c.page_size < 64 ? c.page_size : 64};
+    BoundArgs a = {c, bounds, slots, count, __builtin_ctz((unsigned)c.page_size), (c.kv_heads + 3) / 4, bound_slots(c, count)};
     const dim3 grid((unsigned)(((count + a.each - 1) / a.each * a.head_blocks + 7) / 8 * 8));
     if (c.bits == 8)
         ABQ_BOUND(8);

@@ -27,8 +27,8 @@
 // two waves per SIMD, each with a step under way while it works at another.  20 rows on 48 ragged contexts, 630 MB: 148 us,
 // 4.3 TB/s; 108 rows on 3 x 5500 tokens of 4 bits, 28 us, bound by that work and, at 9 steps a wave, by its start and end.
 //
-// With lists of pages (LISTED) every draft has rows of its own, those of one key head's group.  128 of them on 3072 tokens of 8 bits, 104 MB,
-// 22.7 us with the join, 5.3 TB/s without; 280 of 4 rows on 1600 tokens of 4 bits, 25 us for 65 MB (and 26 for 118 of 8 bits), bound by the
+// With lists of pages (LISTED) every draft has rows of its own, those of one key head's group.  128 of them on 48 pages of 64 tokens of 8 bits,
+// 104 MB, 22.7 us with the join, 5.3 TB/s without; 280 of 4 rows on 1600 tokens of 4 bits, 25 us for 65 MB (and 26 for 118 of 8 bits), bound by the
 // vector work, which is the same for one row as for sixteen.
 #include "abq_decoding.h"
 

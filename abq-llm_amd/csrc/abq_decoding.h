@@ -39,6 +39,7 @@ struct ChooseCall {
 };
 // Bytes of all pages' scores where they are worth a launch of their own; 0 otherwise
 size_t choose_workspace_bytes(int seqs, int max_q, int kv_heads, int max_pages, int likely);
+int bound_slots(const abq_kv_cache &c, int64_t count); // that a workgroup looks through
 hipError_t launch_kv_bound(const abq_kv_cache &c, const abq_kv_bounds &bounds, const int32_t *slots, int64_t count, hipStream_t stream);
 hipError_t launch_attn_choose(const ChooseCall &call, hipStream_t stream);
 

@@ -210,7 +210,8 @@ abq_status abq_kv_bound(const abq_kv_cache *cache, const abq_kv_bounds *bounds, 
         return s;
     if (count < 0 || (count && !slots))
         return ABQ_ERR_INVALID_ARG;
-    if (product(count / 8 + 1, (cache->kv_heads + 3) / 4, 1) > kMostBlocks)
+    // (workgroups in eights)
+    if (product((count - 1) / bound_slots(*cache, count) + 1, (cache->kv_heads + 3) / 4, 1) > kMostBlocks / 8 * 8)
         return ABQ_ERR_TOO_LARGE;
     return hip_status(launch_kv_bound(*cache, *bounds, slots, count, (hipStream_t)stream));
 }

@@ -275,10 +275,10 @@ def test_launches_stay_within_the_threads_that_hip_counts(attn, tmp_path):
     calls = [("rotary", 2 ** 31 - 16, 8, 0, 128), ("rotary", 1 << 24, 32, 8, 128), ("rotary", 7, 1 << 20, 4, 64), ("rotary", 1 << 23, 8, 2, 256),
              ("append", 2 ** 20, 32, 8, 128), ("append", 2 ** 22, 64, 8, 64), ("append", 3, 1 << 14, 512, 128),
              ("fork", 8192, (1 << 22) - 3), ("fork", 4096, 1000), ("fork", 1, 1), ("extend", 8192, 100, 2 ** 31 - 16), ("extend", 5, 100, 4096), ("compact", 8192, 1 << 20),
-             ("copy", 8, 1 << 20), ("copy", 512, (1 << 24) - 1), ("bound", 8, 2 ** 31), ("bound", 64, 1 << 20),
+             ("copy", 8, 1 << 20), ("copy", 512, (1 << 24) - 1), ("bound", 8, 2 ** 34), ("bound", 65536, 1024), ("bound", 65536, 1023), ("bound", 8, 2 ** 27), ("bound", 8, 2 ** 27 - 64), ("bound", 64, 1 << 20),
              ("choose", 8, 1 << 16, 8, 32768, 1 << 19), ("choose", 8, 1, 1, 32768, 1 << 19), ("choose", 32, 2000, 64, 500, 1 << 14), ("choose", 32, 300, 64, 1000, 16000),
              ("sparse", 8, 100000, 8, 32768, 1 << 19), ("sparse", 64, 8, 64, 300, 1 << 19), ("sparse", 8, 1, 1, 32768, 1 << 19)]
-    refused = {("rotary", 2 ** 31 - 16, 8, 0, 128), ("compact", 8192, 1 << 20), ("bound", 8, 2 ** 31), ("choose", 8, 1 << 16, 8, 32768, 1 << 19)}
+    refused = {("rotary", 2 ** 31 - 16, 8, 0, 128), ("compact", 8192, 1 << 20), ("bound", 8, 2 ** 34), ("bound", 65536, 1024), ("bound", 8, 2 ** 27), ("choose", 8, 1 << 16, 8, 32768, 1 << 19)}
     for call, r in zip(calls, launches(tmp_path, calls)):
         assert r["status"] == (attn.abq_gemm.ABQ_ERR_TOO_LARGE if call in refused else 0) and bool(r["launches"]) == (call not in refused), (call, r)
         for made in r["launches"]:
