@@ -161,6 +161,18 @@ def _index(t, dtype, numel, what):
     return t.data_ptr()
 
 
+# (with one device there is nowhere else to be)
+_many_devices = torch.cuda.device_count() > 1
+
+
+def _together(stream, *tensors):
+    """Refuses tensors on another device than the one that a call on this stream runs on (a number as the stream does not say)"""
+    if _many_devices:
+        device = torch._C._cuda_getDevice() if stream is None else getattr(stream, "device_index", None)
+        if device is not None and any(t is not None and t.get_device() not in (-1, device) for t in tensors):
+            raise ValueError("a tensor is on another device than device %d, which the call runs on" % device)
+
+
 def _stream_of(stream):
     """The torch stream that a call's argument stands for"""
     if stream is None:
@@ -243,6 +255,7 @@ class Rotary(_OnStream):
 
     def apply(self, q, k, positions, out=None, stream=None):
         """(q, k) turned, [tokens, heads, dim] each, into out = (q, k), which may be q and k themselves; k may be None."""
+        _together(stream, self.turns, q, k, positions, *(out or ()))
         on = self._on(stream)
         if k is not None and (k.dtype is not q.dtype or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]):
             raise ValueError("q [tokens, heads, dim] and k [tokens, kv heads, dim] of one type are wanted")
@@ -302,12 +315,14 @@ class PageTable(_OnStream):
 
     def fork(self, parents, stream=None):
         """Sequence s takes over the tokens of sequence parents[s] (int32 [sequences]; -1: none) as they were before, on the same pages."""
+        _together(stream, self.table, parents)
         at, on = _index(parents, torch.int32, self.desc.seqs, "parents"), self._on(stream)
         _check(self._fork(self._ref, at, on), "abq_kv_pages_fork")
 
     def extend(self, counts, rows, out=None, stream=None):
         """Room for counts[s] more tokens in sequence s (int32 [sequences]), or counts[s] < 0 taken away.  Returns an Extension, a new one or
         out, which an earlier call with as many rows has given."""
+        _together(stream, self.table, counts, None if out is None else out.whole)
         at, on = _index(counts, torch.int32, self.desc.seqs, "counts"), self._on(stream)
         if out is None:
             out = Extension(rows, self.desc.seqs, self._made(rows + 4 * self.desc.seqs + 1, stream))
@@ -318,6 +333,7 @@ class PageTable(_OnStream):
 
     def compact(self, out=None, stream=None):
         """Moves the live pages to the front; returns (or fills out with) moves [num_pages // 2, 2] for KvCache.copy_pages of every layer."""
+        _together(stream, self.table, out)
         on, half = self._on(stream), self.desc.num_pages // 2
         out = self._made(2 * half, stream).view(half, 2) if out is None else out
         _check(lib().abq_kv_pages_compact(self._ref, _index(out, torch.int32, 2 * half, "moves"), on), "abq_kv_pages_compact")
@@ -399,6 +415,7 @@ class KvCache(_OnStream):
         for x, y in ((q, q_out), (k, k_out)):
             if y is not None and (x is None or x.shape != y.shape or y.dtype is not dtype):
                 raise ValueError("q_out and k_out have to be of the inputs' shapes and type")
+        _together(stream, self.k_codes, rotary.turns, q, k, v, q_out, k_out, positions, slots)
         at, on = _index(slots, torch.int32, shape[0], "slots"), self._on(stream)
         if on.value not in rotary._memory.known:
             rotary._memory.use(stream)
@@ -413,6 +430,7 @@ class KvCache(_OnStream):
         """Copies page pairs[i, 0] to page pairs[i, 1] (int32 [n, 2]; -1: nothing), bounds included."""
         if pairs.dim() != 2 or pairs.shape[1] != 2:
             raise ValueError("pairs of pages [n, 2] are wanted")
+        _together(stream, self.k_codes, pairs)
         at, on = _index(pairs, torch.int32, pairs.numel(), "pairs"), self._on(stream)
         _check(lib().abq_kv_copy_pages(self._ref, self._bounds, at, pairs.shape[0], on), "abq_kv_copy_pages")
 
@@ -420,6 +438,7 @@ class KvCache(_OnStream):
         """Writes the bounds of the pages that these slots complete: behind an append, with its slots."""
         if self.bounds is None:
             raise ValueError("this cache has no bounds")
+        _together(stream, self.k_codes, slots)
         at, on = _index(slots, torch.int32, slots.numel(), "slots"), self._on(stream)
         _check(lib().abq_kv_bound(self._ref, self._bounds, at, slots.numel(), on), "abq_kv_bound")
 
@@ -515,7 +534,8 @@ class TreeAttention(_Attention):
 class SparseAttention(_Attention):
     """Attention of drafted tokens as TreeAttention's, but every draft and key head sees only `count` of the context's complete pages, and what
     stands behind them: the first `first`, the last `last`, and those whose bounds promise the largest scores for its queries.  Each pass
-    chooses them anew into blocks, int32 [drafts, kv heads, count]; with blocks given, those are seen and nothing is chosen."""
+    chooses them anew into blocks, int32 [drafts, kv heads, count]; with blocks given, those are seen and nothing is chosen.  Passes on
+    two streams at once need an object each."""
 
     _calls = ("abq_attn_sparse_workspace_bytes", "abq_attn_sparse_set_workspace", "abq_attn_sparse_exec")
 
@@ -543,6 +563,7 @@ class SparseAttention(_Attention):
         table = _index(page_table, torch.int32, seqs * page_table.shape[-1], "page_table")
         at = [_index(blocks, torch.int32, q.shape[0] * d.kv_heads * count, "blocks"), _index(context, torch.int32, seqs, "context"),
               _index(q_starts, torch.int32, seqs + 1, "q_starts")]
+        _together(None, cache.k_codes, q, out, page_table, context, q_starts, mask, blocks, workspace)
         self.held = (q, cache, page_table, context, q_starts, mask, blocks)
         self.state = SparseState()
         _check(lib().abq_attn_sparse_init(ctypes.byref(d), ctypes.byref(rows[0]), ctypes.byref(rows[1]), _dtype(q), q.shape[1], table, page_table.shape[-1],
@@ -560,6 +581,7 @@ class SparseAttention(_Attention):
 
     def run(self, stream=None):
         """One pass over what the tensors hold now; returns out.  A graph that captures it needs the object for as long as it is replayed."""
+        _together(stream, self.out)
         if self._choose:
             on = abq_gemm._stream_ptr(stream)
             if on.value not in self._known:

@@ -269,6 +269,54 @@ def test_memory_of_the_objects_is_safe_on_other_streams(attn, monkeypatch):
         table.extend(parents, 6, out=given, stream=other)
 
 
+def test_tensors_on_another_device_are_refused(attn, monkeypatch):
+    """Every call's tensors are on the device that its stream is of; with one device nothing is looked up"""
+    torch = attn.torch
+
+    class Fake(torch.Tensor):  # a CPU tensor that says it is on a device: no launch is made
+        is_cuda, on = True, 0
+
+        def get_device(self):
+            return self.on
+
+    def fake(on, *shape, dtype=torch.int32):
+        t = torch.zeros(shape, dtype=dtype).as_subclass(Fake)
+        t.on = on
+        return t
+    StreamsOfHand(torch, monkeypatch)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    half = torch.float16
+
+    def objects(on):
+        r, t, c = (kind.__new__(kind) for kind in (attn.Rotary, attn.PageTable, attn.KvCache))
+        r.turns, r.axes, t.table, t.desc = fake(on, 8, dtype=torch.float64), 1, fake(on, 2, 3), attn.KvPagesDesc(2, 3, 16, 8, None, None, None)
+        c.k_codes, c.desc, c._row, c.bounds = fake(on, 1), cache_desc(attn, head_dim=64), (2, 64), True
+        return r, t, c
+
+    def calls(r, t, c, x, stream):
+        """x: what each call's tensors are made by"""
+        rows = lambda: x(5, 2, 64, dtype=half)  # noqa: E731
+        return (lambda: r.apply(rows(), rows(), x(5), stream=stream), lambda: t.fork(x(2), stream=stream), lambda: t.extend(x(2), 4, stream=stream),
+                lambda: t.compact(x(4, 2), stream=stream), lambda: c.copy_pages(x(3, 2), stream=stream), lambda: c.bound(x(3), stream=stream),
+                lambda: c.append_rotated(r, rows(), rows(), rows(), x(5), x(5), q_out=rows(), stream=stream),
+                lambda: attn.SparseAttention(rows(), c, x(2, 9), x(2), x(3), 2, 100, 4, out=rows(), blocks=x(5, 2, 4)))
+    on_second = type("Stream", (), {"device_index": 1, "cuda_stream": 0x30})()
+    for many, objects_on, x_on, stream in ((True, 1, 0, None), (True, 0, 1, None), (True, 1, 1, None), (True, 0, 0, on_second), (True, 0, 1, on_second)):
+        monkeypatch.setattr(attn, "_many_devices", many)
+        made = calls(*objects(objects_on), lambda *shape, **kw: fake(x_on, *shape, **kw), stream)
+        for call in made[:-1] if stream else made:
+            with pytest.raises(ValueError, match="another device"):
+                call()
+    call = attn.SparseAttention.__new__(attn.SparseAttention)
+    call.out, call._choose = fake(1, 3), True
+    with pytest.raises(ValueError, match="another device"):
+        call.run()
+    for stream, tensors in ((None, [fake(0, 1), None, fake(0, 1)]), (on_second, [fake(1, 1)]), (0x30, [fake(1, 1), fake(0, 1)])):
+        attn._together(stream, *tensors)
+    monkeypatch.setattr(attn, "_many_devices", False)
+    attn._together(None, fake(1, 1))
+
+
 def test_launches_stay_within_the_threads_that_hip_counts(attn, tmp_path):
     """Grid times workgroup of every launch below 2^32, and within what a launch may hold of LDS, at the largest sizes that are taken"""
     from decoding_launch_probe import launches
