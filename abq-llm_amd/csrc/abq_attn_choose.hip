@@ -6,12 +6,14 @@
 // matrix cores (16 x 16 x 64), exact in whole numbers: the choice is the same whatever the order of sums.
 //
 // Bounds are as many bytes as 2 tokens' keys, so reading them is little; what a choice takes is a chain: pages, bounds and query
-// from memory 5 us (128 units of 512 pages, 17 MB), scores 1, three to six turns of the search for the threshold 0.6 each, the list 0.9,
-// and the launch.  One query for each of 16 x 8 heads and 512 pages 11.6 us, for 8 heads and 1500 pages 12.2 in two launches.
+// from memory 5 us (128 units of 512 pages, 17 MB), scores 1, the keys' range and one to four turns of the search for the threshold 0.6
+// each, the list 0.9, and the launch.  One query for each of 16 x 8 heads and 512 pages 11.2 us, for 8 heads and 1500 pages 12.2 in two launches.
 // Bounds are written at 4.4 TB/s where there are many (256 pages of 64 tokens and 32 heads, 69 MB, 15.8 us); sixteen sequences that all end a
 // page take 4.2 us, a call that ends none 2.
 #include "abq_decoding.h"
 #include "abq_quant.h"
+
+#include <type_traits>
 
 namespace abq {
 
@@ -165,6 +167,21 @@ template <int CTRL> __device__ __forceinline__ float add_dpp(float x)
 // over the 16 lanes of a row: neighbours, pairs, mirrored halves, the other eight
 __device__ __forceinline__ float sum_of_row(float x) { return add_dpp<0x128>(add_dpp<0x141>(add_dpp<0x4e>(add_dpp<0xb1>(x)))); }
 
+template <int CTRL> __device__ __forceinline__ uint32_t most_dpp(uint32_t x)
+{
+    return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ uint32_t most_of_row(uint32_t x) { return most_dpp<0x128>(most_dpp<0x141>(most_dpp<0x4e>(most_dpp<0xb1>(x)))); }
+// over a wave, as a scalar
+__device__ __forceinline__ uint32_t most_of_wave(uint32_t x)
+{
+    x = most_of_row(x);
+    const auto rows = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = max(rows[0], rows[1]);
+    const auto halves = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return __builtin_amdgcn_readfirstlane(max(halves[0], halves[1]));
+}
+
 // Floats as unsigned numbers of the same order, none of them 0, and back
 __device__ __forceinline__ uint32_t ordered(float x)
 {
@@ -213,11 +230,11 @@ template <int D, int COUNT> struct Tiles {
     __device__ __forceinline__ bool in_cache(const ChooseArgs &a, int i) const { return (uint32_t)page[i] < (uint32_t)a.c.num_pages; }
 };
 
-// Sixteen rows of queries as the product takes them, in LDS: what is positive of their codes, what is negative (padded against bank conflicts),
+// Rows of queries as the product takes sixteen of them, in LDS: what is positive of their codes, what is negative (padded against bank conflicts),
 // and their scales.  A wave quantises a row: what every wave would do for itself otherwise is most of the kernel's time.
-template <int D> struct Rows16 {
-    __align__(16) int8_t codes[2][16][D + 16];
-    float scales[16];
+template <int D, int ROWS = 16> struct Rows {
+    __align__(16) int8_t codes[2][ROWS][D + 16];
+    float scales[ROWS];
 
     // rows[i] goes to row i0 + i * step; NULL: it stays as it is
     template <int N> __device__ __forceinline__ void quantise(const uint16_t *const (&rows)[N], int i0, int step, int dtype)
@@ -247,18 +264,18 @@ template <int D> struct Rows16 {
                 scales[i0 + i * step] = q.scale;
         }
     }
-    // lane (t, g): the channels 64 j + 16 g .. + 15 of row t, and the scales of rows 4 g .. 4 g + 3, whose sums it gets
-    __device__ __forceinline__ void read(int4v (&up)[D / 64], int4v (&down)[D / 64], float (&scale)[4]) const
+    // Of sixteen from row r on, lane (t, g): the channels 64 j + 16 g .. + 15 of row t, and the scales of rows 4 g .. 4 g + 3, whose sums it gets
+    __device__ __forceinline__ void read(int r, int4v (&up)[D / 64], int4v (&down)[D / 64], float (&scale)[4]) const
     {
         const int t = threadIdx.x & 15, g = threadIdx.x >> 4 & 3;
 #pragma unroll
         for (int j = 0; j < D / 64; ++j) {
-            up[j] = *(const int4v *)&codes[0][t][64 * j + 16 * g];
-            down[j] = *(const int4v *)&codes[1][t][64 * j + 16 * g];
+            up[j] = *(const int4v *)&codes[0][r + t][64 * j + 16 * g];
+            down[j] = *(const int4v *)&codes[1][r + t][64 * j + 16 * g];
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            scale[i] = scales[4 * g + i];
+            scale[i] = scales[r + 4 * g + i];
     }
 };
 
@@ -287,7 +304,7 @@ __device__ __forceinline__ int complete_pages(const ChooseArgs &a, int seq) { re
 // Scores of all pages of a query row into LDS, by a workgroup
 template <int D, int WAVES> __device__ __forceinline__ void score_pages(const ChooseArgs &a, const ChooseUnit &u, uint32_t *keys)
 {
-    __shared__ Rows16<D> rows;
+    __shared__ Rows<D> rows;
     using T = Tiles<D, 4>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = lane & 15, g = lane >> 4;
     const int32_t *pages = a.page_table + (int64_t)u.seq * a.max_pages;
@@ -309,7 +326,7 @@ template <int D, int WAVES> __device__ __forceinline__ void score_pages(const Ch
         __syncthreads();
         int4v up[D / 64], down[D / 64];
         float scale[4];
-        rows.read(up, down, scale);
+        rows.read(0, up, down, scale);
         for (int p0 = 16 * wave; p0 < n; p0 += kRound) {
             if (p0 >= kRound || h0 > 0) { // (else they are there)
                 tiles.ask_pages(a, pages, p0, kStep);
@@ -343,16 +360,34 @@ template <int D, int WAVES> __device__ __forceinline__ void score_pages(const Ch
 template <int WAVES> __device__ __forceinline__ void write_largest(const uint32_t *keys, int n, int want, int32_t *out)
 {
     __shared__ uint32_t in_wave[2][8][16];
+    __shared__ uint2 ends[4][16];
     constexpr int kThreads = 64 * WAVES;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = lane & 15, g = lane >> 4;
+    const int rounded = (n + kThreads - 1) / kThreads * kThreads;
+    const uint32_t first = threadIdx.x < n ? keys[threadIdx.x] : 0, second = threadIdx.x + kThreads < n ? keys[threadIdx.x + kThreads] : 0;
+    // The least key and the largest of pages that are not chosen anyway: the former is among what `want` reach, and so much of the keys' bits is
+    // the same in all: 125 pages of scores between 100 and 300 take 6.9 us, 8.4 from the keys' first bit on.  (Complements, and sums that wrap around, make both a largest one, and nothing of a key that is passed over.)
+    uint32_t from = 0, to = 0;
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const uint32_t key = i < kThreads ? first : i < 2 * kThreads ? second : keys[i];
+        from = max(from, ~key);
+        to = max(to, key + 1);
+    }
+    from = most_of_row(from);
+    to = most_of_row(to);
+    if (t == 0)
+        ends[g][wave] = uint2{from, to};
+    __syncthreads();
+    const uint2 end = t < WAVES ? ends[g][t] : uint2{0, 0};
+    from = ~most_of_wave(end.x);
+    to = most_of_wave(end.y) - 1;
     // The largest number that at least `want` keys reach, three bits at a time; `exact`: reached by no more than those.  Each wave counts its
     // own keys; then lane (w, j) of every wave has wave w's count of those that reach the j-th of seven numbers, so that a turn is one
     // write, one barrier and one read, and what follows from it is the same in all waves.
-    uint32_t least = 0;
+    uint32_t least = from;
     bool exact = false;
-    const int rounded = (n + kThreads - 1) / kThreads * kThreads;
-    const uint32_t first = threadIdx.x < n ? keys[threadIdx.x] : 0, second = threadIdx.x + kThreads < n ? keys[threadIdx.x + kThreads] : 0;
-    for (int shift = 30, round = 0; shift >= 0 && !exact; shift -= 3, ++round) {
+    for (int bits = to > from ? 32 - __builtin_clz(to - from) : 0, round = 0; bits > 0 && !exact; bits -= 3, ++round) {
+        const int shift = max(bits - 3, 0);
         uint32_t count[7] = {};
         auto tally = [&](uint32_t key) {
             const uint32_t digit = key >= least ? (key - least) >> shift : 0;
@@ -448,12 +483,14 @@ template <int D, int WAVES, bool SCORED> __global__ __launch_bounds__(64 * WAVES
 // The scores alone, a workgroup for kScorePages pages of a sequence and key head and for some of the sequence's drafts, whose rows it goes over
 // with the bounds in registers.  Rows of all its drafts' heads fill the product's sixteen; each goes into its draft's largest.
 constexpr int kScoreWaves = 4, kScoreTiles = 2, kScorePages = 16 * kScoreWaves * kScoreTiles;
-// 32 rows of queries a workgroup: more of them in turn take longer than reading the bounds again
-constexpr int score_drafts(int group) { return group >= 32 ? 1 : 32 / group; }
+// 32 rows of queries a workgroup, quantised at once (7 x 5 drafts of 4 heads, 1250 pages 20.7 us, sixteen and sixteen 21.7; 16 x 5 28.4 and 32.3):
+// more of them in turn take longer than reading the bounds again
+constexpr int kScoreRows = 32;
+constexpr int score_drafts(int group) { return group >= kScoreRows ? 1 : kScoreRows / group; }
 
 template <int D> __global__ __launch_bounds__(64 * kScoreWaves) void attn_score_kernel(ChooseArgs a, uint32_t *scored)
 {
-    __shared__ Rows16<D> rows;
+    __shared__ Rows<D, kScoreRows> rows;
     __shared__ uint32_t keys[score_drafts(1)][kScorePages];
     __shared__ float scales[kScorePages]; // of bounds; -inf: the page is not in the cache
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = lane & 15, g = lane >> 4;
@@ -475,19 +512,27 @@ template <int D> __global__ __launch_bounds__(64 * kScoreWaves) void attn_score_
         for (int i = threadIdx.x; i < some * kScorePages; i += 64 * kScoreWaves)
             (&keys[0][0])[i] = 0;
     for (int r0 = 0; r0 < count; r0 += 16) {
-        if (r0 > 0)
-            __syncthreads();
-        const uint16_t *row[16 / kScoreWaves];
+        if (r0 % kScoreRows == 0) {
+            if (r0 > 0)
+                __syncthreads();
+            auto quantise = [&](auto n) { // (half as many loads and branches where there are no more rows: 8 x 8000 pages 25 us, 27 without)
+                const uint16_t *row[decltype(n)::value];
 #pragma unroll
-        for (int i = 0; i < 16 / kScoreWaves; ++i) {
-            const int r = r0 + kScoreWaves * i + wave;
-            row[i] = r < count ? (const uint16_t *)a.q.data + (own.first + d0 + r / a.group) * a.q.row_stride + (int64_t)(head * a.group + r % a.group) * a.q.head_stride : nullptr;
+                for (int i = 0; i < decltype(n)::value; ++i) {
+                    const int r = r0 + kScoreWaves * i + wave;
+                    row[i] = r < count ? (const uint16_t *)a.q.data + (own.first + d0 + r / a.group) * a.q.row_stride + (int64_t)(head * a.group + r % a.group) * a.q.head_stride : nullptr;
+                }
+                rows.quantise(row, wave, kScoreWaves, a.dtype);
+            };
+            if (count - r0 <= 16)
+                quantise(std::integral_constant<int, 16 / kScoreWaves>());
+            else
+                quantise(std::integral_constant<int, kScoreRows / kScoreWaves>());
+            __syncthreads();
         }
-        rows.quantise(row, wave, kScoreWaves, a.dtype);
-        __syncthreads();
         int4v up[D / 64], down[D / 64];
         float scale[4];
-        rows.read(up, down, scale);
+        rows.read(r0 % kScoreRows, up, down, scale);
         int draft[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -576,17 +621,17 @@ template <int D> static hipError_t choose(const ChooseArgs &a, int64_t units, in
         return likely <= 1024 || units > 64 ? choose<D, 8, true>(a, scored, units, stream) : choose<D, 16, true>(a, scored, units, stream);
     }
     // Waves: enough to score all pages in a round of 64 a wave, but no more than leave two (eight waves) or four workgroups to a compute unit
-    // where there are more of these than units.  128 channels, us with 4, 8, 16 waves: 32 of 125 pages 7.6, 7.9, 9.3; 128 of 512 13.9, 13.4, 14.3;
-    // 256 of 1200 29, 25, 23; 280 of 1250 34, 30, 37; 512 of 1200 43, 38, 46; 2048 of 1000 82, 90, 133
+    // where there are more of these than units.  128 channels, us with 4, 8, 16 waves: 32 of 125 pages 6.9, 7.0, 8.1; 128 of 512 12.3, 11.2, 12.3;
+    // 256 of 1200 27, 23.4, 22.7; 280 of 1250 32, 28, 35; 512 of 1200 43, 38, 45; 2048 of 1000 81, 88, 128
     if (likely <= 256 || units > 512)
         return choose<D, 4, false>(a, nullptr, units, stream);
     return likely <= 512 || units > 256 ? choose<D, 8, false>(a, nullptr, units, stream) : choose<D, 16, false>(a, nullptr, units, stream);
 }
 
 // A launch of their own for the scores: where few workgroups would each have many pages, and where several drafts share a sequence's bounds.
-// us in one launch and in two, one draft: 8 units of 600 pages 12.0 and 10.6, of 1500 20.7 and 12.2, of 8000 82 and 27; 64 of 1500 22 and 16.5;
-// but 8 of 300 9.3 and 10.3, 128 of 1200 20.6 and 21.2, 256 of 1200 23.6 and 28.  Drafts: 7 x 5 of 8 heads, 600 pages 18.8 and 17.8, 1250
-// 29.5 and 23.4; 64 of 32 heads, 600 pages 53 and 33; but 7 x 5 of 300 pages 13.4 and 15.6.
+// us in one launch and in two, one draft: 8 units of 600 pages 11.9 and 10.5, of 1500 20.5 and 12.2, of 8000 80 and 25; 64 of 1500 21 and 16;
+// but 8 of 300 8.5 and 10, 128 of 1200 19.9 either way.  Drafts: 7 x 5 of 8 heads, 600 pages 17.9 and 16.5, 1250 28.7 and 20.7; 64 of 32
+// heads, 600 pages 52 and 31.7; but 2 x 27 of 8 heads, 600 pages 18.5 and 18.9.
 size_t choose_workspace_bytes(int seqs, int max_q, int kv_heads, int max_pages, int likely)
 {
     const double units = (double)seqs * max_q * kv_heads, blocks = units * ((max_pages + kScorePages - 1) / kScorePages);
