@@ -255,7 +255,7 @@ abq_status abq_attn_sparse_init(const abq_kv_cache *cache, const abq_rows *q, co
     abq_status s = abq_attn_tree_init(cache, q, out, dtype, heads, page_table, max_pages, context, q_starts, mask, seqs, max_q, max_context, scale, &st.attn);
     if (s != ABQ_OK)
         return s;
-    if (!blocks || count <= 0)
+    if ((q->rows && !blocks) || count <= 0)
         return ABQ_ERR_INVALID_ARG;
     if (count > kMostChosen || product(product(seqs, max_q, cache->kv_heads) + 8, (heads / cache->kv_heads + 15) / 16, 1) > kMostThreads / 512)
         return ABQ_ERR_TOO_LARGE;
