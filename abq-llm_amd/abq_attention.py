@@ -533,19 +533,21 @@ class TreeAttention(_Attention):
 
 class SparseAttention(_Attention):
     """Attention of drafted tokens as TreeAttention's, but every draft and key head sees only `count` of the context's complete pages, and what
-    stands behind them: the first `first`, the last `last`, and those whose bounds promise the largest scores for its queries.  Each pass
-    chooses them anew into blocks, int32 [drafts, kv heads, count]; with blocks given, those are seen and nothing is chosen.  Passes on
-    two streams at once need an object each."""
+    stands behind them: the first `first`, the last `last` (one each by default, as far as `count` has room, the last before the first), and
+    those whose bounds promise the largest scores for its queries.  Each pass chooses them anew into blocks, int32 [drafts, kv heads, count];
+    with blocks given, those are seen and nothing is chosen.  Passes on two streams at once need an object each."""
 
     _calls = ("abq_attn_sparse_workspace_bytes", "abq_attn_sparse_set_workspace", "abq_attn_sparse_exec")
 
-    def __init__(self, q, cache, page_table, context, q_starts, max_q, max_context, count, first=1, last=1, mask=None, scale=None, out=None, workspace=None,
+    def __init__(self, q, cache, page_table, context, q_starts, max_q, max_context, count, first=None, last=None, mask=None, scale=None, out=None, workspace=None,
                  blocks=None):
         d = cache.desc
         if q.dim() != 3 or q.shape[2] != d.head_dim:
             raise ValueError("q [drafts, heads, %d] is wanted" % d.head_dim)
         if blocks is None and cache.bounds is None:
             raise ValueError("this cache has no bounds to choose pages by")
+        last = min(1, max(0, count - (first or 0))) if last is None else last
+        first = min(1, max(0, count - last)) if first is None else first
         if count < 1 or min(first, last) < 0 or first + last > count:
             raise ValueError("count >= first + last pages, one at least, are wanted")
         made = ()

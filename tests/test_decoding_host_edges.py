@@ -5,7 +5,7 @@ pytest.importorskip("torch")
 
 from attention_reference import load_abq_attention  # noqa: E402
 from test_decoding_host import ref, sparse  # noqa: E402
-from test_attention_host import A  # noqa: E402
+from test_attention_host import A, StreamsOfHand, cache_desc  # noqa: E402
 
 
 @pytest.fixture(scope="module")
@@ -23,3 +23,35 @@ def test_attention_to_chosen_pages_without_drafts(attn):
     for kw in ({"count": 0}, {"blocks": None}, {"blocks": None, "q": {"rows": 0}}):
         assert sparse(attn, **kw)[0] == ok.ABQ_ERR_INVALID_ARG, kw
     assert sparse(attn, blocks=A)[0] == ok.ABQ_OK
+
+
+def on_no_device(torch):
+    class Fake(torch.Tensor):  # a CPU tensor that says it is on the device: no launch is made
+        is_cuda = True
+    return lambda *shape, dtype=torch.int32: torch.zeros(shape, dtype=dtype).as_subclass(Fake)
+
+
+def test_one_chosen_page(attn, monkeypatch):
+    """Unless it is said otherwise one page from either end is chosen in any case, as far as there is room for it, the last one first"""
+    torch = attn.torch
+    StreamsOfHand(torch, monkeypatch)
+    monkeypatch.setattr(attn, "_rows", lambda t: attn.Rows(t.data_ptr(), t.shape[0], t.stride(0), t.stride(1)))
+    fake = on_no_device(torch)
+    cache = attn.KvCache.__new__(attn.KvCache)
+    cache.desc, cache._memory = cache_desc(attn, head_dim=64), attn._Memory(())
+    cache.bounds, cache._bounds, cache.k_codes = True, None, fake(1)
+    full = torch.full
+    monkeypatch.setattr(torch, "full", lambda *a, device=None, **kw: full(*a, **kw).as_subclass(type(fake(1))))
+    aligned = torch.zeros(2 * 3 * 4 * 64 + 64, dtype=torch.float16).as_subclass(type(fake(1)))
+    at = -aligned.data_ptr() // 2 % 8
+    q, out = (aligned[at + i * 768:at + (i + 1) * 768].view(3, 4, 64) for i in range(2))
+
+    def forced(**kw):
+        call = attn.SparseAttention(q, cache, fake(2, 9), fake(2), fake(3), 2, 100, out=out, workspace=fake(0), **kw)
+        return call._chosen[-6:-4], call.blocks.shape
+    assert forced(count=1) == ((0, 1), (3, 2, 1)) and forced(count=2) == ((1, 1), (3, 2, 2)) and forced(count=9) == ((1, 1), (3, 2, 9))
+    assert forced(count=1, first=1)[0] == (1, 0) and forced(count=1, first=0, last=0)[0] == (0, 0) and forced(count=3, first=0)[0] == (0, 1)
+    assert forced(count=3, first=3)[0] == (3, 0) and forced(count=3, last=2)[0] == (1, 2) and forced(count=3, last=3)[0] == (0, 3)
+    for kw in ({"count": 1, "first": 1, "last": 1}, {"count": 2, "first": 3}, {"count": 2, "last": 3}, {"count": 3, "last": -1}, {"count": 3, "first": -1}, {"count": 0}):
+        with pytest.raises(ValueError):
+            forced(**kw)
