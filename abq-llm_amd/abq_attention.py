@@ -227,8 +227,8 @@ class Rotary(_OnStream):
             axes = axes or int(axis.max()) + 1
             if int(axis.max()) >= axes:
                 raise ValueError("there are %d axes" % axes)
-        self.turns, self.axes = turns.to(device).contiguous(), axes or 1
-        self.axis = None if axis is None else axis.to(device).contiguous()
+        self.turns, self.axes = turns.to(device, copy=True).contiguous(), axes or 1  # (what is there already as well)
+        self.axis = None if axis is None else axis.to(device, copy=True).contiguous()
         self.desc = RotaryDesc(2 * turns.numel(), self.axes, int(bool(interleaved)), self.turns.data_ptr(), None if axis is None else self.axis.data_ptr())
         self._ref = ctypes.byref(self.desc)
         self._memory = _Memory(tuple(t for t in (self.turns, self.axis) if t is not None))

@@ -55,3 +55,27 @@ def test_one_chosen_page(attn, monkeypatch):
     for kw in ({"count": 1, "first": 1, "last": 1}, {"count": 2, "first": 3}, {"count": 2, "last": 3}, {"count": 3, "last": -1}, {"count": 3, "first": -1}, {"count": 0}):
         with pytest.raises(ValueError):
             forced(**kw)
+
+
+def test_angles_are_the_objects_own(attn, monkeypatch):
+    """Angles and axes that are on the device already, in the type that is wanted, are copied as all others are"""
+    torch = attn.torch
+    StreamsOfHand(torch, monkeypatch)
+    moved = torch.Tensor.to
+
+    def to(t, *a, copy=False, **kw):  # (what is here is on the device already)
+        if a == ("cuda",) or str(kw.get("device")) == "cuda":
+            a, kw = (), {k: v for k, v in kw.items() if k != "device"}
+            return t.clone() if copy else moved(t, **kw) if kw else t
+        return moved(t, *a, copy=copy, **kw)
+    monkeypatch.setattr(torch.Tensor, "to", to)
+    turns, axis = torch.arange(8, dtype=torch.float64), torch.tensor([0, 1] * 4, dtype=torch.int32)
+    for given in (turns, turns.numpy(), torch.stack([turns, turns], 1)[:, 0]):
+        r = attn.Rotary(given, axis)
+        before = r.turns.clone(), r.axis.clone()
+        given *= 2
+        axis.mul_(0)
+        assert torch.equal(r.turns, before[0]) and torch.equal(r.axis, before[1]) and r.turns.is_contiguous()
+        assert (r.desc.turns, r.desc.axis) == (r.turns.data_ptr(), r.axis.data_ptr()) and r.desc.rotary_dim == 16
+        given /= 2
+        axis.copy_(before[1])
