@@ -601,8 +601,11 @@ hipError_t launch_kv_bound(const abq_kv_cache &c, const abq_kv_bounds &bounds, c
 template <int D, int WAVES, bool SCORED> static hipError_t choose(const ChooseArgs &a, const uint32_t *scored, int64_t units, hipStream_t stream)
 {
     const size_t lds = sizeof(uint32_t) * a.max_pages;
-    if (lds > 48 << 10) { // (beyond what a launch gets unasked)
-        const hipError_t e = hipFuncSetAttribute((const void *)attn_choose_kernel<D, WAVES, SCORED>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    // A launch gets 64 KB unasked, of which the kernel's own arrays may take 7.  The limit is the process's: the same one each time, so that
+    // no call lowers it between another thread's asking and its launch.
+    if (lds > 48 << 10) {
+        const hipError_t e = hipFuncSetAttribute((const void *)attn_choose_kernel<D, WAVES, SCORED>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                 (int)sizeof(uint32_t) * kMostChosen);
         if (e != hipSuccess)
             return e;
     }

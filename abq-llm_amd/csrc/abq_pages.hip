@@ -427,7 +427,7 @@ PagesArgs pages_args(const abq_kv_pages &p)
 
 hipError_t launch_pages_fork(const abq_kv_pages &p, const int32_t *parents, hipStream_t stream)
 {
-    // four columns a workgroup, where 64 KB hold them: enough workgroups for the tables of many sequences, 16 bytes a row
+    // four columns a workgroup, where the 64 KB that a launch gets unasked hold them: enough workgroups for the tables of many sequences, 16 bytes a row
     const int shift = p.seqs <= 4096 ? 2 : 1, columns = 1 << shift;
     const dim3 grid((unsigned)((p.max_pages + columns - 1) / columns + 1));
     hipLaunchKernelGGL(pages_fork_kernel, grid, dim3(1024), sizeof(int32_t) * p.seqs << shift, stream, pages_args(p), parents, columns, shift);
