@@ -2,7 +2,8 @@
 // The formulas are those stated in abq_attention.h.
 //
 // A page's keys k of a channel lie between lo and hi, so q k <= max(q, 0) hi + min(q, 0) lo in that channel, and the sum over the channels is at
-// least the score of any of its tokens.  With hi and lo beside each other that is one product of 2 head_dim numbers, in 8 bits on the
+// least the score of any of its tokens (a published method: J. Tang et al., "Query-Aware Sparsity for Efficient Long-Context LLM Inference",
+// ICML 2024).  With hi and lo beside each other that is one product of 2 head_dim numbers, in 8 bits on the
 // matrix cores (16 x 16 x 64), exact in whole numbers: the choice is the same whatever the order of sums.
 //
 // Bounds are as many bytes as 2 tokens' keys, so reading them is little; what a choice takes is a chain: pages, bounds and query

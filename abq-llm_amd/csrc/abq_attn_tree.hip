@@ -29,7 +29,9 @@
 //
 // With lists of pages (LISTED) every draft has rows of its own, those of one key head's group.  128 of them on 48 pages of 64 tokens of 8 bits,
 // 104 MB, 22.7 us with the join, 5.3 TB/s without; 280 of 4 rows on 1600 tokens of 4 bits, 25 us for 65 MB (and 26 for 118 of 8 bits), bound by the
-// vector work, which is the same for one row as for sixteen.
+// vector work, which is the same for one row as for sixteen and too much for so few workgroups; with 512 of them on 48 pages of 64 tokens 4 bits
+// take 49 us, 4.4 TB/s, and 8 bits 85.  Every wave looks for the end of its list by itself, from behind: a thousand entries that name
+// nothing cost 2.5 to 5 us.
 #include "abq_decoding.h"
 
 namespace abq {

@@ -133,7 +133,8 @@ abq_status abq_kv_pages_fork(const abq_kv_pages *pages, const int32_t *parents, 
 /* Gives sequence s room for counts[s] more tokens (device, [seqs]), or takes -counts[s] of its last tokens away.  Tokens to be written in a
  * page that other entries name as well go to a copy of it.  Pages that were free before the call are handed out lowest first, in the order of the
  * sequences, a copy's page before the further ones.  A sequence that would need more than max_pages is left as it is; so are the first
- * one for which the free pages do not suffice and those behind it that need any.  Device arrays, written whole:
+ * one for which the free pages do not suffice and those behind it that need any.  The search for free pages begins at the first page: a call
+ * that needs any takes the longer the more occupied ones lie in front of them.  Device arrays, written whole:
  *   starts  [seqs + 1]  where the sequences' new tokens begin, one behind the other: sums of the positive counts (as q_starts), at most 2^31 - 1
  *   granted [seqs]      counts[s], 0 for a sequence that was left as it was, -(tokens taken away)
  *   copies  [seqs][2]   pages (from, to) to be copied in every layer's cache before anything is written to it, or -1, -1
@@ -248,7 +249,7 @@ abq_status abq_attn_choose(const abq_kv_cache *cache, const abq_kv_bounds *bound
 
 /* Attention of drafted tokens as in abq_attn_tree_init, but of the context, row i and key head h see only the tokens of pages
  * blocks[i][h][0 .. count - 1] (numbers that are not those of complete pages of the context name none; a page that is named
- * twice counts twice) and those behind the last complete page.  count <= 32768. */
+ * twice counts twice) and those behind the last complete page.  count <= 32768, and best not much more than there are pages to name. */
 typedef struct abq_sparse_state {
     abq_attn_state attn;
     const int32_t *blocks;
