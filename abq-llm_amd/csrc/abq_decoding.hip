@@ -36,6 +36,13 @@ abq_status check_turned(const abq_rows *in, const abq_rows *out, int64_t rows, i
     return ABQ_OK;
 }
 
+// Whether results begin where other rows do, which other waves read or write: these lie on one another, whatever their strides
+bool begins_on(const abq_rows *out, const abq_rows *other) { return out && other && out->rows > 0 && out->data == other->data; }
+bool crossed(const abq_rows *q, const abq_rows *q_out, const abq_rows *k, const abq_rows *k_out)
+{
+    return begins_on(q_out, k) || begins_on(q_out, k_out) || begins_on(k_out, q);
+}
+
 // Workgroups of a launch that turns rows of these heads (and of one that quantises values beside it)
 abq_status check_turning(const RotaryCall &c, int64_t further)
 {
@@ -85,6 +92,8 @@ abq_status abq_rotary_apply(const abq_rotary *rotary, const abq_rows *q, const a
     if ((s = check_rotary(rotary, head_dim, positions, position_stride, q->rows)) != ABQ_OK ||
         (s = check_turned(q, q_out, q->rows, heads, head_dim)) != ABQ_OK || (k && (s = check_turned(k, k_out, q->rows, kv_heads, head_dim)) != ABQ_OK))
         return s;
+    if (k && crossed(q, q_out, k, k_out))
+        return ABQ_ERR_INVALID_ARG;
     RotaryCall c = {};
     c.rotary = *rotary;
     c.q = *q;
@@ -119,7 +128,7 @@ abq_status abq_kv_append_rotary(const abq_kv_cache *cache, const abq_rotary *rot
         (s = k_out ? check_turned(k, k_out, k->rows, cache->kv_heads, cache->head_dim) : check_rows(k, k->rows, cache->kv_heads, cache->head_dim)) != ABQ_OK ||
         (q && (s = check_turned(q, q_out, k->rows, heads, cache->head_dim)) != ABQ_OK))
         return s;
-    if (k->rows && (v->data == (k_out ? k_out->data : nullptr) || (q && v->data == q_out->data)))
+    if (begins_on(k_out, v) || begins_on(q_out, v) || crossed(q, q_out, k, k_out))
         return ABQ_ERR_INVALID_ARG;
     RotaryCall c = {};
     c.rotary = *rotary;

@@ -97,7 +97,7 @@ typedef struct abq_rotary {
 } abq_rotary;
 
 /* Turns rows of q into q_out and of k into k_out: into the same rows, in place, or others; but for that nothing that is written may
- * overlap anything else that is read or written.  k (and k_out) may be NULL.  positions: device int32, axis a of token i at
+ * overlap anything else that is read or written (results that begin where other rows do are refused).  k (and k_out) may be NULL.  positions: device int32, axis a of token i at
  * positions[a * position_stride + i]; position_stride >= the number of rows where there are several axes.  head_dim: a multiple of 16, at most 256. */
 abq_status abq_rotary_apply(const abq_rotary *rotary, const abq_rows *q, const abq_rows *q_out, int heads, const abq_rows *k, const abq_rows *k_out,
                             int kv_heads, int head_dim, int dtype, const int32_t *positions, int64_t position_stride, void *stream);

@@ -4,8 +4,8 @@ import pytest
 pytest.importorskip("torch")
 
 from attention_reference import load_abq_attention  # noqa: E402
-from test_decoding_host import ref, sparse  # noqa: E402
-from test_attention_host import A, StreamsOfHand, cache_desc  # noqa: E402
+from test_decoding_host import ref, rotary, sparse  # noqa: E402
+from test_attention_host import A, StreamsOfHand, cache_desc, rows  # noqa: E402
 
 
 @pytest.fixture(scope="module")
@@ -79,3 +79,28 @@ def test_angles_are_the_objects_own(attn, monkeypatch):
         assert (r.desc.turns, r.desc.axis) == (r.turns.data_ptr(), r.axis.data_ptr()) and r.desc.rotary_dim == 16
         given /= 2
         axis.copy_(before[1])
+
+
+def test_turned_rows_that_lie_on_other_rows_are_refused(attn):
+    """q_out on k, k_out on q, or both results on one place: waves would read what others have written"""
+    L, ok = attn.lib(), attn.abq_gemm
+    none = dict.fromkeys(("q", "q_out", "k", "k_out", "v"))
+    at = {"q": 8 * A, "q_out": 12 * A, "k": 16 * A, "k_out": 20 * A, "v": 24 * A}
+
+    def calls(count=12, **places):
+        r = {n: ref(None if p is None else rows(attn, data=p, rows=count)) for n, p in dict(at, **places).items()}
+        angles = ref(rotary(attn))
+        apply = L.abq_rotary_apply(angles, r["q"], r["q_out"], 2, r["k"], r["k_out"], 2, 128, 0, 6 * A, 12, None) if places.get("q", A) else None
+        return apply, L.abq_kv_append_rotary(ref(cache_desc(attn)), angles, r["q"], r["q_out"], 2, r["k"], r["k_out"], r["v"], 0, 6 * A, 12, 5 * A, None)
+    bad = ok.ABQ_ERR_INVALID_ARG
+    for places in ({"q_out": 16 * A}, {"k_out": 8 * A}, {"q_out": 20 * A}, {"q_out": 8 * A, "k_out": 8 * A}, {"q_out": 16 * A, "k_out": 8 * A}, {"q": 16 * A, "q_out": 16 * A}):
+        assert calls(**places) == (bad, bad), places
+    assert calls(q_out=16 * A, k_out=None)[1] == calls(q=None, q_out=None, k_out=24 * A)[1] == bad
+    empty = dict.fromkeys(none, 8 * A)  # no rows: nothing lies on anything
+    assert calls(count=0, **empty) == (ok.ABQ_OK, ok.ABQ_OK)
+
+
+def test_rows_may_be_turned_in_place(attn, tmp_path):
+    from decoding_launch_probe import launches
+    for r in launches(tmp_path, [("rotary", 5, 4, 4, 128), ("rotary", 5, 4, 0, 128), ("append", 5, 4, 4, 128)]):
+        assert r["status"] == 0 and len(r["launches"]) == 1
